@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI declared in include/b2g.h (the library `cs464_b200/libb2g.so`).
+"""ctypes binding of the C ABI declared in include/b2g.h and include/b2g_micro.h (the library `cs464_b200/libb2g.so`).
 
 There is no fallback: if the library is missing or fails to load, every GEMM entry point raises. The reference reaches
 its vendor comparator the same way (ctypes into libcublasLt, baselines/cublaslt.py:44-55).
@@ -34,6 +34,22 @@ EXPORTS = (
 )
 
 
+# every symbol include/b2g_micro.h declares
+MICRO_EXPORTS = (
+    "b2g_micro_layout", "b2g_micro_tensor_scale", "b2g_micro_quantize", "b2g_micro_dequantize", "b2g_micro_plan_create",
+    "b2g_micro_plan_launch", "b2g_micro_plan_destroy", "b2g_micro_matmul", "b2g_micro_rms_norm",
+    "b2g_micro_rms_norm_workspace", "b2g_micro_rms_norm_backward", "b2g_micro_silu_mul", "b2g_micro_silu_mul_backward",
+)
+
+VALUE_F16 = 0
+VALUE_BF16 = 1
+VALUE_F32 = 2
+
+FMT_MXFP8 = 1
+FMT_MXFP4 = 2
+FMT_NVFP4 = 3
+
+
 class Config(ctypes.Structure):
     _fields_ = [("block_m", ctypes.c_int32), ("block_n", ctypes.c_int32), ("block_k", ctypes.c_int32),
                 ("num_warps", ctypes.c_int32), ("num_stages", ctypes.c_int32), ("group_m", ctypes.c_int32),
@@ -47,6 +63,16 @@ class Problem(ctypes.Structure):
                 ("stride_bk", ctypes.c_int64), ("stride_bn", ctypes.c_int64),
                 ("stride_cm", ctypes.c_int64), ("stride_cn", ctypes.c_int64),
                 ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class MicroTensor(ctypes.Structure):
+    _fields_ = [("format", ctypes.c_int32), ("reserved", ctypes.c_int32), ("rows", ctypes.c_int64),
+                ("cols", ctypes.c_int64), ("codes", ctypes.c_void_p), ("pitch", ctypes.c_int64),
+                ("scales", ctypes.c_void_p), ("scale", ctypes.c_void_p)]
+
+
+class MicroMatrix(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("stride_r", ctypes.c_int64), ("stride_c", ctypes.c_int64)]
 
 
 class B2GError(RuntimeError):
@@ -98,6 +124,23 @@ def _declare(lib: ctypes.CDLL) -> None:
                                          c_int32, ctypes.c_double, c_void_p, ctypes.c_int64, c_int32, c_void_p,
                                          c_int32]),
     }
+    i64, mt, mm = ctypes.c_int64, P(MicroTensor), P(MicroMatrix)
+    sig.update({
+        "b2g_micro_layout": (c_int32, [c_int32, i64, i64, P(i64), P(i64)]),
+        "b2g_micro_tensor_scale": (c_int32, [mm, i64, i64, c_int32, c_void_p, c_void_p]),
+        "b2g_micro_quantize": (c_int32, [mm, c_int32, mt, c_void_p]),
+        "b2g_micro_dequantize": (c_int32, [mt, mm, c_int32, c_void_p]),
+        "b2g_micro_plan_create": (c_int32, [mt, mt, c_void_p, i64, c_int32, c_void_p, P(c_void_p)]),
+        "b2g_micro_plan_launch": (c_int32, [c_void_p, c_void_p]),
+        "b2g_micro_plan_destroy": (c_int32, [c_void_p]),
+        "b2g_micro_matmul": (c_int32, [mt, mt, c_void_p, i64, c_int32, c_void_p, c_void_p]),
+        "b2g_micro_rms_norm": (c_int32, [mm, mm, c_void_p, mm, mm, mt, i64, i64, ctypes.c_float, c_int32, c_void_p]),
+        "b2g_micro_rms_norm_workspace": (c_int32, [i64, i64, P(c_size_t)]),
+        "b2g_micro_rms_norm_backward": (c_int32, [mm, mm, c_void_p, mm, mm, c_void_p, c_void_p, c_size_t, i64, i64,
+                                                  ctypes.c_float, c_int32, c_void_p]),
+        "b2g_micro_silu_mul": (c_int32, [mm, mm, mt, i64, i64, c_int32, c_void_p]),
+        "b2g_micro_silu_mul_backward": (c_int32, [mm, mm, mm, i64, i64, c_int32, c_void_p]),
+    })
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
         fn.restype = res

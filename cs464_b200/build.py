@@ -4,8 +4,9 @@ The reference compiles each Triton config on first use (kernels/triton_matmul.py
 prebuilt-cubin bundle to hide it, kernels/bundle.py). Here the whole config space is one runtime-parameterised kernel,
 compiled once from source by this script; first-use compile cost is zero by construction.
 
-`python -m cs464_b200.build` rebuilds when any source or flag changed (the source hash is baked into the library and
-returned by `b2g_source_hash()`).
+`python -m cs464_b200.build` rebuilds when any source or flag changed. The GEMM family's source hash is baked into the
+library and returned by `b2g_source_hash()`: it covers what a stored config key compiles to (the b2g_* sources and b2g.h)
+and not the microscaled operators (the micro_* sources, b2g_micro.h), so that a change there leaves stored winners valid.
 """
 from __future__ import annotations
 
@@ -14,6 +15,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -29,15 +32,23 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
-def source_hash() -> str:
-    """sha256 (16 hex) of every CUDA source, header and build flag: what a stored config key compiles to."""
+def _hash(files: list[Path]) -> str:
     h = hashlib.sha256()
-    files = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
     for f in files:
         h.update(f.name.encode())
         h.update(f.read_bytes())
     h.update(" ".join(ARCH_FLAGS + NVCC_FLAGS).encode())
     return h.hexdigest()[:16]
+
+
+def source_hash() -> str:
+    """sha256 (16 hex) of the GEMM family's CUDA sources, headers and build flags: what a stored config key compiles to."""
+    return _hash(sorted(CSRC.glob("b2g_*.cu")) + sorted(CSRC.glob("b2g_*.cuh")) + [INCLUDE / "b2g.h"])
+
+
+def build_hash() -> str:
+    """The same of every source in the library: whether it is up to date."""
+    return _hash(sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h")))
 
 
 def nvcc() -> str:
@@ -52,28 +63,41 @@ def _stamp() -> Path:
 
 
 def up_to_date() -> bool:
-    return LIB_PATH.exists() and _stamp().exists() and _stamp().read_text().strip() == source_hash()
+    return LIB_PATH.exists() and _stamp().exists() and _stamp().read_text().strip() == build_hash()
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile the library for sm_100a unless it is already built from the current sources."""
     if not force and up_to_date():
         return LIB_PATH
-    digest = source_hash()
+    stamp = build_hash()
+    flags = [f for f in NVCC_FLAGS if f != "-shared"] + [f"-I{INCLUDE}", f"-I{CSRC}", f'-DB2G_SOURCE_HASH="{source_hash()}"']
+    if verbose:
+        flags.append("-Xptxas=-v")
+
+    def run(cmd: list[str]) -> str:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
+        return r.stderr
+
     tmp = LIB_PATH.with_suffix(f".so.tmp{os.getpid()}")
-    cmd = [nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", f'-DB2G_SOURCE_HASH="{digest}"',
-           *map(str, sources()), "-o", str(tmp)]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), file=sys.stderr)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
+    try:
+        with tempfile.TemporaryDirectory() as d:
+            objects = [str(Path(d) / (f.stem + ".o")) for f in sources()]
+            cmds = [[nvcc(), *ARCH_FLAGS, *flags, "-c", str(f), "-o", o] for f, o in zip(sources(), objects)]
+            if verbose:
+                print("\n".join(map(" ".join, cmds)), file=sys.stderr)
+            with ThreadPoolExecutor(max_workers=max(1, min(len(cmds), os.cpu_count() or 1))) as pool:
+                for text in pool.map(run, cmds):
+                    if verbose:
+                        print(text, file=sys.stderr)
+            run([nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, *objects, "-o", str(tmp)])
+    except BaseException:
         tmp.unlink(missing_ok=True)
-        raise RuntimeError(f"nvcc failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
-    if verbose:
-        print(r.stderr, file=sys.stderr)
+        raise
     os.replace(tmp, LIB_PATH)
-    _stamp().write_text(digest + "\n")
+    _stamp().write_text(stamp + "\n")
     return LIB_PATH
 
 

@@ -1,0 +1,359 @@
+// micro_common.cuh — what the microscaled kernels share: the formats, the quantisation of eight values per thread, the
+// scale tiles' addresses, and vector access to fp16 / bf16 / fp32 rows.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <cstdio>
+#include <exception>
+#include <type_traits>
+#include <utility>
+#include <string>
+
+#include "b2g.h"
+#include "b2g_micro.h"
+
+namespace b2g {
+
+int32_t record_error(int32_t code, const std::string& msg);  // b2g_gemm.cu: sets b2g_last_error()
+
+namespace micro {
+
+enum Fmt : int { FMT_NONE = 0, FMT_MXFP8 = B2G_FMT_MXFP8, FMT_MXFP4 = B2G_FMT_MXFP4, FMT_NVFP4 = B2G_FMT_NVFP4 };
+
+constexpr int block_of(int fmt) { return fmt == FMT_NVFP4 ? 16 : 32; }
+
+// Nothing may be thrown across the C boundary: what a body throws (std::bad_alloc) becomes an error code.
+template <typename F>
+int32_t guarded(F&& body) {
+  try {
+    return body();
+  } catch (const std::exception&) {
+    return B2G_ERR_CUDA;
+  }
+}
+
+inline int32_t launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return B2G_OK;
+  return record_error(B2G_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+inline int64_t min_pitch(int fmt, int64_t cols) { return ceil_div(cols, 32) * (fmt == FMT_MXFP8 ? 32 : 16); }
+
+// Checks a microscaled tensor's fields; B2G_OK or an error with text naming `what`.
+inline int32_t check_tensor(const b2g_micro_tensor* t, const char* what) {
+  auto bad = [&](const char* why) { return record_error(B2G_ERR_INVALID_ARG, std::string(what) + ": " + why); };
+  if (!t) return bad("null tensor");
+  if (t->format < FMT_MXFP8 || t->format > FMT_NVFP4) return bad("format must be one of B2G_FMT_*");
+  if (t->rows < 0 || t->cols < 0) return bad("negative dimension");
+  if (t->rows >= (int64_t(1) << 31) - 128 || t->cols >= (int64_t(1) << 31) - 128)
+    return record_error(B2G_ERR_UNSUPPORTED, std::string("dimension_too_large: ") + what + " needs rows and cols < 2^31 - 128");
+  if (t->rows == 0 || t->cols == 0) return B2G_OK;
+  if (!t->codes || !t->scales) return bad("null codes or scales");
+  if (!aligned16(t->codes) || !aligned16(t->scales)) return bad("codes and scales must be 16-byte aligned");
+  if (t->pitch < min_pitch(t->format, t->cols) || t->pitch % (t->format == FMT_MXFP8 ? 32 : 16))
+    return bad("pitch too small or misaligned");
+  if (t->format == FMT_NVFP4 && !t->scale) return bad("NVFP4 needs a tensor scale");
+  return B2G_OK;
+}
+
+struct Mat {
+  const void* p;
+  int64_t sr, sc;
+};
+
+struct Quant {  // where a microscaled tensor goes
+  uint8_t* codes;
+  uint8_t* scales;
+  const float* scale;
+  int64_t pitch, ktiles, code_cols;
+};
+
+// Whether rows of `m` can be read and written in 16-byte pieces.
+inline bool vec_ok(const b2g_micro_matrix* m, int64_t rows, int64_t size) {
+  return m->stride_c == 1 && aligned16(m->ptr) && (rows <= 1 || (m->stride_r * size) % 16 == 0);
+}
+
+inline Mat mat(const b2g_micro_matrix* m) { return Mat{m->ptr, m->stride_r, m->stride_c}; }
+
+inline Quant quant(const b2g_micro_tensor* t) {
+  return Quant{static_cast<uint8_t*>(t->codes), static_cast<uint8_t*>(t->scales), t->scale, t->pitch,
+               ceil_div(t->cols, 4 * block_of(t->format)), ceil_div(t->cols, 32) * 32};
+}
+
+inline int32_t too_large(const char* what) {
+  return record_error(B2G_ERR_UNSUPPORTED, std::string("dimension_too_large: ") + what + " needs fewer elements a call");
+}
+
+constexpr int64_t kMaxGrid = 2147483647;
+
+// f(T{}, std::integral_constant<int, FMT>{}) for a value type and a format
+template <typename F>
+int32_t by_format(int fmt, F&& f) {
+  switch (fmt) {
+    case FMT_MXFP8: return f(std::integral_constant<int, FMT_MXFP8>{});
+    case FMT_MXFP4: return f(std::integral_constant<int, FMT_MXFP4>{});
+    default: return f(std::integral_constant<int, FMT_NVFP4>{});
+  }
+}
+
+template <typename F>
+int32_t by_flag(bool flag, F&& f) {
+  return flag ? f(std::true_type{}) : f(std::false_type{});
+}
+
+template <typename F>
+int32_t by_type(int dtype, F&& f) {
+  switch (dtype) {
+    case B2G_VALUE_F16: return f(__half{});
+    case B2G_VALUE_BF16: return f(__nv_bfloat16{});
+    default: return f(float{});
+  }
+}
+
+inline int32_t check_matrix(const b2g_micro_matrix* m, const char* what) {
+  if (m && m->ptr) return B2G_OK;
+  return record_error(B2G_ERR_INVALID_ARG, std::string("null ") + what);
+}
+
+// ---------------------------------------------------------------- device side
+// Offset of the scale bytes of row `row` in tile column 0 of its row tile; tile column kt adds kt * 512.
+__device__ __forceinline__ int64_t scale_row(int64_t row, int64_t ktiles) {
+  return (row >> 7) * ktiles * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) {
+  return __half2float(v);
+}
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) {
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) {
+  return v;
+}
+
+// Eight consecutive values of one row as they lie in memory: 16 bytes (fp16, bf16) or 32 (fp32).
+template <typename T>
+struct Raw8 {
+  uint4 v;
+};
+template <>
+struct Raw8<float> {
+  uint4 v, w;
+};
+
+__device__ __forceinline__ float2 pair_f32(uint32_t w, __half*) {
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+__device__ __forceinline__ float2 pair_f32(uint32_t w, __nv_bfloat16*) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&o)[8]) {
+  const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = pair_f32(w[i], static_cast<T*>(nullptr));
+    o[2 * i] = f.x;
+    o[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&o)[8]) {
+  const uint32_t w[8] = {r.v.x, r.v.y, r.v.z, r.v.w, r.w.x, r.w.y, r.w.z, r.w.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(w[i]);
+}
+
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, __half*) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> pack8(const float (&v)[8]) {
+  T* t = nullptr;
+  return Raw8<T>{make_uint4(pack_pair(v[0], v[1], t), pack_pair(v[2], v[3], t), pack_pair(v[4], v[5], t),
+                            pack_pair(v[6], v[7], t))};
+}
+template <>
+__device__ __forceinline__ Raw8<float> pack8<float>(const float (&v)[8]) {
+  return Raw8<float>{make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])),
+                     make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]))};
+}
+
+// Columns c .. c+7 of a row that starts at `row`; columns at or past `cols` read as zero. VEC: unit column stride and
+// 16-byte aligned rows, so eight columns that all exist are one or two 16-byte loads.
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw8<T> load8(const T* row, int64_t stride_c, int64_t c, int64_t cols) {
+  if (VEC && c + 8 <= cols) {
+    Raw8<T> r;
+    const uint4* p = reinterpret_cast<const uint4*>(row + c);
+    r.v = __ldg(p);
+    if constexpr (sizeof(T) == 4) r.w = __ldg(p + 1);
+    return r;
+  }
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f32(row[(c + i) * stride_c]) : 0.f;
+  return pack8<T>(v);
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* row, int64_t stride_c, int64_t c, int64_t cols, const Raw8<T>& r) {
+  if (VEC && c + 8 <= cols) {
+    uint4* p = reinterpret_cast<uint4*>(row + c);
+    p[0] = r.v;
+    if constexpr (sizeof(T) == 4) p[1] = r.w;
+    return;
+  }
+  float v[8];
+  unpack8(r, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (c + i < cols) row[(c + i) * stride_c] = from_f32<T>(v[i]);
+}
+
+// The byte of a block's power-of-two scale: with amax = m * 2^e, the smallest exponent at which amax is at most the
+// codes' largest magnitude (448 = 1.75 * 2^8, 6 = 1.5 * 2^2); from the bits alone, so it is exact. 255 (NaN) where the
+// block holds an infinity or a NaN (their bits are above every finite magnitude's).
+template <int FMT>
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
+  constexpr int emax = FMT == FMT_MXFP8 ? 8 : 2;
+  constexpr uint32_t mant = FMT == FMT_MXFP8 ? 0x600000u : 0x400000u;
+  const int e = static_cast<int>(amax_bits >> 23) - emax + ((amax_bits & 0x7fffffu) > mant ? 1 : 0);
+  return amax_bits >= 0x7f800000u ? 255u : static_cast<uint32_t>(max(e, 0));
+}
+
+__device__ __forceinline__ float e4m3_to_f32(uint32_t byte) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+}
+
+// A power-of-two scale's value (2^-127 is subnormal in fp32).
+__device__ __forceinline__ float mx_scale_value(uint32_t byte) {
+  return byte == 255u ? __uint_as_float(0x7fffffffu) : byte ? __uint_as_float(byte << 23) : __uint_as_float(0x00400000u);
+}
+
+// One block's quantiser: its scale byte, and how an element becomes a code's value.
+//   MX: x * 2^-e, exact unless it leaves fp32's range at the bottom, where the code is zero anyway.
+//   NVFP4: x / u, u = block scale * tensor scale, correctly rounded as a division's quotient so that values on the
+//   border between two codes fall as the definition says: one reciprocal a block, then per element the quotient's
+//   estimate corrected by its residual (Markstein, "Computation of elementary functions on the IBM RISC System/6000
+//   processor", 1990). A block whose scale rounds to zero is zero; zeros keep the value's sign.
+template <int FMT>
+struct BlockQuant {
+  uint32_t byte;
+  float mul;   // MX: 2^-e; NVFP4: 1 / u; 0: every code is zero
+  float unit;  // NVFP4: u
+  uint32_t sign;  // NVFP4: the sign bit, 0 in a NaN block
+  __device__ __forceinline__ void init(uint32_t amax_bits, float tensor_scale) {
+    if constexpr (FMT == FMT_NVFP4) {
+      const float s = __fdiv_rn(__uint_as_float(amax_bits), 6.f * tensor_scale);
+      byte = amax_bits >= 0x7f800000u ? 0x7fu : __nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3);
+      unit = e4m3_to_f32(byte) * tensor_scale;
+      mul = (byte == 0u || byte == 0x7fu) ? 0.f : __frcp_rn(unit);
+      sign = byte == 0x7fu ? 0u : 0x80000000u;
+    } else {
+      byte = mx_scale_byte<FMT>(amax_bits);
+      mul = byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
+    }
+  }
+  __device__ __forceinline__ float scaled(float x) const {
+    if constexpr (FMT == FMT_NVFP4) {
+      const float q = x * mul;
+      const float r = mul == 0.f ? 0.f : fmaf(fmaf(-q, unit, x), mul, q);
+      return __uint_as_float((__float_as_uint(r) & 0x7fffffffu) | (__float_as_uint(x) & sign));
+    } else {
+      return mul == 0.f ? 0.f : x * mul;
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+
+__device__ __forceinline__ uint32_t e2m1x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp4x2(make_float2(a, b), __NV_E2M1, cudaRoundNearest);
+  const uint32_t hi = __nv_cvt_float2_to_fp4x2(make_float2(c, d), __NV_E2M1, cudaRoundNearest);
+  return lo | hi << 8;
+}
+
+// Eight values' codes: .x (and .y for MXFP8), lowest column in the lowest bits.
+template <int FMT>
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], const BlockQuant<FMT>& b) {
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = b.scaled(v[i]);
+  if constexpr (FMT == FMT_MXFP8) return make_uint2(e4m3x4(s[0], s[1], s[2], s[3]), e4m3x4(s[4], s[5], s[6], s[7]));
+  else return make_uint2(e2m1x4(s[0], s[1], s[2], s[3]) | e2m1x4(s[4], s[5], s[6], s[7]) << 16, 0u);
+}
+
+// Quantise eight consecutive columns per lane, the warp's 32 lanes holding 256 consecutive columns from `col` (lane 0's
+// first, a multiple of 256 past the row's start), and store them: the codes of columns below `code_cols` (a multiple of
+// 32), and the scale words of tile columns below `ktiles`. A block's lanes (4 for blocks of 32, 2 for 16) share its
+// largest magnitude by shuffles; the four scale bytes of one tile row are gathered into one 4-byte store. Called by a
+// converged warp.
+template <int FMT>
+__device__ __forceinline__ void quantize_store(const float (&v)[8], int lane, int64_t c, int64_t code_cols,
+                                               uint8_t* code_row, uint8_t* scale_row0, int64_t ktiles, float tensor_scale) {
+  constexpr int kLanes = block_of(FMT) / 8;
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+#pragma unroll
+  for (int d = 1; d < kLanes; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  BlockQuant<FMT> b;
+  b.init(m, tensor_scale);
+  const uint2 q = codes8<FMT>(v, b);
+  if (c < code_cols) {
+    if constexpr (FMT == FMT_MXFP8) *reinterpret_cast<uint2*>(code_row + c) = q;
+    else *reinterpret_cast<uint32_t*>(code_row + (c >> 1)) = q.x;
+  }
+  uint32_t w = b.byte << (8 * ((lane / kLanes) & 3));
+  w |= __shfl_xor_sync(0xffffffffu, w, kLanes);
+  w |= __shfl_xor_sync(0xffffffffu, w, 2 * kLanes);
+  const int64_t kt = c / (4 * block_of(FMT));
+  if ((lane & (4 * kLanes - 1)) == 0 && kt < ktiles) *reinterpret_cast<uint32_t*>(scale_row0 + kt * 512) = w;
+}
+
+}  // namespace micro
+}  // namespace b2g

@@ -1,0 +1,560 @@
+// micro_gemm.cu — products of two microscaled tensors on the block-scaled tensor-core kinds: C[M,N] = A[M,K] * B[N,K]^T.
+//
+// Both operands lie as codes with K contiguous and scales in the order the tensor core reads them, so nothing is
+// converted on the way: TMA brings 128 bytes of codes a row (256 columns of 4 bits, 128 of 8) and the scale tiles that
+// belong to them into a ring of shared-memory stages, tcgen05.cp moves the scales on into tensor memory (a region of its
+// own for every stage, free once the stage's MMAs have completed), and four block-scaled MMAs of 32 bytes of K multiply
+// the stage into fp32 accumulators. One CTA takes a 128 x tile_q tile and K split; the MMA's 128 rows run over B's rows (a
+// layer's weights), its narrow side over A's (the tokens), so a few tokens cost a narrow tile. The K splits of a tile are
+// one thread-block cluster and are summed through distributed shared memory.
+// Every wait is bounded as in b2g_gemm.cu: on expiry the status word gets a code and the CTA drains and returns.
+
+#include <cuda.h>
+
+#include <cstring>
+#include <mutex>
+#include <new>
+
+#include "micro_common.cuh"
+#include "micro_ptx.cuh"
+
+namespace b2g {
+namespace micro {
+
+constexpr uint32_t kCtl = 1024;                       // barriers and flags in front of the ring
+constexpr int kMaxStages = 16;
+constexpr uint64_t kWaitNs = 1000000000ull;           // 1 s per wait: far above any legal stall
+constexpr uint64_t kDrainNs = 50000000ull;            // 50 ms to drain in-flight work after an abort
+constexpr uint32_t kMaxSmem = 232448;                 // sm_100 opt-in maximum dynamic shared memory per block
+constexpr int kStepsPerStage = 4;                     // MMAs of 32 bytes of K in a 128-byte stage
+
+constexpr uint32_t O_FULL = 0, O_EMPTY = 128, O_TFULL = 256, O_DRAIN = 272, O_TMEM = 280, O_ABORT = 284;
+
+// status codes: b2g_status_string names them
+constexpr int kProducerTimeout = 0x101, kMmaTimeout = 0x102, kEpilogueTimeout = 0x103;
+
+// Scale tiles (4 blocks a row) of a stage's K, and tensor-memory columns and bytes of one 128-row tile's.
+constexpr int tiles_of(int kind) { return kind == FMT_MXFP8 ? 1 : kind == FMT_MXFP4 ? 2 : 4; }
+// K columns of a stage and of one MMA
+constexpr int stage_k(int kind) { return kind == FMT_MXFP8 ? 128 : 256; }
+constexpr int step_k(int kind) { return stage_k(kind) / kStepsPerStage; }
+// K step `s` of a stage: its scales' tile, and the byte in the tile's cells where they start
+constexpr int step_tile(int kind, int s) { return kind == FMT_MXFP8 ? 0 : kind == FMT_MXFP4 ? s / 2 : s; }
+constexpr uint32_t step_id(int kind, int s) { return kind == FMT_MXFP8 ? s : kind == FMT_MXFP4 ? (s & 1) * 2 : 0; }
+
+// P: the operand on the MMA's row side (rows_p), Q: the one on its column side.
+struct Params {
+  int32_t rows_p, rows_q, K, num_kb;
+  int32_t tile_q, q_tiles;           // columns of a tile; 128-row scale tiles they span
+  int32_t stages, split;
+  int32_t tiles_p, tiles_q, units;
+  uint32_t q_bytes, stage_bytes;     // Q's codes of a stage; its place in the ring, whole KB
+  uint32_t tx_bytes;                 // what its copies bring: codes and scales of both operands
+  uint32_t acc_cols, tmem_cols;
+  void* out;
+  int64_t ldc;
+  int32_t out_bf16, vec;             // vec: C's rows can be stored in 16-byte pieces
+  const float *scale_a, *scale_b;    // NVFP4 tensor scales
+  int* status;
+};
+
+__device__ __noinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int* status, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (;;) {
+    if (mbar_try_wait_hint(bar, parity, 1000000u)) return true;
+    if (*abort_flag) return false;
+    if (global_timer_ns() - t0 > kWaitNs) {
+      *abort_flag = 1u;
+      if (status) atomicCAS(status, 0, code);
+      return false;
+    }
+  }
+}
+
+__device__ __noinline__ void drain_phase(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (global_timer_ns() - t0 > limit_ns) return;
+  }
+}
+
+__device__ __forceinline__ uint32_t cvt2(float a, float b, int bf16) {
+  return bf16 ? pack_pair(a, b, static_cast<__nv_bfloat16*>(nullptr)) : pack_pair(a, b, static_cast<__half*>(nullptr));
+}
+
+__device__ __forceinline__ uint16_t cvt1(float a, int bf16) {
+  return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(a)) : __half_as_ushort(__float2half_rn(a));
+}
+
+// Scales of stage columns in tensor memory: P's tiles first (4 columns each), then Q's, K tile by K tile.
+template <int KIND>
+__device__ __forceinline__ uint32_t scale_cols(int q_tiles) {
+  return tiles_of(KIND) * 4u * (1u + static_cast<uint32_t>(q_tiles));
+}
+
+// Issue one stage: its scales into tensor memory, then up to four MMAs (fewer where K ends inside the stage: codes past
+// K are zero but the scales there may be any bytes). `sp`, `sq`, `cp`, `cq`: shared addresses of P's and Q's codes and of
+// their scales.
+template <int KIND, int PAIR>
+__device__ __forceinline__ void issue_stage(uint32_t d, uint64_t p_desc, uint64_t q_desc, uint32_t cp, uint32_t cq,
+                                            uint32_t tmem_scales, int q_tiles, const uint32_t (&idesc)[kStepsPerStage],
+                                            int steps, uint32_t first) {
+  constexpr int T = tiles_of(KIND);
+  const uint64_t pd = sdesc_plain(cp), qd = sdesc_plain(cq);
+  const uint32_t tq = tmem_scales + 4 * T;
+#pragma unroll
+  for (int k = 0; k < T; ++k) {
+    scales_to_tmem_w<PAIR>(tmem_scales + 4 * k, pd + k * 32);
+    scales_to_tmem_w<PAIR>(tq + 4 * q_tiles * k, qd + k * 32);
+    if (q_tiles == 2) scales_to_tmem_w<PAIR>(tq + 8 * k + 4, qd + (T + k) * 32);
+  }
+#pragma unroll
+  for (int s = 0; s < kStepsPerStage; ++s) {
+    if (s < steps)
+      umma_scaled_w<KIND, PAIR>(d, p_desc + s * 2, q_desc + s * 2, idesc[s], tmem_scales + 4 * step_tile(KIND, s),
+                                tq + 4 * q_tiles * step_tile(KIND, s), s == 0 ? first : 1u);
+  }
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(192, 1)
+    product_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap map_p,
+                   const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_sp,
+                   const __grid_constant__ CUtensorMap map_sq) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr uint32_t kPBytes = 128 * 128, kTileBytes = 512u * tiles_of(KIND);
+  const uint32_t ctl = smem_addr(smem_raw);
+  const uint32_t ring = (ctl + kCtl + 1023u) & ~1023u;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem_raw + O_ABORT);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int unit = static_cast<int>(blockIdx.x);
+  const int tile = unit / p.split, split = unit - tile * p.split;
+  const int tp = tile / p.tiles_q, tq = tile - tp * p.tiles_q;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(split) * p.num_kb / p.split);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(split + 1) * p.num_kb / p.split);
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_p);
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_sp);
+    tma_prefetch_desc(&map_sq);
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(ctl + O_FULL + 8 * s, 1);
+      mbar_init(ctl + O_EMPTY + 8 * s, 1);
+    }
+    mbar_init(ctl + O_TFULL, 1);
+    mbar_init(ctl + O_DRAIN, 1);
+    *abort_flag = 0u;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(ctl + O_TMEM, p.tmem_cols);
+    tmem_relinquish();
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + O_TMEM);
+
+  if (warp == 0) {
+    if (lane == 0) {  // TMA producer
+      int s = 0, issued = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const uint32_t empty = ctl + O_EMPTY + 8 * s, full = ctl + O_FULL + 8 * s;
+        if (!mbar_try_wait(empty, ph ^ 1u) && !wait_phase(empty, ph ^ 1u, abort_flag, p.status, kProducerTimeout)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(full, p.tx_bytes);
+        const uint32_t base = ring + s * p.stage_bytes;
+        tma_load_2d(base, &map_p, full, kb * 128, tp * 128);
+        tma_load_2d(base + kPBytes, &map_q, full, kb * 128, tq * p.tile_q);
+        tma_load_3d(base + kPBytes + p.q_bytes, &map_sp, full, 0, kb * tiles_of(KIND), tp);
+        tma_load_3d(base + kPBytes + p.q_bytes + kTileBytes, &map_sq, full, 0, kb * tiles_of(KIND), tq * p.tile_q / 128);
+        ++issued;
+        if (++s == p.stages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      if (!ok) {  // let the copies already issued land before shared memory is released
+        for (int i = min(issued, p.stages); i > 0; --i) {
+          if (--s < 0) {
+            s = p.stages - 1;
+            ph ^= 1u;
+          }
+          drain_phase(ctl + O_FULL + 8 * s, ph, kDrainNs);
+        }
+      }
+    }
+  } else if (warp == 1) {  // MMA issuer: the warp waits together, lane 0 issues
+    uint32_t idesc[kStepsPerStage];
+#pragma unroll
+    for (int i = 0; i < kStepsPerStage; ++i) idesc[i] = idesc_scaled(KIND, step_id(KIND, i), 128, p.tile_q);
+    const uint64_t pd = sdesc_sw128(ring, 16u, 1024u), qd = sdesc_sw128(ring + kPBytes, 16u, 1024u);
+    const uint32_t cols = scale_cols<KIND>(p.q_tiles);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const uint32_t full = ctl + O_FULL + 8 * s;
+      if (!mbar_try_wait(full, ph) && !wait_phase(full, ph, abort_flag, p.status, kMmaTimeout)) {
+        ok = false;
+        break;
+      }
+      const uint32_t base = ring + s * p.stage_bytes, off = s * (p.stage_bytes >> 4);
+      const int left = p.K - kb * stage_k(KIND);
+      const int steps = left >= stage_k(KIND) ? kStepsPerStage : (left + step_k(KIND) - 1) / step_k(KIND);
+      issue_stage<KIND, 0>(tmem, pd + off, qd + off, base + kPBytes + p.q_bytes, base + kPBytes + p.q_bytes + kTileBytes,
+                           tmem + p.acc_cols + s * cols, p.q_tiles, idesc, steps, kb == kb0 ? 0u : 1u);
+      umma_commit_w(ctl + O_EMPTY + 8 * s);
+      if (++s == p.stages) {
+        s = 0;
+        ph ^= 1u;
+      }
+    }
+    if (ok && kb1 > kb0) umma_commit_w(ctl + O_TFULL);
+    umma_commit_w(ctl + O_DRAIN);
+    drain_phase(ctl + O_DRAIN, 0, ok ? kWaitNs : kDrainNs);
+  } else {
+    // Epilogue, part one: this split's fp32 tile into shared memory as [column j][row i] (128 + 4 floats a column: 32
+    // lanes store 32 consecutive words). The ring is free: every MMA has completed.
+    const int q = warp & 3;
+    const bool some = kb1 > kb0;
+    if (!some || wait_phase(ctl + O_TFULL, 0u, abort_flag, p.status, kEpilogueTimeout)) {
+      tc_fence_after();
+      const int i = q * 32 + lane;
+      for (int c = 0; c < p.tile_q; c += 32) {
+        const int n = min(32, p.tile_q - c);
+        uint32_t v[32];
+        if (some) {
+          const uint32_t at = tmem + c + (static_cast<uint32_t>(q * 32) << 16);
+          if (n == 32) tmem_ld_32cols(at, v);
+          else tmem_ld_16cols(at, v);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < n) st_shared_u32(ring + ((c + j) * 132 + i) * 4u, some ? v[j] : 0u);
+      }
+    }
+  }
+  // Part two: CTA r of the cluster adds its share of the tile over the cluster's CTAs in split order, scales, converts
+  // and stores, eight consecutive columns of C at a time. Every thread of every CTA reaches both barriers.
+  __syncwarp();
+  if (p.split > 1) cluster_sync();
+  else __syncthreads();
+  {
+    const float alpha = p.scale_a ? *p.scale_a * *p.scale_b : 1.f;
+    const int cols = min(p.tile_q, p.rows_q - tq * p.tile_q);  // columns of the tile inside C^T
+    const int groups = cols * 16;
+    const int g0 = groups * split / p.split, g1 = groups * (split + 1) / p.split;
+    uint16_t* out = static_cast<uint16_t*>(p.out);
+    for (int g = g0 + static_cast<int>(threadIdx.x); g < g1; g += 192) {
+      const int j = g >> 4, i = (g & 15) * 8;
+      const int64_t n = static_cast<int64_t>(tp) * 128 + i;
+      if (n >= p.rows_p) continue;
+      const uint32_t off = ring + (j * 132 + i) * 4u;
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < p.split; ++s) {
+        const uint32_t at = p.split > 1 ? map_to_rank(off, s) : off;
+        const float4 x = ld_cluster_v4(at), y = ld_cluster_v4(at + 16);
+        v[0] += x.x;
+        v[1] += x.y;
+        v[2] += x.z;
+        v[3] += x.w;
+        v[4] += y.x;
+        v[5] += y.y;
+        v[6] += y.z;
+        v[7] += y.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= alpha;
+      uint16_t* o = out + (static_cast<int64_t>(tq) * p.tile_q + j) * p.ldc + n;
+      if (p.vec && n + 8 <= p.rows_p) {
+        *reinterpret_cast<uint4*>(o) = make_uint4(cvt2(v[0], v[1], p.out_bf16), cvt2(v[2], v[3], p.out_bf16),
+                                                  cvt2(v[4], v[5], p.out_bf16), cvt2(v[6], v[7], p.out_bf16));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (n + k < p.rows_p) o[k] = cvt1(v[k], p.out_bf16);
+      }
+    }
+  }
+  __syncwarp();
+  if (p.split > 1) cluster_sync();  // a CTA's shared memory stays until its peers have read it
+  else __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, p.tmem_cols);
+}
+
+// ---------------------------------------------------------------- host side
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static std::once_flag once;
+  static EncodeFn fn = nullptr;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(f);
+    else
+      cudaGetLastError();
+  });
+  return fn;
+}
+
+// Codes as rows of bytes: boxes of 128 bytes x `box_rows` rows, 128-byte swizzle. What lies past a row's last code byte
+// reads as zero.
+int32_t encode_codes(CUtensorMap* map, const b2g_micro_tensor* t, int box_rows) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return record_error(B2G_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const int64_t bytes = t->format == FMT_MXFP8 ? t->cols : (t->cols + 1) / 2;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(bytes), static_cast<cuuint64_t>(t->rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(t->pitch)};
+  const cuuint32_t box[2] = {128u, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t elem[2] = {1u, 1u};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, t->codes, dims, strides, box, elem,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return B2G_OK;
+  return record_error(B2G_ERR_CUDA, "cuTensorMapEncodeTiled (codes): error " + std::to_string(static_cast<int>(r)));
+}
+
+// Scales as [row tile][K tile][512 bytes]: boxes of `ktiles` K tiles x `row_tiles` row tiles. Tiles that do not exist
+// read as zero.
+int32_t encode_scales(CUtensorMap* map, const b2g_micro_tensor* t, int ktiles, int row_tiles) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return record_error(B2G_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const int64_t kt = ceil_div(t->cols, 4 * block_of(t->format));
+  const cuuint64_t dims[3] = {128u, static_cast<cuuint64_t>(kt), static_cast<cuuint64_t>(ceil_div(t->rows, 128))};
+  const cuuint64_t strides[2] = {512u, static_cast<cuuint64_t>(kt * 512)};
+  const cuuint32_t box[3] = {128u, static_cast<cuuint32_t>(ktiles), static_cast<cuuint32_t>(row_tiles)};
+  const cuuint32_t elem[3] = {1u, 1u, 1u};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, t->scales, dims, strides, box, elem,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return B2G_OK;
+  return record_error(B2G_ERR_CUDA, "cuTensorMapEncodeTiled (scales): error " + std::to_string(static_cast<int>(r)));
+}
+
+// Function attributes, once per device.
+int32_t init_device(int dev) {
+  static std::mutex mu;
+  static bool done[64];
+  std::lock_guard<std::mutex> lock(mu);
+  if (dev >= 0 && dev < 64 && done[dev]) return B2G_OK;
+  const void* fns[] = {reinterpret_cast<const void*>(product_kernel<FMT_MXFP8>),
+                       reinterpret_cast<const void*>(product_kernel<FMT_MXFP4>),
+                       reinterpret_cast<const void*>(product_kernel<FMT_NVFP4>)};
+  for (const void* f : fns) {
+    const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return record_error(B2G_ERR_CUDA, std::string("kernel attributes: ") + cudaGetErrorString(e));
+    }
+  }
+  if (dev >= 0 && dev < 64) done[dev] = true;
+  return B2G_OK;
+}
+
+// Clusters of 1..8 CTAs with the whole shared memory of an SM each that a B200 holds at once (a cluster lives inside a
+// GPC): a launch of more would run in waves.
+constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+
+struct Plan {
+  Params p;
+  CUtensorMap map_p, map_q, map_sp, map_sq;
+  int kind, device, grid;
+  uint32_t smem;
+  bool empty;    // no output element
+  bool zero;     // K = 0: C is zero
+  int64_t M, N;
+};
+
+uint32_t pow2_cols(uint32_t x) {
+  uint32_t c = 32;
+  while (c < x) c <<= 1;
+  return c;
+}
+
+int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b, void* C, int64_t ldc, int32_t dtype,
+                  int32_t* status) {
+  if (const int32_t rc = check_tensor(a, "a")) return rc;
+  if (const int32_t rc = check_tensor(b, "b")) return rc;
+  if (a->format != b->format) return record_error(B2G_ERR_UNSUPPORTED, "format_mismatch: a and b need one format");
+  if (a->cols != b->cols) return record_error(B2G_ERR_INVALID_ARG, "a and b differ in columns (the dimension summed over)");
+  if (dtype != B2G_VALUE_F16 && dtype != B2G_VALUE_BF16)
+    return record_error(B2G_ERR_INVALID_ARG, "dtype must be B2G_VALUE_F16 or B2G_VALUE_BF16");
+  pl.M = a->rows;
+  pl.N = b->rows;
+  pl.kind = a->format;
+  pl.empty = pl.M == 0 || pl.N == 0;
+  pl.zero = a->cols == 0;
+  if (pl.empty) return B2G_OK;
+  if (!C || ldc < pl.N) return record_error(B2G_ERR_INVALID_ARG, "null C or ldc below N");
+  if (cudaGetDevice(&pl.device) != cudaSuccess) {
+    cudaGetLastError();
+    return record_error(B2G_ERR_CUDA, "no CUDA device");
+  }
+  Params& p = pl.p;
+  std::memset(&p, 0, sizeof p);
+  p.out = C;
+  p.ldc = ldc;
+  if (pl.zero) return B2G_OK;
+  if (const int32_t rc = init_device(pl.device)) return rc;
+  p.out_bf16 = dtype == B2G_VALUE_BF16;
+  p.vec = aligned16(C) && ldc % 8 == 0;
+  p.status = status;
+  if (pl.kind == FMT_NVFP4) {
+    p.scale_a = a->scale;
+    p.scale_b = b->scale;
+  }
+  p.K = static_cast<int32_t>(a->cols);
+  p.num_kb = static_cast<int32_t>(ceil_div(a->cols, stage_k(pl.kind)));
+  const int T = tiles_of(pl.kind);
+  // rows run over B, columns over A
+  p.rows_p = static_cast<int32_t>(pl.N);
+  p.rows_q = static_cast<int32_t>(pl.M);
+  p.tile_q = pl.M <= 16 ? 16 : pl.M <= 32 ? 32 : pl.M <= 64 ? 64 : 128;
+  p.q_tiles = 1;
+  p.tiles_p = static_cast<int32_t>(ceil_div(p.rows_p, 128));
+  p.tiles_q = static_cast<int32_t>(ceil_div(p.rows_q, p.tile_q));
+  const int64_t tiles = static_cast<int64_t>(p.tiles_p) * p.tiles_q;
+  // K splits, one cluster: as many as keep every cluster resident at once and leave each split two stages
+  p.split = 1;
+  for (int s = 2; s <= 8; ++s)
+    if (tiles <= kClusters[s] && p.num_kb >= 2 * s) p.split = s;
+  if (tiles * p.split > kMaxGrid) return too_large("product");
+  p.units = static_cast<int32_t>(tiles * p.split);
+  pl.grid = p.units;
+  p.q_bytes = static_cast<uint32_t>(p.tile_q) * 128u;
+  p.tx_bytes = 128u * 128u + p.q_bytes + 512u * T * (1 + p.q_tiles);
+  p.stage_bytes = (p.tx_bytes + 1023u) & ~1023u;
+  p.acc_cols = pow2_cols(p.tile_q);
+  // Shared memory: clusters take a whole SM's each, so that no CTA of another launch can hold tensor memory there while
+  // this cluster's CTAs wait for one another; single CTAs take at most half, two to an SM, and at most half of the
+  // tensor memory.
+  const uint32_t room = p.split > 1 ? kMaxSmem : 113u * 1024u;
+  const uint32_t cols = tiles_of(pl.kind) * 4u * (1u + p.q_tiles);
+  uint32_t stages = (room - 2048u) / p.stage_bytes;
+  const uint32_t most_cols = p.split > 1 ? 512u : 256u;
+  if (stages > (most_cols - p.acc_cols) / cols) stages = (most_cols - p.acc_cols) / cols;
+  if (stages > static_cast<uint32_t>(kMaxStages)) stages = kMaxStages;
+  p.stages = static_cast<int32_t>(stages);
+  p.tmem_cols = pow2_cols(p.acc_cols + stages * cols);
+  uint32_t ring = stages * p.stage_bytes;
+  const uint32_t tile_bytes = static_cast<uint32_t>(p.tile_q) * 132u * 4u;
+  if (ring < tile_bytes) ring = tile_bytes;
+  pl.smem = p.split > 1 ? kMaxSmem : 2048u + ring;
+  if (p.split == 1 && pl.smem < 78u * 1024u) pl.smem = 78u * 1024u;  // never three to an SM: tensor memory holds two
+  if (const int32_t rc = encode_codes(&pl.map_p, b, 128)) return rc;
+  if (const int32_t rc = encode_codes(&pl.map_q, a, p.tile_q)) return rc;
+  if (const int32_t rc = encode_scales(&pl.map_sp, b, T, 1)) return rc;
+  return encode_scales(&pl.map_sq, a, T, p.q_tiles);
+}
+
+int32_t plan_launch(const Plan& pl, cudaStream_t st) {
+  if (pl.empty) return B2G_OK;
+  int cur = -1;
+  if (cudaGetDevice(&cur) != cudaSuccess || cur != pl.device) {
+    cudaGetLastError();
+    return record_error(B2G_ERR_INVALID_ARG, "plan was made on device " + std::to_string(pl.device) + " but device " +
+                                                 std::to_string(cur) + " is current");
+  }
+  if (pl.zero) {
+    const cudaError_t e = cudaMemset2DAsync(pl.p.out, static_cast<size_t>(pl.p.ldc) * 2, 0, static_cast<size_t>(pl.N) * 2,
+                                            static_cast<size_t>(pl.M), st);
+    if (e == cudaSuccess) return B2G_OK;
+    cudaGetLastError();
+    return record_error(B2G_ERR_CUDA, std::string("memset: ") + cudaGetErrorString(e));
+  }
+  cudaLaunchConfig_t lc = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attr;
+  lc.numAttrs = 1;
+  lc.stream = st;
+  lc.gridDim = dim3(static_cast<unsigned>(pl.grid), 1, 1);
+  lc.blockDim = dim3(192, 1, 1);
+  lc.dynamicSmemBytes = pl.smem;
+  if (pl.p.split > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(pl.p.split);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    lc.numAttrs = 2;
+  }
+  const auto go = [&](auto kernel) { return cudaLaunchKernelEx(&lc, kernel, pl.p, pl.map_p, pl.map_q, pl.map_sp, pl.map_sq); };
+  cudaError_t e = cudaSuccess;
+  by_format(pl.kind, [&](auto f) -> int32_t {
+    constexpr int F = decltype(f)::value;
+    e = go(product_kernel<F>);
+    return B2G_OK;
+  });
+  if (e == cudaSuccess) return B2G_OK;
+  cudaGetLastError();
+  return record_error(B2G_ERR_CUDA, std::string("product launch: ") + cudaGetErrorString(e));
+}
+
+}  // namespace micro
+}  // namespace b2g
+
+using namespace b2g;
+using namespace b2g::micro;
+
+struct b2g_micro_plan {
+  Plan plan;
+};
+
+extern "C" {
+
+int32_t b2g_micro_plan_create(const b2g_micro_tensor* a, const b2g_micro_tensor* b, void* C, int64_t ldc, int32_t dtype,
+                              int32_t* status, b2g_micro_plan** out) {
+  return guarded([&]() -> int32_t {
+    if (!out) return record_error(B2G_ERR_INVALID_ARG, "null plan output");
+    *out = nullptr;
+    b2g_micro_plan* p = new (std::nothrow) b2g_micro_plan();
+    if (!p) return record_error(B2G_ERR_CUDA, "out of host memory");
+    const int32_t rc = plan_init(p->plan, a, b, C, ldc, dtype, status);
+    if (rc != B2G_OK) {
+      delete p;
+      return rc;
+    }
+    *out = p;
+    return B2G_OK;
+  });
+}
+
+int32_t b2g_micro_plan_launch(const b2g_micro_plan* plan, void* stream) {
+  return guarded([&]() -> int32_t {
+    if (!plan) return record_error(B2G_ERR_INVALID_ARG, "null plan");
+    return plan_launch(plan->plan, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int32_t b2g_micro_plan_destroy(b2g_micro_plan* plan) {
+  delete plan;
+  return B2G_OK;
+}
+
+int32_t b2g_micro_matmul(const b2g_micro_tensor* a, const b2g_micro_tensor* b, void* C, int64_t ldc, int32_t dtype,
+                         int32_t* status, void* stream) {
+  return guarded([&]() -> int32_t {
+    Plan pl;
+    if (const int32_t rc = plan_init(pl, a, b, C, ldc, dtype, status)) return rc;
+    return plan_launch(pl, static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,427 @@
+// micro_norm.cu — root-mean-square norm of a row with the residual's addition, its output as values or as a microscaled
+// tensor, and its gradient.
+//
+// Bound by memory: each row is read once, held in registers between the sum of squares and the scaling, and written
+// once. `tpr` threads share a row, eight consecutive columns each per round of tpr * 8 columns; ROUNDS rounds are held
+// in registers (1, 2 or 4: as few as the row needs, since registers are what limits the rows in flight); past 4 rounds
+// the row is read again (from L2).
+
+#include "micro_common.cuh"
+
+namespace b2g {
+namespace micro {
+
+constexpr int kMostRounds = 4;
+constexpr int kMaxThreads = 512;  // per row, and per block where that is more than 128
+
+// Blocks of kMaxThreads an SM holds at once, by rounds held in registers.
+constexpr int blocks_per_sm(int rounds) { return rounds <= 2 ? 2 : 1; }
+
+// Sum over the `tpr` threads of each row of the block (tpr a multiple of 32; rows of a block are consecutive groups of
+// warps), the same bits in every thread: warps by shuffles, then the row's warps in order through `part` (one float2
+// per warp). `buf` alternates so that one barrier per call is enough.
+__device__ __forceinline__ float2 row_sum(float2 v, int tpr, float2 (*part)[32], int buf) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, d);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, d);
+  }
+  if (tpr == 32) return v;
+  const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp / per * per;
+  if ((threadIdx.x & 31) == 0) part[buf][warp] = v;
+  __syncthreads();
+  float2 s = make_float2(0.f, 0.f);
+  for (int i = 0; i < per; ++i) {
+    s.x += part[buf][first + i].x;
+    s.y += part[buf][first + i].y;
+  }
+  return s;
+}
+
+// FMT_NONE writes values (y), the formats write q; rows from `rows` to the end of their 128-row scale tile get zero
+// scales. RES: h = x + residual, else h = x.
+template <typename T, int FMT, bool RES, bool VEC, int ROUNDS>
+__global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
+    norm_kernel(Mat x, Mat res, const T* w, T* h, int64_t shr, int64_t shc, T* y, int64_t syr, int64_t syc, Quant q,
+                int64_t rows, int64_t cols, float eps, int tpr) {
+  __shared__ float2 part[2][32];
+  const int t = threadIdx.x % tpr;
+  const int64_t row = blockIdx.x * static_cast<int64_t>(blockDim.x / tpr) + threadIdx.x / tpr;
+  const bool live = row < rows;
+  const int64_t width = tpr * 8;
+  const T* xr = static_cast<const T*>(x.p) + row * x.sr;
+  const T* rr = RES ? static_cast<const T*>(res.p) + row * res.sr : nullptr;
+  const int64_t lim = live ? cols : 0;
+  const float ts = FMT == FMT_NVFP4 ? *q.scale : 0.f;
+
+  auto sum8 = [&](const Raw8<T>& a, const Raw8<T>& b, float(&v)[8]) {
+    unpack8(a, v);
+    if (RES) {
+      float f[8];
+      unpack8(b, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += f[i];
+    }
+  };
+
+  float v[ROUNDS][8];
+  float2 s = make_float2(0.f, 0.f);
+  {
+    Raw8<T> a[ROUNDS], b[ROUNDS];
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+      const int64_t c = k * width + t * 8;
+      if (k * width < cols) {
+        a[k] = load8<T, VEC>(xr, x.sc, c, lim);
+        if (RES) b[k] = load8<T, VEC>(rr, res.sc, c, lim);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+      const int64_t c = k * width + t * 8;
+      if (k * width < cols) {
+        sum8(a[k], b[k], v[k]);
+        if (RES && h && c < lim) store8<T, VEC>(h + row * shr, shc, c, lim, pack8<T>(v[k]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s.x = fmaf(v[k][i], v[k][i], s.x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
+      }
+    }
+  }
+  if constexpr (ROUNDS == kMostRounds) for (int64_t c0 = ROUNDS * width; c0 < cols; c0 += width) {
+    const int64_t c = c0 + t * 8;
+    Raw8<T> a = load8<T, VEC>(xr, x.sc, c, lim), b = a;
+    if (RES) b = load8<T, VEC>(rr, res.sc, c, lim);
+    float f[8];
+    sum8(a, b, f);
+    if (RES && h && c < lim) store8<T, VEC>(h + row * shr, shc, c, lim, pack8<T>(f));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s.x = fmaf(f[i], f[i], s.x);
+  }
+  s = row_sum(s, tpr, part, 0);
+  const float r = rsqrtf(s.x / static_cast<float>(cols) + eps);
+
+  const int64_t cover = FMT == FMT_NONE ? cols : q.ktiles * 4 * block_of(FMT);  // whole scale tiles
+  auto finish = [&](float(&f)[8], int64_t c) {
+    float g[8];
+    unpack8(load8<T, VEC>(w, 1, c, cols), g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = live && c + i < cols ? f[i] * r * g[i] : 0.f;
+    if constexpr (FMT == FMT_NONE) {
+      if (c < lim) store8<T, VEC>(y + row * syr, syc, c, lim, pack8<T>(f));
+    } else {
+      quantize_store<FMT>(f, threadIdx.x & 31, c, live ? q.code_cols : 0, q.codes + row * q.pitch,
+                          q.scales + scale_row(row, q.ktiles), q.ktiles, ts);
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k)
+    if (k * width < cover) finish(v[k], k * width + t * 8);
+  if constexpr (ROUNDS == kMostRounds) for (int64_t c0 = ROUNDS * width; c0 < cover; c0 += width) {
+    const int64_t c = c0 + t * 8;
+    Raw8<T> a = load8<T, VEC>(xr, x.sc, c, lim), b = a;
+    if (RES) b = load8<T, VEC>(rr, res.sc, c, lim);
+    float f[8];
+    sum8(a, b, f);
+    finish(f, c);
+  }
+}
+
+// Gradient: a block walks rows blockIdx.x * rpb + k * gridDim.x * rpb, so its threads keep their columns and add up the
+// weight's gradient in registers (rounds past the fourth: in the block's own row of the workspace). Each group of tpr
+// threads leaves one fp32 row of partial sums in the workspace; norm_dweight_kernel adds them in a fixed order.
+template <typename T, bool DH, bool VEC, int ROUNDS>
+__global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
+    norm_backward_kernel(Mat dy, Mat h, const T* w, Mat dh, T* dx, int64_t sxr, int64_t sxc, float* partial,
+                         int64_t rows, int64_t cols, float eps, int tpr) {
+  __shared__ float2 part[2][32];
+  const int t = threadIdx.x % tpr;
+  const int rpb = blockDim.x / tpr;
+  const int64_t group = blockIdx.x * static_cast<int64_t>(rpb) + threadIdx.x / tpr;
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * rpb;
+  const int64_t width = tpr * 8;
+  float* mine = partial + group * cols;
+  float acc[ROUNDS][8];
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[k][i] = 0.f;
+  const int64_t trips = (rows + groups - 1) / groups;
+  int buf = 0;
+  for (int64_t trip = 0; trip < trips; ++trip) {
+    const int64_t row = trip * groups + group;
+    const int64_t lim = row < rows ? cols : 0;  // every thread of the block reaches the barrier
+    const T* dyr = static_cast<const T*>(dy.p) + row * dy.sr;
+    const T* hr = static_cast<const T*>(h.p) + row * h.sr;
+    Raw8<T> a[ROUNDS], b[ROUNDS];
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+      const int64_t c = k * width + t * 8;
+      if (k * width < cols) {
+        a[k] = load8<T, VEC>(dyr, dy.sc, c, lim);
+        b[k] = load8<T, VEC>(hr, h.sc, c, lim);
+      }
+    }
+    float2 s = make_float2(0.f, 0.f);
+    auto add = [&](const Raw8<T>& ra, const Raw8<T>& rb, int64_t c) {
+      float d[8], v[8], g[8];
+      unpack8(ra, d);
+      unpack8(rb, v);
+      unpack8(load8<T, VEC>(w, 1, c, cols), g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s.x = fmaf(v[i], v[i], s.x);
+        s.y = fmaf(d[i] * g[i], v[i], s.y);
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k)
+      if (k * width < cols) add(a[k], b[k], k * width + t * 8);
+    if constexpr (ROUNDS == kMostRounds) for (int64_t c0 = ROUNDS * width; c0 < cols; c0 += width) {
+      const int64_t c = c0 + t * 8;
+      add(load8<T, VEC>(dyr, dy.sc, c, lim), load8<T, VEC>(hr, h.sc, c, lim), c);
+    }
+    s = row_sum(s, tpr, part, buf);
+    buf ^= 1;
+    const float n = static_cast<float>(cols);
+    const float r = rsqrtf(s.x / n + eps);
+    const float m = r * r * (s.y / n);  // dx = r * (dy * w - h * m)
+    auto finish = [&](const Raw8<T>& ra, const Raw8<T>& rb, int64_t c, float(&sum)[8]) {
+      float d[8], v[8], g[8], e[8], o[8];
+      unpack8(ra, d);
+      unpack8(rb, v);
+      unpack8(load8<T, VEC>(w, 1, c, cols), g);
+      if (DH) unpack8(load8<T, VEC>(static_cast<const T*>(dh.p) + row * dh.sr, dh.sc, c, lim), e);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        o[i] = r * (d[i] * g[i] - v[i] * m);
+        if (DH) o[i] += e[i];
+        sum[i] = fmaf(d[i] * r, v[i], sum[i]);
+      }
+      if (c < lim) store8<T, VEC>(dx + row * sxr, sxc, c, lim, pack8<T>(o));
+    };
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k)
+      if (k * width < cols && lim) finish(a[k], b[k], k * width + t * 8, acc[k]);
+    if constexpr (ROUNDS == kMostRounds) for (int64_t c0 = ROUNDS * width; c0 < cols && lim; c0 += width) {
+      const int64_t c = c0 + t * 8;
+      float sum[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] = trip > 0 && c + i < cols ? mine[c + i] : 0.f;
+      finish(load8<T, VEC>(dyr, dy.sc, c, lim), load8<T, VEC>(hr, h.sc, c, lim), c, sum);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < cols) mine[c + i] = sum[i];
+    }
+  }
+  if (group >= rows)  // a group without rows: its sums are zero
+    for (int64_t c = ROUNDS * width + t; c < cols; c += tpr) mine[c] = 0.f;
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    const int64_t c = k * width + t * 8;
+    if (c + 8 <= cols && cols % 4 == 0) {
+      reinterpret_cast<float4*>(mine + c)[0] = make_float4(acc[k][0], acc[k][1], acc[k][2], acc[k][3]);
+      reinterpret_cast<float4*>(mine + c)[1] = make_float4(acc[k][4], acc[k][5], acc[k][6], acc[k][7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < cols) mine[c + i] = acc[k][i];
+    }
+  }
+}
+
+// dweight[c] = sum over the groups' partial rows, in order within each of 8 strands, then the strands in order.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_dweight_kernel(const float* partial, int64_t groups, int64_t cols, T* dw) {
+  __shared__ float part[8][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t c = blockIdx.x * int64_t(32) + x;
+  float s = 0.f;
+  if (c < cols) {
+    int64_t g = y;
+    for (; g + 24 < groups; g += 32) {
+      float f[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) f[u] = partial[(g + 8 * u) * cols + c];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += f[u];
+    }
+    for (; g < groups; g += 8) s += partial[g * cols + c];
+  }
+  part[y][x] = s;
+  __syncthreads();
+  if (y == 0 && c < cols) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += part[i][x];
+    dw[c] = from_f32<T>(s);
+  }
+}
+
+struct Split {
+  int tpr, threads, rounds;
+  int64_t blocks, groups;
+};
+
+int pow2_threads(int64_t n, int most) {
+  int t = 32;
+  while (t < n && t < most) t *= 2;
+  return t;
+}
+
+int rounds_of(int64_t cols, int tpr) {
+  const int64_t n = ceil_div(cols, int64_t(tpr) * 8);
+  return n <= 1 ? 1 : n <= 2 ? 2 : kMostRounds;
+}
+
+// Threads per row: with many rows, two rounds of eight columns a thread keep more loads in flight per thread; with few,
+// one round shortens the row's own time. Blocks of at least 128 threads.
+Split forward_split(int64_t rows, int64_t cols) {
+  Split s;
+  const int64_t chunks = ceil_div(cols, 8);
+  s.tpr = rows >= 592 ? pow2_threads(ceil_div(chunks, 2), kMaxThreads) : pow2_threads(chunks, kMaxThreads);
+  s.threads = s.tpr < 128 ? 128 : s.tpr;
+  s.rounds = rounds_of(cols, s.tpr);
+  s.groups = rows;
+  s.blocks = ceil_div(rows, s.threads / s.tpr);
+  return s;
+}
+
+// The gradient's blocks stay for many rows: as many as the GPU holds at once, fewer where there are fewer rows.
+Split backward_split(int64_t rows, int64_t cols) {
+  Split s;
+  s.tpr = pow2_threads(ceil_div(cols, 8), kMaxThreads);
+  s.threads = s.tpr < 128 ? 128 : s.tpr;
+  s.rounds = rounds_of(cols, s.tpr);
+  const int rpb = s.threads / s.tpr;
+  const int64_t most = 148 * blocks_per_sm(s.rounds) * (kMaxThreads / s.threads);
+  s.blocks = ceil_div(rows, rpb);
+  if (s.blocks > most) s.blocks = most;
+  s.groups = s.blocks * rpb;
+  return s;
+}
+
+}  // namespace micro
+}  // namespace b2g
+
+using namespace b2g;
+using namespace b2g::micro;
+
+extern "C" {
+
+int32_t b2g_micro_rms_norm(const b2g_micro_matrix* x, const b2g_micro_matrix* residual, const void* weight,
+                           const b2g_micro_matrix* h, const b2g_micro_matrix* y, const b2g_micro_tensor* q, int64_t rows,
+                           int64_t cols, float eps, int32_t dtype, void* stream) {
+  return guarded([&]() -> int32_t {
+    if (rows < 0 || cols < 0 || (dtype != B2G_VALUE_F16 && dtype != B2G_VALUE_BF16) || (!y && !q) || (y && q))
+      return record_error(B2G_ERR_INVALID_ARG, "rms_norm: bad dimension or dtype, or not one output");
+    if (q) {
+      if (const int32_t rc = check_tensor(q, "q")) return rc;
+      if (q->rows != rows || q->cols != cols) return record_error(B2G_ERR_INVALID_ARG, "rms_norm: q is not [rows, cols]");
+    }
+    if (rows == 0 || cols == 0) return B2G_OK;
+    if (const int32_t rc = check_matrix(x, "x")) return rc;
+    if (residual)
+      if (const int32_t rc = check_matrix(residual, "residual")) return rc;
+    if (h)
+      if (const int32_t rc = check_matrix(h, "h")) return rc;
+    if (y)
+      if (const int32_t rc = check_matrix(y, "y")) return rc;
+    if (!weight) return record_error(B2G_ERR_INVALID_ARG, "null weight");
+    const Split s = forward_split(q ? ceil_div(rows, 128) * 128 : rows, cols);
+    if (s.blocks > kMaxGrid) return too_large("rms_norm");
+    const bool vec = vec_ok(x, rows, 2) && (!residual || vec_ok(residual, rows, 2)) && (!h || vec_ok(h, rows, 2)) &&
+                     (!y || vec_ok(y, rows, 2)) && aligned16(weight);
+    return by_type(dtype, [&](auto t) -> int32_t {
+      using T = decltype(t);
+      if constexpr (sizeof(T) == 4) {
+        return B2G_ERR_INVALID_ARG;
+      } else {
+        const Mat none{nullptr, 0, 1};
+        const auto go = [&](auto kernel) {
+          kernel<<<static_cast<unsigned>(s.blocks), s.threads, 0, static_cast<cudaStream_t>(stream)>>>(
+              mat(x), residual ? mat(residual) : none, static_cast<const T*>(weight), h ? static_cast<T*>(h->ptr) : nullptr,
+              h ? h->stride_r : 0, h ? h->stride_c : 1, y ? static_cast<T*>(y->ptr) : nullptr, y ? y->stride_r : 0,
+              y ? y->stride_c : 1, q ? quant(q) : Quant{}, rows, cols, eps, s.tpr);
+          return launched("rms_norm launch");
+        };
+        const auto pick = [&](auto f) -> int32_t {
+          constexpr int F = decltype(f)::value;
+          return by_flag(residual, [&](auto res) {
+            constexpr bool R = decltype(res)::value;
+            if (!vec) return go(norm_kernel<T, F, R, false, kMostRounds>);
+            return s.rounds == 1 ? go(norm_kernel<T, F, R, true, 1>)
+                                 : s.rounds == 2 ? go(norm_kernel<T, F, R, true, 2>) : go(norm_kernel<T, F, R, true, kMostRounds>);
+          });
+        };
+        return q ? by_format(q->format, pick) : pick(std::integral_constant<int, FMT_NONE>{});
+      }
+    });
+  });
+}
+
+int32_t b2g_micro_rms_norm_workspace(int64_t rows, int64_t cols, size_t* bytes) {
+  return guarded([&]() -> int32_t {
+    if (rows < 0 || cols < 0 || !bytes) return record_error(B2G_ERR_INVALID_ARG, "rms_norm_workspace: bad argument");
+    *bytes = rows && cols ? static_cast<size_t>(backward_split(rows, cols).groups * cols) * sizeof(float) : 0;
+    return B2G_OK;
+  });
+}
+
+int32_t b2g_micro_rms_norm_backward(const b2g_micro_matrix* dy, const b2g_micro_matrix* h, const void* weight,
+                                    const b2g_micro_matrix* dh, const b2g_micro_matrix* dx, void* dweight,
+                                    void* workspace, size_t workspace_bytes, int64_t rows, int64_t cols, float eps,
+                                    int32_t dtype, void* stream) {
+  return guarded([&]() -> int32_t {
+    if (rows < 0 || cols < 0 || (dtype != B2G_VALUE_F16 && dtype != B2G_VALUE_BF16))
+      return record_error(B2G_ERR_INVALID_ARG, "rms_norm_backward: bad dimension or dtype");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (cols == 0) return B2G_OK;
+    if (!dweight || !weight) return record_error(B2G_ERR_INVALID_ARG, "null weight or dweight");
+    if (rows == 0) {  // a sum over no rows
+      const cudaError_t e = cudaMemsetAsync(dweight, 0, static_cast<size_t>(cols) * 2, st);
+      if (e == cudaSuccess) return B2G_OK;
+      cudaGetLastError();
+      return record_error(B2G_ERR_CUDA, std::string("memset: ") + cudaGetErrorString(e));
+    }
+    if (const int32_t rc = check_matrix(dy, "dy")) return rc;
+    if (const int32_t rc = check_matrix(h, "h")) return rc;
+    if (const int32_t rc = check_matrix(dx, "dx")) return rc;
+    if (dh)
+      if (const int32_t rc = check_matrix(dh, "dh")) return rc;
+    const Split s = backward_split(rows, cols);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < static_cast<size_t>(s.groups * cols) * sizeof(float))
+      return record_error(B2G_ERR_WORKSPACE, "rms_norm_backward: workspace missing, misaligned or too small");
+    const int64_t wgrid = ceil_div(cols, 32);
+    if (wgrid > kMaxGrid) return too_large("rms_norm_backward");
+    const bool vec = vec_ok(dy, rows, 2) && vec_ok(h, rows, 2) && vec_ok(dx, rows, 2) && (!dh || vec_ok(dh, rows, 2)) &&
+                     aligned16(weight);
+    return by_type(dtype, [&](auto t) -> int32_t {
+      using T = decltype(t);
+      if constexpr (sizeof(T) == 4) {
+        return B2G_ERR_INVALID_ARG;
+      } else {
+        const Mat none{nullptr, 0, 1};
+        const auto go = [&](auto kernel) {
+          kernel<<<static_cast<unsigned>(s.blocks), s.threads, 0, st>>>(
+              mat(dy), mat(h), static_cast<const T*>(weight), dh ? mat(dh) : none, static_cast<T*>(dx->ptr), dx->stride_r,
+              dx->stride_c, static_cast<float*>(workspace), rows, cols, eps, s.tpr);
+          return launched("rms_norm_backward launch");
+        };
+        const int32_t rc = by_flag(dh, [&](auto f) {
+          constexpr bool D = decltype(f)::value;
+          if (!vec) return go(norm_backward_kernel<T, D, false, kMostRounds>);
+          return s.rounds == 1 ? go(norm_backward_kernel<T, D, true, 1>)
+                               : s.rounds == 2 ? go(norm_backward_kernel<T, D, true, 2>) : go(norm_backward_kernel<T, D, true, kMostRounds>);
+        });
+        if (rc) return rc;
+        norm_dweight_kernel<T><<<static_cast<unsigned>(wgrid), 256, 0, st>>>(static_cast<const float*>(workspace), s.groups, cols,
+                                                                           static_cast<T*>(dweight));
+        return launched("rms_norm_backward reduce launch");
+      }
+    });
+  });
+}
+
+}  // extern "C"

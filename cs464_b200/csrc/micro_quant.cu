@@ -1,0 +1,525 @@
+// micro_quant.cu — quantisation into microscaled tensors and back, and the SiLU gate between two products.
+//
+// All of it moves bytes: the time is that of reading the values and writing codes and scales once. A warp's task is
+// 256 columns of the four rows j, j + 32, j + 64, j + 96 of a 128-row scale tile: eight columns a lane, one 16-byte load
+// a row, four loads in flight, and the four rows' scale words lie in one 16-byte piece of the tile.
+
+#include "micro_common.cuh"
+
+namespace b2g {
+namespace micro {
+
+constexpr int kWarps = 8;  // per block
+
+// ---------------------------------------------------------------- largest magnitude -> NVFP4 tensor scale
+// The smallest power of two 2^e >= 2^-100 with amax <= 2688 * 2^e (2688 = 6 * 448 = 1.3125 * 2^11). Every block takes
+// the maximum of its own candidate: the order does not matter. Infinities and NaN do not count.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kWarps * 32) tensor_scale_kernel(Mat x, int64_t rows, int64_t cols, float* scale) {
+  const int64_t chunks = (cols + 7) / 8;
+  const int64_t total = rows * chunks;
+  uint32_t m = 0;
+  const T* p = static_cast<const T*>(x.p);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total; i += 4 * step) {
+    Raw8<T> r[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t k = i + u * step;
+      const int64_t row = k < total ? k / chunks : 0;
+      const int64_t c = k < total ? (k - row * chunks) * 8 : cols;
+      r[u] = load8<T, VEC>(p + row * x.sr, x.sc, c, cols);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float v[8];
+      unpack8(r[u], v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t a = abs_bits(v[q]);
+        m = max(m, a >= 0x7f800000u ? 0u : a);
+      }
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  __shared__ uint32_t part[kWarps];
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) m = max(m, part[w]);
+    const int e = static_cast<int>(m >> 23) - 11 + ((m & 0x7fffffu) > 0x280000u ? 1 : 0);
+    atomicMax(reinterpret_cast<int*>(scale), max(e, 27) << 23);  // positive floats order as their bits do
+  }
+}
+
+// ---------------------------------------------------------------- rows -> codes and scales
+// Source of the rows' values: the values themselves, or the gate of a [gate | up] row.
+template <typename T>
+struct ValueSource {
+  static constexpr int kLoads = 1;
+  __device__ __forceinline__ static void value(const Raw8<T> (&r)[1], float (&v)[8]) { unpack8(r[0], v); }
+};
+
+// 1 / (1 + exp(-x)), the exponential and the division in their fast forms: their errors (2 + 1.173 |x| and 2 ulps) are far
+// below the rounding of any output type where the result is not itself negligible. Where exp(-x) passes 2^126 the result
+// is 0.
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
+template <typename T>
+struct GateSource {
+  static constexpr int kLoads = 2;
+  __device__ __forceinline__ static void value(const Raw8<T> (&r)[2], float (&v)[8]) {
+    float g[8], u[8];
+    unpack8(r[0], g);
+    unpack8(r[1], u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = g[i] * sigmoid(g[i]) * u[i];
+  }
+};
+
+template <typename T, int FMT, bool VEC, template <typename> class SRC>
+__global__ void __launch_bounds__(kWarps * 32)
+    quantize_rows_kernel(Mat x, int64_t rows, int64_t cols, Quant q, int64_t col_chunks, int64_t tasks) {
+  const int lane = threadIdx.x & 31;
+  const int64_t task = blockIdx.x * static_cast<int64_t>(kWarps) + (threadIdx.x >> 5);
+  if (task >= tasks) return;
+  // neighbouring warps take neighbouring column chunks of the same rows
+  const int64_t rj = task / col_chunks;
+  const int64_t c = (task - rj * col_chunks) * 256 + lane * 8;
+  const int64_t row0 = (rj >> 5) * 128 + (rj & 31);
+  const float ts = FMT == FMT_NVFP4 ? *q.scale : 0.f;
+  using S = SRC<T>;
+  Raw8<T> r[4][S::kLoads];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + 32 * i;
+#pragma unroll
+    for (int k = 0; k < S::kLoads; ++k) {
+      const T* p = static_cast<const T*>(x.p) + row * x.sr + k * cols * x.sc;
+      r[i][k] = load8<T, VEC>(p, x.sc, row < rows ? c : cols, cols);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + 32 * i;
+    float v[8];
+    S::value(r[i], v);
+    // rows past the last get zero scales and no codes
+    quantize_store<FMT>(v, lane, c, row < rows ? q.code_cols : 0, q.codes + row * q.pitch,
+                        q.scales + scale_row(row, q.ktiles), q.ktiles, ts);
+  }
+}
+
+// ---------------------------------------------------------------- columns (a transposed view) -> codes and scales
+// x has unit ROW stride: what is contiguous in memory runs along the rows of the tensor that is made, across blocks.
+// A block takes 128 rows x 128 columns; a lane holds 4 rows x 32 columns in registers (32 loads of 4 values, a warp's
+// load covering 128 consecutive values), finds its rows' largest magnitudes without any exchange, and leaves codes in
+// shared memory, from which whole rows of the tile are stored. Four warps, 32 columns each.
+template <typename T>
+struct Raw4 {
+  uint2 v;
+};
+template <>
+struct Raw4<float> {
+  uint4 v;
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack4(const Raw4<T>& r, float (&o)[4]) {
+  const float2 a = pair_f32(r.v.x, static_cast<T*>(nullptr)), b = pair_f32(r.v.y, static_cast<T*>(nullptr));
+  o[0] = a.x;
+  o[1] = a.y;
+  o[2] = b.x;
+  o[3] = b.y;
+}
+__device__ __forceinline__ void unpack4(const Raw4<float>& r, float (&o)[4]) {
+  o[0] = __uint_as_float(r.v.x);
+  o[1] = __uint_as_float(r.v.y);
+  o[2] = __uint_as_float(r.v.z);
+  o[3] = __uint_as_float(r.v.w);
+}
+
+template <typename T, int FMT, bool VEC>
+__global__ void __launch_bounds__(128) quantize_cols_kernel(Mat x, int64_t rows, int64_t cols, Quant q) {
+  constexpr int kRowBytes = FMT == FMT_MXFP8 ? 128 : 64;       // a tile row's codes
+  constexpr int kPieces = kRowBytes / 16;                      // in 16-byte pieces
+  constexpr int kWarpPieces = kPieces / 4;                     // of one warp's 32 columns: 2 or 1
+  constexpr int kBlk = block_of(FMT), kSub = 32 / kBlk;        // blocks in a warp's 32 columns: 1 or 2
+  constexpr int kScaleBytes = 128 * 4 * kSub;                  // the tile's scales: 1 or 2 tiles of 512 bytes
+  __shared__ uint4 codes[128 * kPieces];
+  __shared__ __align__(16) uint8_t scales[kScaleBytes];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t rt = blockIdx.x;                               // row tile
+  const int64_t ct = blockIdx.y;                               // 128-column tile
+  const int64_t r0 = rt * 128 + lane * 4, c0 = ct * 128 + warp * 32;
+  const T* p = static_cast<const T*>(x.p);
+  Raw4<T> raw[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const int64_t c = c0 + i;
+    const T* at = p + r0 + c * x.sc;
+    if (VEC && c < cols && r0 + 4 <= rows) {
+      raw[i].v = __ldg(reinterpret_cast<const decltype(raw[i].v)*>(at));
+    } else {
+      float f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = c < cols && r0 + k < rows ? to_f32(at[k]) : 0.f;
+      if constexpr (sizeof(T) == 4) {
+        raw[i].v = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+      } else {
+        raw[i].v = make_uint2(pack_pair(f[0], f[1], static_cast<T*>(nullptr)), pack_pair(f[2], f[3], static_cast<T*>(nullptr)));
+      }
+    }
+  }
+  const float ts = FMT == FMT_NVFP4 ? *q.scale : 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = lane * 4 + k;  // tile row
+    uint32_t word[8];            // 32 columns' codes: 8 words (e4m3) or 4 (e2m1)
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) {
+      float v[kBlk];
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < kBlk; ++i) {
+        float f[4];
+        unpack4(raw[s * kBlk + i], f);
+        v[i] = f[k];
+        m = max(m, abs_bits(v[i]));
+      }
+      BlockQuant<FMT> b;
+      b.init(m, ts);
+#pragma unroll
+      for (int g = 0; g < kBlk / 8; ++g) {
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = v[8 * g + i];
+        const uint2 w = codes8<FMT>(e, b);
+        if constexpr (FMT == FMT_MXFP8) {
+          word[2 * g] = w.x;
+          word[2 * g + 1] = w.y;
+        } else {
+          word[s * (kBlk / 8) + g] = w.x;
+        }
+      }
+      const int blk = warp * kSub + s;  // block of the tile's 4 or 8
+      scales[(blk >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (blk & 3)] = static_cast<uint8_t>(b.byte);
+    }
+#pragma unroll
+    for (int h = 0; h < kWarpPieces; ++h)  // pieces XOR-ed by the row so that a warp's stores spread over the banks
+      codes[r * kPieces + ((warp * kWarpPieces + h) ^ ((r >> 2) & (kPieces - 1)))] =
+          make_uint4(word[4 * h], word[4 * h + 1], word[4 * h + 2], word[4 * h + 3]);
+  }
+  __syncthreads();
+  const int64_t code_bytes = FMT == FMT_MXFP8 ? q.code_cols : q.code_cols / 2;
+  for (int i = threadIdx.x; i < 128 * kPieces; i += 128) {
+    const int r = i / kPieces, h = i % kPieces;
+    const int64_t at = ct * kRowBytes + h * 16;
+    if (rt * 128 + r < rows && at < code_bytes)
+      *reinterpret_cast<uint4*>(q.codes + (rt * 128 + r) * q.pitch + at) = codes[r * kPieces + (h ^ ((r >> 2) & (kPieces - 1)))];
+  }
+  if (threadIdx.x < kScaleBytes / 16) {
+    const int64_t kt = ct * kSub + threadIdx.x / 32;
+    if (kt < q.ktiles)
+      *reinterpret_cast<uint4*>(q.scales + (rt * q.ktiles + kt) * 512 + (threadIdx.x & 31) * 16) =
+          reinterpret_cast<const uint4*>(scales)[threadIdx.x];
+  }
+}
+
+// ---------------------------------------------------------------- codes and scales -> values
+// A lane reads 16 columns' codes of four rows (16 bytes each of e4m3, 8 of e2m1) and each row's one scale byte.
+template <typename T, int FMT, bool VEC>
+__global__ void __launch_bounds__(kWarps * 32)
+    dequantize_kernel(const uint8_t* codes, int64_t pitch, const uint8_t* scales, const float* scale, int64_t rows,
+                      int64_t cols, int64_t ktiles, T* out, int64_t sr, int64_t sc, int64_t col_chunks, int64_t tasks) {
+  const int lane = threadIdx.x & 31;
+  const int64_t task = blockIdx.x * static_cast<int64_t>(kWarps) + (threadIdx.x >> 5);
+  if (task >= tasks) return;
+  const int64_t rj = task / col_chunks;
+  const int64_t c = (task - rj * col_chunks) * 512 + lane * 16;
+  if (c >= cols) return;
+  const int64_t row0 = (rj >> 5) * 128 + (rj & 31);
+  const float ts = FMT == FMT_NVFP4 ? *scale : 1.f;
+  const int64_t blk = c / block_of(FMT);
+  const uint8_t* sp = scales + scale_row(row0, ktiles) + (blk >> 2) * 512 + (blk & 3);
+  uint4 q[4];
+  uint32_t s[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + 32 * i;
+    if (row < rows) {  // a row's codes are readable up to a multiple of 32 columns
+      if constexpr (FMT == FMT_MXFP8) {
+        q[i] = __ldg(reinterpret_cast<const uint4*>(codes + row * pitch + c));
+      } else {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + row * pitch + (c >> 1)));
+        q[i] = make_uint4(w.x, w.y, 0u, 0u);
+      }
+      s[i] = __ldg(sp + i * 4);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + 32 * i;
+    if (row >= rows) break;
+    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+    float bs;
+    if constexpr (FMT == FMT_NVFP4) bs = e4m3_to_f32(s[i]);
+    else bs = mx_scale_value(s[i]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        __half2_raw p;
+        if constexpr (FMT == FMT_MXFP8)
+          p = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[2 * h + k / 2] >> (16 * (k & 1))), __NV_E4M3);
+        else
+          p = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(w[h] >> (8 * k)), __NV_E2M1);
+        const float2 f = __half22float2(__half2(p));
+        // code * block scale is exact in fp32 (4 bits of e4m3 with a power of two, 2 bits of e2m1 with 4 of e4m3)
+        v[2 * k] = f.x * bs;
+        v[2 * k + 1] = f.y * bs;
+        if constexpr (FMT == FMT_NVFP4) {
+          v[2 * k] *= ts;
+          v[2 * k + 1] *= ts;
+        }
+      }
+      store8<T, VEC>(out + row * sr, sc, c + 8 * h, cols, pack8<T>(v));
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the gate as values, and its gradient
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) gate_kernel(Mat x, T* y, int64_t syr, int64_t syc, int64_t rows, int64_t cols) {
+  const int64_t chunks = (cols + 7) / 8, total = rows * chunks;
+  const int64_t k = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x;
+  if (k >= total) return;
+  const int64_t row = k / chunks, c = (k - row * chunks) * 8;
+  const T* p = static_cast<const T*>(x.p) + row * x.sr;
+  Raw8<T> r[2] = {load8<T, VEC>(p, x.sc, c, cols), load8<T, VEC>(p + cols * x.sc, x.sc, c, cols)};
+  float v[8];
+  GateSource<T>::value(r, v);
+  store8<T, VEC>(y + row * syr, syc, c, cols, pack8<T>(v));
+}
+
+// With s = sigmoid(g): d gate = dy * up * s * (1 + g * (1 - s)), d up = dy * g * s. 1 - s is taken as sigmoid(-g), which
+// keeps its digits where s is near one.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+    gate_backward_kernel(Mat dy, Mat x, T* dx, int64_t sxr, int64_t sxc, int64_t rows, int64_t cols) {
+  const int64_t chunks = (cols + 7) / 8, total = rows * chunks;
+  const int64_t k = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x;
+  if (k >= total) return;
+  const int64_t row = k / chunks, c = (k - row * chunks) * 8;
+  const T* p = static_cast<const T*>(x.p) + row * x.sr;
+  const Raw8<T> rg = load8<T, VEC>(p, x.sc, c, cols), ru = load8<T, VEC>(p + cols * x.sc, x.sc, c, cols);
+  const Raw8<T> rd = load8<T, VEC>(static_cast<const T*>(dy.p) + row * dy.sr, dy.sc, c, cols);
+  float g[8], u[8], d[8], dg[8], du[8];
+  unpack8(rg, g);
+  unpack8(ru, u);
+  unpack8(rd, d);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float e = __expf(-fabsf(g[i])), inv = __fdividef(1.f, 1.f + e);  // e <= 1: nothing overflows
+    const float s = g[i] >= 0.f ? inv : e * inv, t = g[i] >= 0.f ? e * inv : inv;  // sigmoid(g), sigmoid(-g)
+    dg[i] = d[i] * u[i] * s * (1.f + g[i] * t);
+    du[i] = d[i] * g[i] * s;
+  }
+  T* o = dx + row * sxr;
+  store8<T, VEC>(o, sxc, c, cols, pack8<T>(dg));
+  store8<T, VEC>(o + cols * sxc, sxc, c, cols, pack8<T>(du));
+}
+
+// ---------------------------------------------------------------- host side
+template <typename T, int FMT, bool VEC, template <typename> class SRC>
+int32_t run_rows(const Mat& x, int64_t rows, int64_t cols, const Quant& q, cudaStream_t st) {
+  const int64_t col_chunks = ceil_div(q.ktiles * 4 * block_of(FMT), 256);  // whole scale tiles, so that all are written
+  const int64_t tasks = ceil_div(rows, 128) * 32 * col_chunks;
+  const int64_t grid = ceil_div(tasks, kWarps);
+  if (grid > kMaxGrid) return too_large("quantisation");
+  quantize_rows_kernel<T, FMT, VEC, SRC><<<static_cast<unsigned>(grid), kWarps * 32, 0, st>>>(x, rows, cols, q, col_chunks, tasks);
+  return launched("quantize launch");
+}
+
+template <typename T, int FMT>
+int32_t run_quantize(const b2g_micro_matrix* x, const b2g_micro_tensor* t, cudaStream_t st) {
+  const Quant q = quant(t);
+  const Mat m = mat(x);
+  // Contiguous along the rows and not along the columns: the transposed kernel (4096 x 2047 bf16 through its transpose
+  // takes it from the strided loads of the other). One column is read alike by both.
+  if (x->stride_r == 1 && x->stride_c != 1 && t->cols > 1 && t->rows > 1) {
+    const int64_t gx = ceil_div(t->rows, 128), gy = ceil_div(t->cols, 128);
+    if (gy <= 65535) {
+      const bool vec = (reinterpret_cast<uintptr_t>(x->ptr) % (4 * sizeof(T))) == 0 && x->stride_c % 4 == 0;
+      const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
+      if (vec) quantize_cols_kernel<T, FMT, true><<<grid, 128, 0, st>>>(m, t->rows, t->cols, q);
+      else quantize_cols_kernel<T, FMT, false><<<grid, 128, 0, st>>>(m, t->rows, t->cols, q);
+      return launched("quantize launch");
+    }
+  }
+  if (vec_ok(x, t->rows, sizeof(T))) return run_rows<T, FMT, true, ValueSource>(m, t->rows, t->cols, q, st);
+  return run_rows<T, FMT, false, ValueSource>(m, t->rows, t->cols, q, st);
+}
+
+}  // namespace micro
+}  // namespace b2g
+
+using namespace b2g;
+using namespace b2g::micro;
+
+extern "C" {
+
+int32_t b2g_micro_layout(int32_t format, int64_t rows, int64_t cols, int64_t* pitch, int64_t* scale_bytes) {
+  return guarded([&]() -> int32_t {
+    if (format < FMT_MXFP8 || format > FMT_NVFP4 || rows < 0 || cols < 0 || !pitch || !scale_bytes)
+      return record_error(B2G_ERR_INVALID_ARG, "layout: bad format, dimension or output pointer");
+    *pitch = min_pitch(format, cols);
+    *scale_bytes = ceil_div(rows, 128) * ceil_div(cols, 4 * block_of(format)) * 512;
+    return B2G_OK;
+  });
+}
+
+int32_t b2g_micro_tensor_scale(const b2g_micro_matrix* x, int64_t rows, int64_t cols, int32_t dtype, float* scale,
+                               void* stream) {
+  return guarded([&]() -> int32_t {
+    if (rows < 0 || cols < 0 || dtype < B2G_VALUE_F16 || dtype > B2G_VALUE_F32 || !scale)
+      return record_error(B2G_ERR_INVALID_ARG, "tensor_scale: bad dimension, dtype or output pointer");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = cudaMemsetAsync(scale, 0, sizeof(float), st);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return record_error(B2G_ERR_CUDA, std::string("memset: ") + cudaGetErrorString(e));
+    }
+    if (rows && cols)
+      if (const int32_t rc = check_matrix(x, "x")) return rc;
+    const b2g_micro_matrix none = {nullptr, 0, 1};
+    if (!rows || !cols) x = &none;
+    return by_type(dtype, [&](auto t) -> int32_t {
+      using T = decltype(t);
+      Mat m = mat(x);
+      int64_t r = rows, c = cols;
+      if (x->stride_r == 1 && x->stride_c != 1) {  // the maximum does not care which way the matrix lies
+        std::swap(m.sr, m.sc);
+        std::swap(r, c);
+      }
+      const b2g_micro_matrix view = {const_cast<void*>(m.p), m.sr, m.sc};
+      const int64_t want = ceil_div(r * ceil_div(c, 8), kWarps * 32 * 4);
+      const unsigned grid = static_cast<unsigned>(want < 1 ? 1 : want > 148 * 8 ? 148 * 8 : want);
+      if (vec_ok(&view, r, sizeof(T))) tensor_scale_kernel<T, true><<<grid, kWarps * 32, 0, st>>>(m, r, c, scale);
+      else tensor_scale_kernel<T, false><<<grid, kWarps * 32, 0, st>>>(m, r, c, scale);
+      return launched("tensor_scale launch");
+    });
+  });
+}
+
+int32_t b2g_micro_quantize(const b2g_micro_matrix* x, int32_t dtype, const b2g_micro_tensor* q, void* stream) {
+  return guarded([&]() -> int32_t {
+    if (const int32_t rc = check_tensor(q, "q")) return rc;
+    if (dtype < B2G_VALUE_F16 || dtype > B2G_VALUE_F32) return record_error(B2G_ERR_INVALID_ARG, "quantize: bad dtype");
+    if (q->rows == 0 || q->cols == 0) return B2G_OK;
+    if (const int32_t rc = check_matrix(x, "x")) return rc;
+    return by_type(dtype, [&](auto t) {
+      return by_format(q->format, [&](auto f) {
+        return run_quantize<decltype(t), decltype(f)::value>(x, q, static_cast<cudaStream_t>(stream));
+      });
+    });
+  });
+}
+
+int32_t b2g_micro_dequantize(const b2g_micro_tensor* q, const b2g_micro_matrix* out, int32_t dtype, void* stream) {
+  return guarded([&]() -> int32_t {
+    if (const int32_t rc = check_tensor(q, "q")) return rc;
+    if (dtype < B2G_VALUE_F16 || dtype > B2G_VALUE_F32) return record_error(B2G_ERR_INVALID_ARG, "dequantize: bad dtype");
+    if (q->rows == 0 || q->cols == 0) return B2G_OK;
+    if (const int32_t rc = check_matrix(out, "out")) return rc;
+    const int64_t col_chunks = ceil_div(q->cols, 512), tasks = ceil_div(q->rows, 128) * 32 * col_chunks;
+    const int64_t grid = ceil_div(tasks, kWarps);
+    if (grid > kMaxGrid) return too_large("dequantisation");
+    return by_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      return by_format(q->format, [&](auto f) -> int32_t {
+        constexpr int F = decltype(f)::value;
+        const auto go = [&](auto kernel) {
+          kernel<<<static_cast<unsigned>(grid), kWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(
+              static_cast<const uint8_t*>(q->codes), q->pitch, static_cast<const uint8_t*>(q->scales), q->scale, q->rows,
+              q->cols, ceil_div(q->cols, 4 * block_of(F)), static_cast<T*>(out->ptr), out->stride_r, out->stride_c,
+              col_chunks, tasks);
+        };
+        if (vec_ok(out, q->rows, sizeof(T))) go(dequantize_kernel<T, F, true>);
+        else go(dequantize_kernel<T, F, false>);
+        return launched("dequantize launch");
+      });
+    });
+  });
+}
+
+int32_t b2g_micro_silu_mul(const b2g_micro_matrix* gate_up, const b2g_micro_matrix* y, const b2g_micro_tensor* q,
+                           int64_t rows, int64_t cols, int32_t dtype, void* stream) {
+  return guarded([&]() -> int32_t {
+    if (rows < 0 || cols < 0 || (dtype != B2G_VALUE_F16 && dtype != B2G_VALUE_BF16) || (!y && !q) || (y && q))
+      return record_error(B2G_ERR_INVALID_ARG, "silu_mul: bad dimension or dtype, or not one output");
+    if (q) {
+      if (const int32_t rc = check_tensor(q, "q")) return rc;
+      if (q->rows != rows || q->cols != cols) return record_error(B2G_ERR_INVALID_ARG, "silu_mul: q is not [rows, cols]");
+    }
+    if (rows == 0 || cols == 0) return B2G_OK;
+    if (const int32_t rc = check_matrix(gate_up, "gate_up")) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return by_type(dtype, [&](auto t) -> int32_t {
+      using T = decltype(t);
+      if constexpr (sizeof(T) == 4) {
+        return B2G_ERR_INVALID_ARG;
+      } else {
+        const bool vec = vec_ok(gate_up, rows, 2) && cols % 8 == 0;  // the up half starts `cols` values into the row
+        if (q) {
+          return by_format(q->format, [&](auto f) {
+            constexpr int F = decltype(f)::value;
+            return vec ? run_rows<T, F, true, GateSource>(mat(gate_up), rows, cols, quant(q), st)
+                       : run_rows<T, F, false, GateSource>(mat(gate_up), rows, cols, quant(q), st);
+          });
+        }
+        if (const int32_t rc = check_matrix(y, "y")) return rc;
+        const int64_t grid = ceil_div(rows * ceil_div(cols, 8), 256);
+        if (grid > kMaxGrid) return too_large("silu_mul");
+        if (vec && vec_ok(y, rows, 2))
+          gate_kernel<T, true><<<static_cast<unsigned>(grid), 256, 0, st>>>(mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols);
+        else
+          gate_kernel<T, false><<<static_cast<unsigned>(grid), 256, 0, st>>>(mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols);
+        return launched("silu_mul launch");
+      }
+    });
+  });
+}
+
+int32_t b2g_micro_silu_mul_backward(const b2g_micro_matrix* dy, const b2g_micro_matrix* gate_up,
+                                    const b2g_micro_matrix* dgate_up, int64_t rows, int64_t cols, int32_t dtype,
+                                    void* stream) {
+  return guarded([&]() -> int32_t {
+    if (rows < 0 || cols < 0 || (dtype != B2G_VALUE_F16 && dtype != B2G_VALUE_BF16))
+      return record_error(B2G_ERR_INVALID_ARG, "silu_mul_backward: bad dimension or dtype");
+    if (rows == 0 || cols == 0) return B2G_OK;
+    if (const int32_t rc = check_matrix(dy, "dy")) return rc;
+    if (const int32_t rc = check_matrix(gate_up, "gate_up")) return rc;
+    if (const int32_t rc = check_matrix(dgate_up, "dgate_up")) return rc;
+    const int64_t grid = ceil_div(rows * ceil_div(cols, 8), 256);
+    if (grid > kMaxGrid) return too_large("silu_mul_backward");
+    return by_type(dtype, [&](auto t) -> int32_t {
+      using T = decltype(t);
+      if constexpr (sizeof(T) == 4) {
+        return B2G_ERR_INVALID_ARG;
+      } else {
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        T* out = static_cast<T*>(dgate_up->ptr);
+        if (vec_ok(dy, rows, 2) && vec_ok(gate_up, rows, 2) && vec_ok(dgate_up, rows, 2) && cols % 8 == 0)
+          gate_backward_kernel<T, true><<<static_cast<unsigned>(grid), 256, 0, st>>>(mat(dy), mat(gate_up), out, dgate_up->stride_r, dgate_up->stride_c, rows, cols);
+        else
+          gate_backward_kernel<T, false><<<static_cast<unsigned>(grid), 256, 0, st>>>(mat(dy), mat(gate_up), out, dgate_up->stride_r, dgate_up->stride_c, rows, cols);
+        return launched("silu_mul_backward launch");
+      }
+    });
+  });
+}
+
+}  // extern "C"

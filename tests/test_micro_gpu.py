@@ -1,0 +1,695 @@
+"""The microscaled operators on a B200 against 64-bit references (oracle/micro.py for the formats, formulas here for the
+layers). Quantisation is compared bit for bit; where values are computed, each tolerance is derived beside it."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from cs464_b200 import micro
+from cs464_b200.suites import LLAMA_LAYERS, WEIGHT_STD
+from oracle import micro as om
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = tuple(micro.FORMATS)
+HALF = (torch.float16, torch.bfloat16)
+ALL = (*HALF, torch.float32)
+
+
+def half_step(dtype) -> float:
+    return torch.finfo(dtype).eps / 2
+
+
+def normal(*shape, dtype=torch.bfloat16, seed=0, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g, dtype=torch.float64) * std).to(dtype).cuda()
+
+
+def f64(t: torch.Tensor) -> np.ndarray:
+    return t.detach().double().cpu().numpy()
+
+
+def stored(q: micro.MicroTensor):
+    """(codes, scale bytes) of a MicroTensor; everything outside them must be zero."""
+    c, s, zero = om.unpack(q.codes.cpu().numpy(), q.scales.cpu().numpy(), *q.shape, q.format)
+    assert zero, "bytes outside the tensor's codes and scales are not zero"
+    return c, s
+
+
+def check_quantized(q: micro.MicroTensor, x: np.ndarray):
+    g = None if q.scale is None else float(q.scale)
+    c, s = stored(q)
+    rc, rs = om.quantize(x, q.format, g)
+    assert np.array_equal(s, rs), (s != rs).sum()
+    assert np.array_equal(c, rc), ((c != rc).sum(), c[c != rc][:4], rc[c != rc][:4])
+
+
+# ---------------------------------------------------------------- quantise and dequantise
+SHAPES = [(1, 1), (1, 31), (3, 33), (1, 4096), (16, 128), (33, 96), (127, 257), (128, 128), (129, 1000), (300, 64), (257, 4)]
+
+
+def views(rows, cols, dtype, seed):
+    """The same values through different strides and alignments."""
+    x = normal(rows, cols, dtype=dtype, seed=seed) * torch.exp2(
+        torch.arange(cols, device="cuda") % 7 - 3).to(dtype)
+    yield "contiguous", x
+    yield "transposed", x.t().contiguous().t()
+    wide = torch.zeros(rows, cols + 3, dtype=dtype, device="cuda")
+    wide[:, 1:cols + 1] = x
+    yield "odd rows", wide[:, 1:cols + 1]
+    tall = torch.zeros(cols, rows + 3, dtype=dtype, device="cuda")
+    tall[:, 1:rows + 1] = x.t()
+    yield "odd columns", tall[:, 1:rows + 1].t()
+    step = torch.zeros(2 * rows, 3 * cols, dtype=dtype, device="cuda")
+    step[::2, ::3] = x
+    yield "steps", step[::2, ::3]
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_bit_for_bit(fmt, dtype):
+    for i, (rows, cols) in enumerate(SHAPES):
+        for name, x in views(rows, cols, dtype, i):
+            q = micro.quantize(x, fmt)
+            if fmt == "nvfp4":
+                assert float(q.scale) == om.tensor_scale(f64(x)), name
+            check_quantized(q, f64(x))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_special_values(fmt, dtype):
+    """Infinities, NaN, both zeros, the type's extremes and subnormals, ties, blocks of zeros: alone in a block and among
+    ordinary values, by rows and through a transpose."""
+    info = torch.finfo(dtype)
+    special = [float("inf"), -float("inf"), float("nan"), 0.0, -0.0, info.max, info.min, info.tiny, info.tiny / 8,
+               info.smallest_normal * 1.5, 6.0, 448.0, 0.25, 2.5, 5.0]
+    x = torch.zeros(len(special) * 3, 96, dtype=dtype)
+    for i, v in enumerate(special):
+        x[3 * i, 5] = v                      # alone in its block of zeros
+        x[3 * i + 1, :] = 1.0
+        x[3 * i + 1, 40] = v                 # among ones; the other blocks of the row keep theirs
+        x[3 * i + 2, :] = v                  # the whole row
+    x = x.cuda()
+    with np.errstate(all="ignore"):
+        for t in (x, x.t().contiguous().t(), x.t()):
+            q = micro.quantize(t, fmt)
+            check_quantized(q, f64(t))
+            d = q.dequantize(torch.float32)
+            c, s = om.quantize(f64(t), fmt, None if q.scale is None else float(q.scale))
+            v = om.values(c, s, fmt, None if q.scale is None else float(q.scale))
+            assert np.array_equal(np.isnan(f64(d)), np.isnan(v))
+
+
+def test_nvfp4_given_scale_and_saturation():
+    x = normal(65, 160, dtype=torch.float32, seed=3)
+    for g in (2.0 ** -9, 0.25, 1.0 / 448, 3.3e-4, 100.0):
+        q = micro.quantize(x, "nvfp4", scale=torch.full((1,), g, device="cuda"))
+        g32 = float(np.float32(g))
+        c, s = stored(q)
+        rc, rs = om.quantize(f64(x), "nvfp4", g32)
+        # a scale that is no power of two makes unit = block scale * g round in fp32: a value within an fp32 half step
+        # (relative 2^-24, twice) of the border between two codes may fall on its other side. Count those borders.
+        v = np.abs(f64(x)).reshape(65, -1, 16) / (om.E4M3[rs] * g32)[..., None]
+        with np.errstate(invalid="ignore"):
+            near = (np.abs(v[..., None] / np.array([.25, .75, 1.25, 1.75, 2.5, 3.5, 5.0]) - 1) < 2.0 ** -22).any(-1)
+        assert np.array_equal(s, rs) and ((c != rc) <= near.reshape(c.shape)).all()
+    top = micro.quantize(torch.full((1, 16), 1e6, device="cuda"), "nvfp4", scale=torch.ones(1, device="cuda"))
+    assert (f64(top.dequantize(torch.float32)) == 2688.0).all()
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_dequantize(fmt, dtype):
+    for rows, cols in SHAPES:
+        x = normal(rows, cols, dtype=torch.float32, seed=rows)
+        q = micro.quantize(x, fmt)
+        g = None if q.scale is None else float(q.scale)
+        v = om.values(*om.quantize(f64(x), fmt, g), fmt, g)
+        # code * scale has at most 6 significant bits and the tensor scale is a power of two: fp32 holds it, bf16 too;
+        # fp16 also where it is in range, which |x| < 8 is but for scales below its subnormals' step, 2^-24
+        want = torch.from_numpy(v).to(dtype)
+        out = q.dequantize(dtype).cpu()
+        assert torch.equal(out, want), (rows, cols)
+        place = torch.full((rows + 1, 2 * cols + 1), 7.0, dtype=dtype, device="cuda")
+        micro.dequantize(q, out=place[:rows, 1::2])
+        assert torch.equal(place[:rows, 1::2].cpu(), want)
+        assert (place[rows:] == 7).all() and (place[:, 0::2] == 7).all()  # what is not q's stays as it was
+
+
+# ---------------------------------------------------------------- products
+def random_operand(rows, cols, fmt, seed, std=1.0):
+    q = micro.quantize(normal(rows, cols, dtype=torch.float32, seed=seed, std=std), fmt)
+    g = None if q.scale is None else float(q.scale)
+    return q, om.values(*stored(q), fmt, g)
+
+
+def check_product(c: torch.Tensor, a: np.ndarray, b: np.ndarray):
+    """|c - ref| <= half a step of the output's type + the accumulation's error. One MMA adds the exact products of its K
+    step (32 or 64 columns) to an fp32 accumulator; a rounding or truncation there loses at most 2^-22 of the largest
+    partial sum, itself at most S = sum |a| |b|. ceil(K / 32) steps, up to 8 sums across K splits, one scaling."""
+    ref = a @ b.T
+    bound = half_step(c.dtype) * np.abs(ref) + (-(-a.shape[1] // 32) + 9) * 2.0 ** -22 * (np.abs(a) @ np.abs(b).T)
+    bound += 2.0 ** -25 if c.dtype == torch.float16 else 0  # half of fp16's smallest subnormal
+    err = np.abs(f64(c) - ref)
+    assert np.isfinite(f64(c)).all() and (err <= bound).all(), (err - bound).max()
+
+
+PRODUCTS = [(1, 1, 1), (1, 128, 256), (1, 1000, 4096), (7, 130, 96), (16, 4096, 33), (17, 257, 500), (33, 96, 1031),
+            (64, 512, 2048), (65, 127, 64), (128, 384, 640), (129, 129, 129), (200, 1024, 300), (300, 264, 1500),
+            (5, 8, 14336), (512, 640, 256), (1024, 768, 320), (1000, 1111, 777)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_product(fmt, dtype):
+    for i, (m, n, k) in enumerate(PRODUCTS):
+        qa, a = random_operand(m, k, fmt, 2 * i)
+        qb, b = random_operand(n, k, fmt, 2 * i + 1, std=0.05)
+        check_product(micro.micro_matmul(qa, qb, dtype=dtype), a, b)
+    micro.check_status()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_product_every_k(fmt):
+    """K from one column over the ends of blocks, scale tiles, MMA steps and stages: codes past K do not exist, and what
+    lies in the ring's shared memory there is left from earlier stages."""
+    for k in [*range(1, 70, 7), 95, 97, 127, 128, 129, 191, 193, 255, 256, 257, 320, 383, 385, 511, 513, 1023, 1025]:
+        qa, a = random_operand(40, k, fmt, k)
+        qb, b = random_operand(70, k, fmt, k + 1)
+        check_product(micro.micro_matmul(qa, qb), a, b)
+
+
+@pytest.mark.parametrize("layer", list(LLAMA_LAYERS))
+def test_product_llama_layers(layer):
+    """The layers' projections at decode and prefill sizes, 512 of the output columns checked in 64 bits."""
+    k, n = LLAMA_LAYERS[layer]
+    for fmt in FORMATS:
+        qb = micro.quantize(normal(n, k, dtype=torch.float32, std=WEIGHT_STD), fmt)
+        at = torch.randperm(n, generator=torch.Generator().manual_seed(1))[:512].cuda()
+        b = qb.dequantize(torch.float32)[at].double()
+        for m in (1, 16, 128, 2048):
+            qa = micro.quantize(normal(m, k, dtype=torch.float32, seed=m), fmt)
+            a = qa.dequantize(torch.float32).double()
+            c = micro.micro_matmul(qa, qb)[:, at].double()
+            ref, s = a @ b.T, a.abs() @ b.abs().T
+            bound = half_step(torch.bfloat16) * ref.abs() + (-(-k // 32) + 9) * 2.0 ** -22 * s  # as in check_product
+            assert ((c - ref).abs() <= bound).all(), (layer, fmt, m)
+    micro.check_status()
+
+
+def test_product_of_nan_blocks_stays_in_its_rows():
+    """A NaN scale makes its own row (or column) of the product NaN and nothing else, in every format."""
+    for fmt in FORMATS:
+        x, w = normal(40, 256, dtype=torch.float32), normal(300, 256, dtype=torch.float32, seed=1)
+        x[7, 200] = float("inf")
+        w[299, 3] = float("nan")
+        qa = micro.quantize(x, fmt)
+        qb = micro.quantize(w, fmt)
+        c = f64(micro.micro_matmul(qa, qb))
+        bad = np.zeros((40, 300), bool)
+        bad[7], bad[:, 299] = True, True
+        assert np.array_equal(np.isnan(c), bad), fmt
+
+
+def test_product_output_views_and_empty():
+    for fmt in FORMATS:
+        qa, a = random_operand(37, 200, fmt, 1)
+        qb, b = random_operand(61, 200, fmt, 2)
+        for start, width in ((0, 64), (8, 72), (1, 63), (3, 70)):  # aligned and odd rows
+            big = torch.full((40, width + start), 5.0, dtype=torch.bfloat16, device="cuda")
+            out = big[:37, start:start + 61]
+            assert micro.micro_matmul(qa, qb, out=out) is out
+            check_product(out, a, b)
+            assert (big[37:] == 5).all() and (big[:, :start] == 5).all() and (big[:, start + 61:] == 5).all()
+        one = torch.empty(1, 61, dtype=torch.float16, device="cuda").as_strided((1, 61), (7, 1))
+        qa1, a1 = random_operand(1, 200, fmt, 3)
+        check_product(micro.micro_matmul(qa1, qb, out=one), a1, b)
+        no_k = [micro.quantize(torch.empty(n, 0, device="cuda"), fmt) for n in (5, 6)]
+        assert (micro.micro_matmul(*no_k) == 0).all()
+        none = micro.quantize(torch.empty(0, 200, device="cuda"), fmt)
+        assert micro.micro_matmul(none, qb).shape == (0, 61) and micro.micro_matmul(qa, none).shape == (37, 0)
+
+
+def test_product_repeats_bit_for_bit_and_runner():
+    for fmt in FORMATS:
+        for m, n, k in ((1, 4096, 4096), (130, 1000, 2000), (1024, 2048, 512)):
+            qa, _ = random_operand(m, k, fmt, 1)
+            qb, _ = random_operand(n, k, fmt, 2)
+            first = micro.micro_matmul(qa, qb)
+            run = micro.MicroMatmul().make_runner(qa, qb)
+            for _ in range(3):
+                assert torch.equal(run(), first)
+            run.raise_on_status()
+
+
+def test_product_refusals():
+    x = normal(4, 64)
+    q8, q4, qn = (micro.quantize(x, f) for f in FORMATS)
+    with pytest.raises(ValueError, match="one format"):
+        micro.micro_matmul(q8, q4)
+    with pytest.raises(ValueError, match="must agree"):
+        micro.micro_matmul(q8, micro.quantize(normal(4, 32), "mxfp8"))
+    with pytest.raises(TypeError, match="float16 or bfloat16"):
+        micro.micro_matmul(q8, q8, dtype=torch.float32)
+    for out in (torch.empty(4, 5, dtype=torch.bfloat16, device="cuda"),
+                torch.empty(4, 4, dtype=torch.bfloat16, device="cuda").t(),
+                torch.empty(1, 4, dtype=torch.bfloat16, device="cuda").expand(4, 4)):
+        with pytest.raises(ValueError, match="out must be"):
+            micro.micro_matmul(q8, q8, out=out)
+    with pytest.raises(TypeError, match="out must be"):
+        micro.micro_matmul(q8, q8, out=torch.empty(4, 4, device="cuda"))
+    with pytest.raises(ValueError, match="codes of a"):
+        micro.MicroTensor(q8.codes[:, :32], q8.scales, (4, 64), "mxfp8")
+    with pytest.raises(ValueError, match="codes of a"):
+        micro.MicroTensor(q8.codes[:, 1:], q8.scales, (4, 33), "mxfp8")
+    with pytest.raises(ValueError, match="scales of a"):
+        micro.MicroTensor(q8.codes, q8.scales[:-1], (4, 64), "mxfp8")
+    with pytest.raises(ValueError, match="no tensor scale"):
+        micro.MicroTensor(q8.codes, q8.scales, (4, 64), "mxfp8", torch.ones(1, device="cuda"))
+    with pytest.raises(ValueError, match="scale must be"):
+        micro.MicroTensor(qn.codes, qn.scales, (4, 64), "nvfp4")
+    with pytest.raises(ValueError, match="scale must be"):
+        micro.quantize(x, "nvfp4", scale=torch.ones(1))
+    with pytest.raises(ValueError, match="no tensor scale"):
+        micro.quantize(x, "mxfp4", scale=torch.ones(1, device="cuda"))
+    with pytest.raises(TypeError, match="x must be"):
+        micro.quantize(x.double(), "mxfp8")
+    with pytest.raises(ValueError, match="a matrix"):
+        micro.quantize(x[0], "mxfp8")
+    with pytest.raises(TypeError, match="packed"):
+        q4.code_values()
+
+
+# ---------------------------------------------------------------- norm
+def norm64(x, w, eps, res=None):
+    h = x if res is None else x + res
+    return h * w / np.sqrt((h * h).mean(1, keepdims=True) + eps), h
+
+
+def norm_tolerance(y, dtype):
+    """Half a step of the output's type, and in fp32 the sum of squares (pairwise over threads: a few tens of roundings of
+    2^-24), a reciprocal root of two ulps and three products: below 2^-18 in all."""
+    return (half_step(dtype) + 2.0 ** -18) * np.abs(y) + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -130)
+
+
+NORMS = [(1, 1), (1, 4096), (2, 7), (5, 64), (3, 1000), (130, 129), (600, 72), (33, 2048), (700, 520), (4, 8200), (2, 16384),
+         (3, 16392), (2, 40001)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_norm_values(dtype):
+    for i, (rows, cols) in enumerate(NORMS):
+        x, r = normal(rows, cols, dtype=dtype, seed=i), normal(rows, cols, dtype=dtype, seed=i + 50, std=2.0)
+        w = normal(cols, dtype=dtype, seed=i + 99)
+        for res in (None, r):
+            y, h = micro.rms_norm(x, w, residual=res, eps=1e-5)
+            ry, rh = norm64(f64(x), f64(w), 1e-5, None if res is None else f64(res))
+            assert (np.abs(f64(y) - ry) <= norm_tolerance(ry, dtype)).all(), (rows, cols)
+            # the sum of two values of the type in fp32 (half an ulp of fp32 at most), then rounded
+            assert (np.abs(f64(h) - rh) <= (half_step(dtype) + 2.0 ** -24) * np.abs(rh)).all()
+            assert h is x if res is None else True
+
+
+def check_coded(q: micro.MicroTensor, y: np.ndarray, slack: float):
+    """q holds y, known to the kernel up to a relative error `slack`: every value is within half a step of its code
+    (relative to the block scale that q uses) plus that error, and every block scale is the definition's or, where the
+    largest magnitude lies within `slack` of the border between two, its neighbour."""
+    fmt = q.format
+    g = None if q.scale is None else float(q.scale)
+    c, s = stored(q)
+    _, rs = om.quantize(y, fmt, g)
+    lo = om.quantize(y * (1 - slack), fmt, g)[1].astype(int)
+    hi = om.quantize(y * (1 + slack), fmt, g)[1].astype(int)
+    assert ((s >= lo) & (s <= hi)).all()
+    assert (s != rs).mean() < 0.01
+    v = om.values(c, s, fmt, g)
+    with np.errstate(divide="ignore"):
+        unit = np.repeat(om.E4M3[s] * g if fmt == "nvfp4" else 2.0 ** (s.astype(int) - 127.0), om.BLOCK[fmt], 1)[:, :y.shape[1]]
+    u = np.abs(y) / np.where(unit > 0, unit, np.inf)
+    if fmt == "mxfp8":
+        step = 2.0 ** (np.maximum(np.floor(np.log2(np.maximum(u, 2.0 ** -6))), -6) - 3)
+        top = 448.0
+    else:
+        step = np.where(u < 2, 0.5, np.where(u < 4, 1.0, 2.0))
+        top = 6.0
+    tol = (step / 2 + 2 * slack * u + np.maximum(u - top, 0)) * unit
+    zero = unit == 0  # an nvfp4 block whose scale rounds to zero is zero
+    assert (np.abs(v - y)[~zero] <= tol[~zero] * (1 + 1e-9)).all() and (v[zero] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_norm_coded(fmt, dtype):
+    for i, (rows, cols) in enumerate(NORMS):
+        x, r = normal(rows, cols, dtype=dtype, seed=i), normal(rows, cols, dtype=dtype, seed=i + 50)
+        w = normal(cols, dtype=dtype, seed=i + 99)
+        scale = torch.full((1,), 0.01, device="cuda") if fmt == "nvfp4" else None
+        for res in (None, r):
+            q, h = micro.rms_norm(x, w, residual=res, format=fmt, scale=scale)
+            ry, rh = norm64(f64(x), f64(w), 1e-5, None if res is None else f64(res))
+            check_coded(q, ry, 2.0 ** -18)
+            assert (np.abs(f64(h) - rh) <= (half_step(dtype) + 2.0 ** -24) * np.abs(rh)).all()
+
+
+def test_norm_of_strided_and_special_rows():
+    """Views of every kind, rows of zeros, infinities and NaN; a row that is not finite leaves the others alone."""
+    base = normal(40, 300, seed=3)
+    w = normal(256, seed=4)
+    for x in (base[:33, 4:260], base[:33, 40:296], normal(256, 33, seed=5).t(), normal(1, 256, seed=6).expand(33, 256),
+              normal(66, 512, seed=7)[::2, ::2]):
+        ry, _ = norm64(f64(x), f64(w), 1e-5)
+        assert (np.abs(f64(micro.rms_norm(x, w)[0]) - ry) <= norm_tolerance(ry, torch.bfloat16)).all()
+        check_coded(micro.rms_norm(x, w, format="mxfp8")[0], ry, 2.0 ** -18)
+        ry, _ = norm64(f64(x), f64(w), 1e-5, f64(base[:33, 7:263]))
+        y, _ = micro.rms_norm(x, w, residual=base[:33, 7:263])
+        assert (np.abs(f64(y) - ry) <= norm_tolerance(ry, torch.bfloat16)).all()
+    x = normal(6, 256, seed=8)
+    x[1] = 0
+    x[2, 3], x[4, 5] = float("inf"), float("nan")
+    y = micro.rms_norm(x, w)[0]
+    d = micro.rms_norm(x, w, format="mxfp8")[0].dequantize()
+    good = [0, 1, 3, 5]
+    ry, _ = norm64(f64(x)[good], f64(w), 1e-5)
+    assert (np.abs(f64(y)[good] - ry) <= norm_tolerance(ry, torch.bfloat16)).all()
+    assert np.isfinite(f64(d)[good]).all() and (f64(y)[1] == 0).all() and (f64(d)[1] == 0).all()
+    assert np.isnan(f64(y)[4]).all() and np.isnan(f64(y)[2, 3]) and np.isnan(f64(d)[4]).all()
+    assert micro.rms_norm(x[:0], w)[0].shape == (0, 256)
+    y3, h3 = micro.rms_norm(x[good].view(2, 2, 256), w, residual=x[good].view(2, 2, 256))
+    assert y3.shape == h3.shape == (2, 2, 256)
+
+
+def norm_grad64(dy, h, w, eps, dh=None):
+    n = h.shape[1]
+    r = 1.0 / np.sqrt((h * h).mean(1, keepdims=True) + eps)
+    dot = (dy * w * h).sum(1, keepdims=True)
+    dx = r * dy * w - h * r ** 3 * dot / n
+    return dx + (0 if dh is None else dh), (dy * h * r).sum(0), r
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_norm_backward(dtype):
+    for i, (rows, cols) in enumerate(NORMS + [(3000, 64), (1500, 1024)]):
+        dy, h = normal(rows, cols, dtype=dtype, seed=i), normal(rows, cols, dtype=dtype, seed=i + 20)
+        w, dh = normal(cols, dtype=dtype, seed=i + 40), normal(rows, cols, dtype=dtype, seed=i + 60)
+        for extra in (None, dh):
+            dx, dw = micro.rms_norm_backward(dy, h, w, 1e-5, dh=extra)
+            a, b, c = f64(dy), f64(h), f64(w)
+            rx, rw, r = norm_grad64(a, b, c, 1e-5, None if extra is None else f64(extra))
+            # dx: half a step of the type, and fp32 errors below 2^-18 of the terms' magnitudes (as in norm_tolerance;
+            # the mean's against the sum of its terms' magnitudes)
+            mag = np.abs(a * c) * r + np.abs(b) * r ** 3 * np.abs(a * b * c).mean(1, keepdims=True)
+            tiny = 2.0 ** -25 if dtype == torch.float16 else 0
+            assert (np.abs(f64(dx) - rx) <= half_step(dtype) * np.abs(rx) + 2.0 ** -18 * (mag + np.abs(rx)) + tiny).all(), (rows, cols)
+            # dw: a sum over the rows in fp32, at most rows additions of 2^-24 each of the terms' sum
+            tol = half_step(dtype) * np.abs(rw) + (2.0 ** -18 + rows * 2.0 ** -24) * np.abs(a * b * r).sum(0) + tiny
+            assert (np.abs(f64(dw) - rw) <= tol).all(), (rows, cols)
+            again = micro.rms_norm_backward(dy, h, w, 1e-5, dh=extra)
+            assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
+
+
+def test_norm_gradient_formula_against_differences():
+    """The formula the gradients are tested against, by central differences of the 64-bit forward pass."""
+    rng = np.random.default_rng(0)
+    x, w, dy, dh = rng.normal(size=(3, 9)), rng.normal(size=9), rng.normal(size=(3, 9)), rng.normal(size=(3, 9))
+    dx, dw, _ = norm_grad64(dy, x, w, 1e-5, dh)
+    loss = lambda x, w: (norm64(x, w, 1e-5)[0] * dy).sum() + (x * dh).sum()  # noqa: E731
+    e = 1e-6
+    for i in np.ndindex(x.shape):
+        d = np.zeros_like(x)
+        d[i] = e
+        assert abs((loss(x + d, w) - loss(x - d, w)) / (2 * e) - dx[i]) < 1e-7
+    for i in range(9):
+        d = np.zeros(9)
+        d[i] = e
+        assert abs((loss(x, w + d) - loss(x, w - d)) / (2 * e) - dw[i]) < 1e-7
+
+
+def test_norm_autograd_with_shared_and_broadcast_inputs():
+    """Gradients through autograd: strided and expanded upstream gradients, either output unused, x used twice."""
+    x0, r0, w0 = normal(20, 72, seed=1), normal(20, 72, seed=2), normal(72, seed=3)
+    for use in ("both", "y", "h", "same"):
+        x, r, w = (t.clone().requires_grad_() for t in (x0, r0, w0))
+        y, h = micro.rms_norm(x, w, residual=x if use == "same" else r)
+        gy, gh = normal(72, 20, seed=4).t(), normal(20, 1, seed=5).expand(20, 72)
+        loss = (y * gy).sum() if use != "h" else 0
+        loss = loss + ((h * gh).sum() if use != "y" else 0)
+        loss.backward()
+        hr = f64(h)
+        rx, rw, _ = norm_grad64(f64(gy) * (use != "h"), hr, f64(w0), 1e-5, f64(gh) * (use != "y"))
+        tol = half_step(torch.bfloat16) * np.abs(rx) + 2.0 ** -16 * (np.abs(rx).max() + 1)
+        if use == "same":  # two contributions of dx, added in bf16
+            assert (np.abs(f64(x.grad) - 2 * rx) <= 4 * tol).all()
+        else:
+            assert (np.abs(f64(x.grad) - rx) <= tol).all() and torch.equal(x.grad, r.grad)
+        if use == "h":
+            assert w.grad is None or (w.grad == 0).all()
+        else:
+            assert (np.abs(f64(w.grad) - rw) <= half_step(torch.bfloat16) * np.abs(rw) + 1e-3).all()
+    x = x0.clone().requires_grad_()
+    y, h = micro.rms_norm(x, w0)
+    assert h is x
+    (g,) = torch.autograd.grad(y.sum(), x)
+    rx, _, _ = norm_grad64(np.ones((20, 72)), f64(x0), f64(w0), 1e-5)
+    assert (np.abs(f64(g) - rx) <= half_step(torch.bfloat16) * np.abs(rx) + 2.0 ** -16 * (np.abs(rx).max() + 1)).all()
+    with pytest.raises(ValueError, match="no gradient"):
+        micro.rms_norm(x, w0, format="mxfp8")
+    with torch.no_grad():
+        micro.rms_norm(x, w0, format="mxfp8")
+
+
+def test_layer_refusals():
+    x, w = normal(4, 64), normal(64)
+    with pytest.raises(ValueError, match="weight must be"):
+        micro.rms_norm(x, w[:63])
+    with pytest.raises(TypeError, match="weight must be bfloat16"):
+        micro.rms_norm(x, w.half())
+    with pytest.raises(TypeError, match="x must be"):
+        micro.rms_norm(x.float(), w.float())
+    with pytest.raises(ValueError, match="residual is"):
+        micro.rms_norm(x, w, residual=x[:3])
+    with pytest.raises(ValueError, match="nvfp4 needs"):
+        micro.rms_norm(x, w, format="nvfp4")
+    with pytest.raises(ValueError, match="no tensor scale"):
+        micro.rms_norm(x, w, format="mxfp8", scale=torch.ones(1, device="cuda"))
+    with pytest.raises(ValueError, match="scale belongs"):
+        micro.rms_norm(x, w, scale=torch.ones(1, device="cuda"))
+    with pytest.raises(ValueError, match="one shape"):
+        micro.rms_norm_backward(x[:3], x, w)
+    with pytest.raises(ValueError, match=r"\[gate \| up\]"):
+        micro.silu_mul(x[:, :63])
+    with pytest.raises(ValueError, match="dy is"):
+        micro.silu_mul_backward(x, x)
+    with pytest.raises(ValueError, match="x must be"):
+        micro.micro_linear(x, normal(8, 63))
+    with pytest.raises(TypeError, match="w must be bfloat16"):
+        micro.micro_linear(x, normal(8, 64).half())
+
+
+# ---------------------------------------------------------------- gate
+def gate64(x):
+    c = x.shape[1] // 2
+    g, u = x[:, :c], x[:, c:]
+    with np.errstate(over="ignore"):
+        return g / (1 + np.exp(-g)) * u
+
+
+def gate_grad64(dy, x):
+    c = x.shape[1] // 2
+    g, u = x[:, :c], x[:, c:]
+    with np.errstate(over="ignore"):
+        s = 1 / (1 + np.exp(-g))
+    return np.concatenate([dy * u * s * (1 + g * (1 - s)), dy * g * s], 1)
+
+
+GATES = [(1, 1), (1, 14336), (3, 5), (2, 31), (130, 33), (64, 128), (129, 1000), (40, 1096), (2047, 72)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_gate(dtype):
+    """The fast exponential errs by at most 2 + 1.173 |gate| ulps (25 of 2^-23 for the |gate| < 20 here, below 2^-18.3),
+    the division by 2 ulps, two products and a sum by half an ulp each: below 2^-18 in all."""
+    for i, (rows, cols) in enumerate(GATES):
+        wide = normal(rows, 2 * cols + 5, dtype=dtype, seed=i, std=4.0)
+        for x in (wide[:, :2 * cols], wide[:, 5:], wide.contiguous()[:, 1:2 * cols + 1], wide[:, :2 * cols].t().contiguous().t(),
+                  wide[:, :2 * cols].contiguous()):
+            ry = gate64(f64(x))
+            tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -130
+            y = micro.silu_mul(x)
+            assert (np.abs(f64(y) - ry) <= (half_step(dtype) + 2.0 ** -18) * np.abs(ry) + tiny).all(), (rows, cols)
+            for fmt in FORMATS:
+                q = micro.silu_mul(x, format=fmt, scale=torch.full((1,), 0.05, device="cuda") if fmt == "nvfp4" else None)
+                check_coded(q, ry, 2.0 ** -18)
+            dy = normal(rows, cols, dtype=dtype, seed=i + 30)
+            a, b = f64(dy), f64(x)
+            rg = gate_grad64(a, b)
+            # 1 + g (1 - s) cancels near g = -1.28: its error is against the terms' magnitudes
+            c = cols
+            s = 1 / (1 + np.exp(-b[:, :c]))
+            mag = np.concatenate([np.abs(a * b[:, c:]) * s * (1 + np.abs(b[:, :c]) * (1 - s)), np.abs(rg[:, c:])], 1)
+            got = f64(micro.silu_mul_backward(dy, x))
+            assert (np.abs(got - rg) <= half_step(dtype) * np.abs(rg) + 2.0 ** -18 * mag + tiny).all(), (rows, cols)
+
+
+def test_gate_extremes():
+    big = torch.finfo(torch.bfloat16).max
+    g = torch.tensor([[0.0, -0.0, 100.0, -100.0, 1e4, -1e4, big, -big, 89.0, -89.0, -88.0, 30.0]], dtype=torch.bfloat16, device="cuda")
+    x = torch.cat([g, torch.ones_like(g)], 1)
+    y = f64(micro.silu_mul(x))
+    assert (np.abs(y - gate64(f64(x))) <= (half_step(torch.bfloat16) + 2.0 ** -15) * np.abs(gate64(f64(x))) + 1e-35).all()
+    d = f64(micro.silu_mul_backward(torch.ones_like(g), x))
+    assert np.isfinite(d).all() and d[0, 2] == 1.0 and d[0, 3] == 0.0 and d[0, 6] == 1.0 and abs(d[0, 7]) == 0.0
+    assert micro.silu_mul(x[:0]).shape == (0, 12) and micro.silu_mul(x.view(1, 1, 24)).shape == (1, 1, 12)
+
+
+def test_gate_gradient_formula_against_differences():
+    rng = np.random.default_rng(0)
+    x, dy, e = rng.normal(size=(2, 12)) * 2, rng.normal(size=(2, 6)), 1e-6
+    grad = gate_grad64(dy, x)
+    for i in np.ndindex(x.shape):
+        d = np.zeros_like(x)
+        d[i] = e
+        assert abs(((gate64(x + d) - gate64(x - d)) * dy).sum() / (2 * e) - grad[i]) < 1e-7
+    t = torch.from_numpy(x).bfloat16().cuda().requires_grad_()
+    (g,) = torch.autograd.grad(micro.silu_mul(t), t, torch.from_numpy(dy).bfloat16().cuda())
+    r = gate_grad64(f64(torch.from_numpy(dy).bfloat16()), f64(t))
+    assert (np.abs(f64(g) - r) <= 2.0 ** -8 * np.abs(r) + 1e-4).all()
+
+
+# ---------------------------------------------------------------- runs of them together
+def q64(x: np.ndarray, fmt: str) -> np.ndarray:
+    g = om.tensor_scale(x) if fmt == "nvfp4" else None
+    return om.values(*om.quantize(x, fmt, g), fmt, g)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_linear_training(fmt):
+    """Forward and both gradients: each product of exactly known quantised operands, within check_product's bound."""
+    for m, n, k in ((1, 40, 64), (33, 130, 100), (200, 72, 257)):
+        x, w = normal(m, k, seed=1).requires_grad_(), normal(n, k, seed=2, std=0.05).requires_grad_()
+        dy = normal(n, m, seed=3).t()
+        y = micro.micro_linear(x, w, fmt)
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+        a, b, d = f64(x), f64(w), f64(dy)
+        check_product(y.detach(), q64(a, fmt), q64(b, fmt))
+        check_product(dx, q64(d, fmt), q64(b.T, fmt))
+        check_product(dw, q64(d.T, fmt), q64(a.T, fmt))
+    x3 = normal(2, 3, 64, seed=4).requires_grad_()
+    w = normal(8, 64, seed=5)
+    y = micro.micro_linear(x3, w, fmt)
+    assert y.shape == (2, 3, 8)
+    y.sum().backward()  # an expanded gradient
+    check_product(x3.grad.view(6, 64), q64(np.ones((6, 8)), fmt), q64(f64(w).T, fmt))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens", [1, 40, 300])
+def test_mlp(fmt, tokens):
+    """Norm, product, gate and product in a row. Every stage is checked on what the stage before really gave, within its
+    own tolerance, so that nothing accumulates into a loose bound; the whole is the same as its parts."""
+    hidden, ff = 256, 352
+    x, r, nw = normal(tokens, hidden, seed=1), normal(tokens, hidden, seed=2), normal(hidden, seed=3)
+    gu = micro.quantize(normal(2 * ff, hidden, seed=4, std=0.05), fmt)
+    down = micro.quantize(normal(hidden, ff, seed=5, std=0.05), fmt)
+    scales = (torch.full((1,), 0.01, device="cuda"), torch.full((1,), 0.01, device="cuda")) if fmt == "nvfp4" else None
+    y, h = micro.micro_mlp(x, r, nw, gu, down, scales=scales)
+    s = scales or (None, None)
+    n, h2 = micro.rms_norm(x, nw, residual=r, format=fmt, scale=s[0])
+    check_coded(n, norm64(f64(x), f64(nw), 1e-5, f64(r))[0], 2.0 ** -18)
+    p = micro.micro_matmul(n, gu)
+
+    def v(q):
+        return om.values(*stored(q), fmt, None if q.scale is None else float(q.scale))
+    check_product(p, v(n), v(gu))
+    g = micro.silu_mul(p, format=fmt, scale=s[1])
+    check_coded(g, gate64(f64(p)), 2.0 ** -18)
+    check_product(y, v(g), v(down))
+    assert torch.equal(y, micro.micro_matmul(g, down)) and torch.equal(h, h2)
+    micro.check_status()
+
+
+def test_capture_replay_and_streams():
+    """A training step and an inference block captured into two graphs that are replayed at once on two streams, with new
+    inputs, between eager steps on the same leaves. (torch refuses the capture of any operator's backward pass while an
+    eager autograd graph of the same leaves is alive: theirs is gone before the capture begins.)"""
+    fmt = "mxfp8"
+    x, w = normal(130, 256, seed=1).requires_grad_(), normal(96, 256, seed=2).requires_grad_()
+    dy, nw = normal(130, 96, seed=3), normal(96, seed=4)
+    torch.autograd.grad(micro.micro_linear(x, w, fmt), (x, w), dy)
+
+    def step():
+        y = micro.micro_linear(x, w, fmt)
+        n, _ = micro.rms_norm(y, nw)
+        return (n.detach(), *torch.autograd.grad(n, (x, w), dy))
+
+    def block():
+        q, h = micro.rms_norm(dy, nw, residual=dy, format="nvfp4", scale=scale)
+        return q.dequantize(), h, micro.micro_matmul(q, qw), micro.quantize(dy, "nvfp4").dequantize()
+
+    scale = torch.full((1,), 0.01, device="cuda")
+    qw = micro.quantize(normal(64, 96, seed=5), "nvfp4")
+    graphs = []
+    for f in (step, block):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            f()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = f()
+        graphs.append((g, out, f))
+    torch.autograd.grad(micro.micro_linear(x, w, fmt), (x, w), dy)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for seed in (10, 11):
+        with torch.no_grad():
+            x.copy_(normal(130, 256, seed=seed))
+            dy.copy_(normal(130, 96, seed=seed + 1))
+        torch.cuda.synchronize()
+        for (g, _, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for _, out, f in graphs:
+            for a, b in zip(out, f()):
+                assert torch.equal(a, b)
+    micro.check_status()
+
+
+def test_two_products_at_once():
+    """Products on two streams at the same time, K split over clusters in both."""
+    ops = [(random_operand(m, 4096, fmt, i), random_operand(1000, 4096, fmt, i + 9)) for i, (m, fmt) in
+           enumerate(((1, "nvfp4"), (100, "mxfp8")))]
+    want = [micro.micro_matmul(a[0], b[0]) for a, b in ops]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ops]
+    got = [[], []]
+    for _ in range(50):
+        for i, ((a, b), s) in enumerate(zip(ops, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(micro.micro_matmul(a[0], b[0]))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, t) for t in g)
+    micro.check_status()
+
+
+def test_offsets_past_32_bits():
+    """Rows that lie more than 2^31 values into their buffers (6 GB at most here): first and last rows against the same
+    rows quantised alone."""
+    rows, cols = 70000, 32768
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[:2], x[-3:] = normal(2, cols, seed=1), normal(3, cols, seed=2)
+    x[2:-3] = 1.0
+    q = micro.quantize(x, "mxfp4")
+    ends = torch.cat([x[:2], x[-3:]])
+    want = micro.quantize(ends, "mxfp4").dequantize()
+    d = q.dequantize()
+    assert torch.equal(torch.cat([d[:2], d[-3:]]), want) and bool((d[2:-3] == 1).all())
+    del d
+    qa, a = random_operand(1, cols, "mxfp4", 3)
+    c = micro.micro_matmul(qa, q)
+    check_product(torch.cat([c[:, :2], c[:, -3:]], 1), a, f64(want))
+    c = micro.micro_matmul(q, qa)  # the long side as rows
+    check_product(torch.cat([c[:2], c[-3:]]), f64(want), a)
