@@ -4,9 +4,11 @@
 // converted on the way: TMA brings 128 bytes of codes a row (256 columns of 4 bits, 128 of 8) and the scale tiles that
 // belong to them into a ring of shared-memory stages, tcgen05.cp moves the scales on into tensor memory (a region of its
 // own for every stage, free once the stage's MMAs have completed), and four block-scaled MMAs of 32 bytes of K multiply
-// the stage into fp32 accumulators. One CTA takes a 128 x tile_q tile and K split; the MMA's 128 rows run over B's rows (a
-// layer's weights), its narrow side over A's (the tokens), so a few tokens cost a narrow tile. The K splits of a tile are
-// one thread-block cluster and are summed through distributed shared memory.
+// the stage into fp32 accumulators. Two kernels:
+//   product_kernel       one CTA per 128 x tile_q tile and K split; the MMA's 128 rows run over B's rows (a layer's
+//                        weights), its narrow side over A's (the tokens), so a few tokens cost a narrow tile. The K
+//                        splits of a tile are one thread-block cluster and are summed through distributed shared memory.
+//   product_pair_kernel  CTA pairs (cta_group::2) of 256 x 256 tiles for products with many of them.
 // Every wait is bounded as in b2g_gemm.cu: on expiry the status word gets a code and the CTA drains and returns.
 
 #include <cuda.h>
@@ -28,7 +30,7 @@ constexpr uint64_t kDrainNs = 50000000ull;            // 50 ms to drain in-fligh
 constexpr uint32_t kMaxSmem = 232448;                 // sm_100 opt-in maximum dynamic shared memory per block
 constexpr int kStepsPerStage = 4;                     // MMAs of 32 bytes of K in a 128-byte stage
 
-constexpr uint32_t O_FULL = 0, O_EMPTY = 128, O_TFULL = 256, O_DRAIN = 272, O_TMEM = 280, O_ABORT = 284;
+constexpr uint32_t O_FULL = 0, O_EMPTY = 128, O_TFULL = 256, O_TEMPTY = 264, O_DRAIN = 272, O_TMEM = 280, O_ABORT = 284;
 
 // status codes: b2g_status_string names them
 constexpr int kProducerTimeout = 0x101, kMmaTimeout = 0x102, kEpilogueTimeout = 0x103;
@@ -47,7 +49,7 @@ struct Params {
   int32_t rows_p, rows_q, K, num_kb;
   int32_t tile_q, q_tiles;           // columns of a tile; 128-row scale tiles they span
   int32_t stages, split;
-  int32_t tiles_p, tiles_q, units;
+  int32_t tiles_p, tiles_q, units, group;
   uint32_t q_bytes, stage_bytes;     // Q's codes of a stage; its place in the ring, whole KB
   uint32_t tx_bytes;                 // what its copies bring: codes and scales of both operands
   uint32_t acc_cols, tmem_cols;
@@ -293,6 +295,221 @@ __global__ void __launch_bounds__(192, 1)
   if (warp == 1) tmem_dealloc(tmem, p.tmem_cols);
 }
 
+// ---------------------------------------------------------------- CTA pairs
+constexpr int kPairEpilogueWarps = 8;
+constexpr uint32_t kPairStaging = kPairEpilogueWarps * 4096u;
+
+// Tile `t` of the pairs' walk: bands of `group` tile rows, inside a band down the rows first, so that the tiles that run
+// at one time share operands in L2.
+__device__ __forceinline__ void pair_tile(const Params& p, int t, int& tp, int& tq) {
+  const int band = p.group * p.tiles_q;
+  const int g = t / band, r = t - g * band;
+  const int h = min(p.group, p.tiles_p - g * p.group);
+  tq = r / h;
+  tp = g * p.group + (r - tq * h);
+}
+
+// 256 x 256 tiles, a persistent CTA pair on each: every CTA loads its 128 rows of P, half of Q's 256 and the scales of
+// its P rows and of all of Q (both tensor memories hold Q's scales), the leader issues MMAs of M = 256, and each CTA ends
+// with a 128 x 256 accumulator. 256 accumulator columns and the stages' scales fill tensor memory, so there is one
+// accumulator: the epilogue's eight warps bring it into registers, already rounded, and free it at once (a few hundred
+// cycles), and store while the next tile's MMAs run.
+template <int KIND>
+__global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
+    product_pair_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap map_p,
+                        const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_sp,
+                        const __grid_constant__ CUtensorMap map_sq) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr uint32_t kPBytes = 128 * 128, kTileBytes = 512u * tiles_of(KIND);
+  const uint32_t ctl = smem_addr(smem_raw);
+  const uint32_t ring = (ctl + kCtl + 1023u) & ~1023u;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem_raw + O_ABORT);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const bool leader = rank == 0;
+  const int first = static_cast<int>(cluster_id_x()), step = static_cast<int>(num_clusters_x());
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_p);
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_sp);
+    tma_prefetch_desc(&map_sq);
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(ctl + O_FULL + 8 * s, 1);
+      mbar_init(ctl + O_EMPTY + 8 * s, 1);
+    }
+    mbar_init(ctl + O_TFULL, 1);
+    mbar_init(ctl + O_TEMPTY, 2 * kPairEpilogueWarps);  // one arrival per epilogue warp of both CTAs, at the leader's
+    mbar_init(ctl + O_DRAIN, 1);
+    *abort_flag = 0u;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(ctl + O_TMEM, p.tmem_cols);
+    tmem_relinquish_pair();
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers exist before any signal crosses
+  tc_fence_after();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + O_TMEM);
+
+  if (warp == 0) {
+    if (lane == 0) {  // TMA producer: each CTA's copies count on the leader's barriers
+      const uint32_t full0 = map_to_rank(ctl + O_FULL, 0);
+      int s = 0, issued = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int t = first; ok && t < p.units; t += step) {
+        int tp, tq;
+        pair_tile(p, t, tp, tq);
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          const uint32_t empty = ctl + O_EMPTY + 8 * s, full = full0 + 8 * s;
+          if (!mbar_try_wait(empty, ph ^ 1u) && !wait_phase(empty, ph ^ 1u, abort_flag, p.status, kProducerTimeout)) {
+            ok = false;
+            break;
+          }
+          if (leader) mbar_arrive_expect_tx(ctl + O_FULL + 8 * s, p.tx_bytes);
+          const uint32_t base = ring + s * p.stage_bytes;
+          tma_load_2d_pair(base, &map_p, full, kb * 128, tp * 256 + rank * 128);
+          tma_load_2d_pair(base + kPBytes, &map_q, full, kb * 128, tq * 256 + rank * 128);
+          tma_load_3d_pair(base + kPBytes + p.q_bytes, &map_sp, full, 0, kb * tiles_of(KIND), tp * 2 + rank);
+          tma_load_3d_pair(base + kPBytes + p.q_bytes + kTileBytes, &map_sq, full, 0, kb * tiles_of(KIND), tq * 2);
+          ++issued;
+          if (++s == p.stages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      if (!ok && leader) {  // the leader's barriers count the pair's copies: let those already issued land
+        for (int i = min(issued, p.stages); i > 0; --i) {
+          if (--s < 0) {
+            s = p.stages - 1;
+            ph ^= 1u;
+          }
+          drain_phase(ctl + O_FULL + 8 * s, ph, kDrainNs);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (leader) {  // MMA issuer for both CTAs
+      uint32_t idesc[kStepsPerStage];
+#pragma unroll
+      for (int i = 0; i < kStepsPerStage; ++i) idesc[i] = idesc_scaled(KIND, step_id(KIND, i), 256, 256);
+      const uint64_t pd = sdesc_sw128(ring, 16u, 1024u), qd = sdesc_sw128(ring + kPBytes, 16u, 1024u);
+      constexpr uint32_t cols = tiles_of(KIND) * 12u;  // a stage's scales: one tile row of P, two of Q
+      const uint32_t empty0 = map_to_rank(ctl + O_EMPTY, 0), empty1 = map_to_rank(ctl + O_EMPTY, 1);
+      const uint32_t tfull0 = map_to_rank(ctl + O_TFULL, 0), tfull1 = map_to_rank(ctl + O_TFULL, 1);
+      const int last = p.K - (p.num_kb - 1) * stage_k(KIND);
+      const int last_steps = (last + step_k(KIND) - 1) / step_k(KIND);
+      int s = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int t = first; ok && t < p.units; t += step) {
+        if (!mbar_try_wait(ctl + O_TEMPTY, acc_ph ^ 1u) &&
+            !wait_phase(ctl + O_TEMPTY, acc_ph ^ 1u, abort_flag, p.status, kMmaTimeout)) {
+          ok = false;
+          break;
+        }
+        acc_ph ^= 1u;
+        tc_fence_after();
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          const uint32_t full = ctl + O_FULL + 8 * s;
+          if (!mbar_try_wait(full, ph) && !wait_phase(full, ph, abort_flag, p.status, kMmaTimeout)) {
+            ok = false;
+            break;
+          }
+          const uint32_t base = ring + s * p.stage_bytes, off = s * (p.stage_bytes >> 4);
+          issue_stage<KIND, 1>(tmem, pd + off, qd + off, base + kPBytes + p.q_bytes,
+                               base + kPBytes + p.q_bytes + kTileBytes, tmem + p.acc_cols + s * cols, 2, idesc,
+                               kb + 1 == p.num_kb ? last_steps : kStepsPerStage, kb == 0 ? 0u : 1u);
+          umma_commit_pair_w(empty0 + 8 * s);
+          umma_commit_pair_w(empty1 + 8 * s);
+          if (++s == p.stages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (!ok) break;
+        umma_commit_pair_w(tfull0);
+        umma_commit_pair_w(tfull1);
+      }
+      umma_commit_pair_w(map_to_rank(ctl + O_DRAIN, 0));
+      drain_phase(ctl + O_DRAIN, 0, ok ? kWaitNs : kDrainNs);
+    }
+  } else {
+    const int e = warp - 2, q = warp & 3, half = e >> 2;  // tensor-memory lane quarter, half of the columns
+    const uint32_t tempty = map_to_rank(ctl + O_TEMPTY, 0);
+    const uint32_t stg = ring + p.stages * p.stage_bytes + static_cast<uint32_t>(e) * 4096u;
+    const float alpha = p.scale_a ? *p.scale_a * *p.scale_b : 1.f;
+    uint16_t* out = static_cast<uint16_t*>(p.out);
+    uint32_t ph = 0;
+    for (int t = first; t < p.units; t += step) {
+      int tp, tq;
+      pair_tile(p, t, tp, tq);
+      if (!wait_phase(ctl + O_TFULL, ph, abort_flag, p.status, kEpilogueTimeout)) break;
+      ph ^= 1u;
+      tc_fence_after();
+      uint32_t w[64];  // the row's 128 columns, rounded
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tmem_ld_32cols(tmem + half * 128 + c * 32 + (static_cast<uint32_t>(q * 32) << 16), v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          w[c * 16 + j] = cvt2(__uint_as_float(v[2 * j]) * alpha, __uint_as_float(v[2 * j + 1]) * alpha, p.out_bf16);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty);
+      const int64_t row0 = static_cast<int64_t>(tp) * 256 + rank * 128 + q * 32;
+      const int64_t col0 = static_cast<int64_t>(tq) * 256 + half * 128;
+      if (p.vec) {
+        // 32 rows x 64 columns at a time through shared memory (16-byte pieces XOR-ed by the row), so that a store
+        // instruction writes four whole 128-byte row segments
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            st_shared_v4(stg + lane * 128 + ((j ^ (lane & 7)) << 4),
+                         make_uint4(w[h * 32 + 4 * j], w[h * 32 + 4 * j + 1], w[h * 32 + 4 * j + 2], w[h * 32 + 4 * j + 3]));
+          __syncwarp();
+          const int64_t col = col0 + h * 64 + (lane & 7) * 8;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3);
+            const uint4 x = ld_shared_v4(stg + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+            if (row0 + r < p.rows_p) {
+              uint16_t* o = out + (row0 + r) * p.ldc + col;
+              if (col + 8 <= p.rows_q) {
+                *reinterpret_cast<uint4*>(o) = x;
+              } else {
+                const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  if (col + k < p.rows_q) o[k] = static_cast<uint16_t>(u[k / 2] >> (16 * (k & 1)));
+              }
+            }
+          }
+          __syncwarp();
+        }
+      } else if (row0 + lane < p.rows_p) {
+        uint16_t* o = out + (row0 + lane) * p.ldc + col0;
+#pragma unroll
+        for (int k = 0; k < 128; ++k)
+          if (col0 + k < p.rows_q) o[k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync();  // the pair's MMAs and signals are done in both CTAs
+  if (warp == 1) tmem_dealloc_pair(tmem, p.tmem_cols);
+}
+
 // ---------------------------------------------------------------- host side
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -355,7 +572,10 @@ int32_t init_device(int dev) {
   if (dev >= 0 && dev < 64 && done[dev]) return B2G_OK;
   const void* fns[] = {reinterpret_cast<const void*>(product_kernel<FMT_MXFP8>),
                        reinterpret_cast<const void*>(product_kernel<FMT_MXFP4>),
-                       reinterpret_cast<const void*>(product_kernel<FMT_NVFP4>)};
+                       reinterpret_cast<const void*>(product_kernel<FMT_NVFP4>),
+                       reinterpret_cast<const void*>(product_pair_kernel<FMT_MXFP8>),
+                       reinterpret_cast<const void*>(product_pair_kernel<FMT_MXFP4>),
+                       reinterpret_cast<const void*>(product_pair_kernel<FMT_NVFP4>)};
   for (const void* f : fns) {
     const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
     if (e != cudaSuccess) {
@@ -371,10 +591,16 @@ int32_t init_device(int dev) {
 // GPC): a launch of more would run in waves.
 constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
 
+constexpr int kPairs = 74;  // CTA pairs resident at once
+
+// Pairs where their 256 x 256 tiles fill the GPU.
+bool use_pairs(int64_t M, int64_t N) { return M > 128 && ceil_div(M, 256) * ceil_div(N, 256) >= kPairs / 2; }
+
 struct Plan {
   Params p;
   CUtensorMap map_p, map_q, map_sp, map_sq;
   int kind, device, grid;
+  bool pair;
   uint32_t smem;
   bool empty;    // no output element
   bool zero;     // K = 0: C is zero
@@ -422,6 +648,36 @@ int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b
   p.K = static_cast<int32_t>(a->cols);
   p.num_kb = static_cast<int32_t>(ceil_div(a->cols, stage_k(pl.kind)));
   const int T = tiles_of(pl.kind);
+  pl.pair = use_pairs(pl.M, pl.N);
+  if (pl.pair) {  // rows run over A, columns over B: C's rows are stored as they lie
+    p.rows_p = static_cast<int32_t>(pl.M);
+    p.rows_q = static_cast<int32_t>(pl.N);
+    p.tile_q = 256;
+    p.q_tiles = 2;
+    p.tiles_p = static_cast<int32_t>(ceil_div(pl.M, 256));
+    p.tiles_q = static_cast<int32_t>(ceil_div(pl.N, 256));
+    const int64_t tiles = static_cast<int64_t>(p.tiles_p) * p.tiles_q;
+    if (tiles > kMaxGrid / 2) return too_large("product");
+    p.units = static_cast<int32_t>(tiles);
+    p.group = 8;
+    p.split = 1;
+    pl.grid = 2 * (tiles < kPairs ? static_cast<int>(tiles) : kPairs);
+    p.q_bytes = 128u * 128u;
+    const uint32_t cta_bytes = 2u * 128u * 128u + 512u * T * 3;
+    p.tx_bytes = 2u * cta_bytes;
+    p.stage_bytes = (cta_bytes + 1023u) & ~1023u;
+    p.acc_cols = 256;
+    p.tmem_cols = 512;
+    const uint32_t cols = T * 4u * 3u;
+    uint32_t stages = (kMaxSmem - 2048u - kPairStaging) / p.stage_bytes;
+    if (stages > 256u / cols) stages = 256u / cols;
+    p.stages = static_cast<int32_t>(stages);
+    pl.smem = kMaxSmem;
+    if (const int32_t rc = encode_codes(&pl.map_p, a, 128)) return rc;
+    if (const int32_t rc = encode_codes(&pl.map_q, b, 128)) return rc;
+    if (const int32_t rc = encode_scales(&pl.map_sp, a, T, 1)) return rc;
+    return encode_scales(&pl.map_sq, b, T, 2);
+  }
   // rows run over B, columns over A
   p.rows_p = static_cast<int32_t>(pl.N);
   p.rows_q = static_cast<int32_t>(pl.M);
@@ -486,11 +742,12 @@ int32_t plan_launch(const Plan& pl, cudaStream_t st) {
   lc.numAttrs = 1;
   lc.stream = st;
   lc.gridDim = dim3(static_cast<unsigned>(pl.grid), 1, 1);
-  lc.blockDim = dim3(192, 1, 1);
+  lc.blockDim = dim3(pl.pair ? (2 + kPairEpilogueWarps) * 32 : 192, 1, 1);
   lc.dynamicSmemBytes = pl.smem;
-  if (pl.p.split > 1) {
+  const int cluster = pl.pair ? 2 : pl.p.split;
+  if (cluster > 1) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(pl.p.split);
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     lc.numAttrs = 2;
@@ -499,7 +756,7 @@ int32_t plan_launch(const Plan& pl, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   by_format(pl.kind, [&](auto f) -> int32_t {
     constexpr int F = decltype(f)::value;
-    e = go(product_kernel<F>);
+    e = pl.pair ? go(product_pair_kernel<F>) : go(product_kernel<F>);
     return B2G_OK;
   });
   if (e == cudaSuccess) return B2G_OK;
