@@ -74,6 +74,26 @@ __device__ __noinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile 
   }
 }
 
+// The same for a converged warp, which goes on with one answer: the votes make it, and with it every loop counter and
+// descriptor of the warp's loop, uniform in the compiler's eyes. Operands of tcgen05 instructions come from uniform
+// registers; from per-thread ones each costs a move of tens of cycles, and the issue, not the tensor core, sets the pace.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int* status, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (;;) {
+    if (__all_sync(0xffffffffu, mbar_try_wait_hint(bar, parity, 1000000u))) return true;
+    if (__any_sync(0xffffffffu, *abort_flag != 0u)) return false;
+    if (__any_sync(0xffffffffu, global_timer_ns() - t0 > kWaitNs)) {
+      *abort_flag = 1u;
+      if (status) atomicCAS(status, 0, code);
+      return false;
+    }
+  }
+}
+
+// A value that every lane has, in a uniform register.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
 __device__ __noinline__ void drain_phase(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
   const uint64_t t0 = global_timer_ns();
   while (!mbar_try_wait(bar, parity)) {
@@ -103,19 +123,20 @@ __device__ __forceinline__ void issue_stage(uint32_t d, uint64_t p_desc, uint64_
                                             uint32_t tmem_scales, int q_tiles, const uint32_t (&idesc)[kStepsPerStage],
                                             int steps, uint32_t first) {
   constexpr int T = tiles_of(KIND);
-  const uint64_t pd = sdesc_plain(cp), qd = sdesc_plain(cq);
   const uint32_t tq = tmem_scales + 4 * T;
+  const uint32_t pl = static_cast<uint32_t>(p_desc), ql = static_cast<uint32_t>(q_desc);
 #pragma unroll
   for (int k = 0; k < T; ++k) {
-    scales_to_tmem_w<PAIR>(tmem_scales + 4 * k, pd + k * 32);
-    scales_to_tmem_w<PAIR>(tq + 4 * q_tiles * k, qd + k * 32);
-    if (q_tiles == 2) scales_to_tmem_w<PAIR>(tq + 8 * k + 4, qd + (T + k) * 32);
+    scales_to_tmem_w<PAIR>(tmem_scales + 4 * k, cp + k * 512);
+    scales_to_tmem_w<PAIR>(tq + 4 * q_tiles * k, cq + k * 512);
+    if (q_tiles == 2) scales_to_tmem_w<PAIR>(tq + 8 * k + 4, cq + (T + k) * 512);
   }
 #pragma unroll
   for (int s = 0; s < kStepsPerStage; ++s) {
     if (s < steps)
-      umma_scaled_w<KIND, PAIR>(d, p_desc + s * 2, q_desc + s * 2, idesc[s], tmem_scales + 4 * step_tile(KIND, s),
-                                tq + 4 * q_tiles * step_tile(KIND, s), s == 0 ? first : 1u);
+      umma_scaled_w<KIND, PAIR>(d, pl + s * 2, ql + s * 2, static_cast<uint32_t>(p_desc >> 32), idesc[s],
+                                tmem_scales + 4 * step_tile(KIND, s), tq + 4 * q_tiles * step_tile(KIND, s),
+                                s == 0 ? first : 1u);
   }
 }
 
@@ -200,21 +221,21 @@ __global__ void __launch_bounds__(192, 1)
 #pragma unroll
     for (int i = 0; i < kStepsPerStage; ++i) idesc[i] = idesc_scaled(KIND, step_id(KIND, i), 128, p.tile_q);
     const uint64_t pd = sdesc_sw128(ring, 16u, 1024u), qd = sdesc_sw128(ring + kPBytes, 16u, 1024u);
-    const uint32_t cols = scale_cols<KIND>(p.q_tiles);
+    const uint32_t cols = scale_cols<KIND>(p.q_tiles), utmem = uniform(tmem);
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
     for (int kb = kb0; kb < kb1; ++kb) {
       const uint32_t full = ctl + O_FULL + 8 * s;
-      if (!mbar_try_wait(full, ph) && !wait_phase(full, ph, abort_flag, p.status, kMmaTimeout)) {
+      if (!warp_wait(full, ph, abort_flag, p.status, kMmaTimeout)) {
         ok = false;
         break;
       }
       const uint32_t base = ring + s * p.stage_bytes, off = s * (p.stage_bytes >> 4);
       const int left = p.K - kb * stage_k(KIND);
       const int steps = left >= stage_k(KIND) ? kStepsPerStage : (left + step_k(KIND) - 1) / step_k(KIND);
-      issue_stage<KIND, 0>(tmem, pd + off, qd + off, base + kPBytes + p.q_bytes, base + kPBytes + p.q_bytes + kTileBytes,
-                           tmem + p.acc_cols + s * cols, p.q_tiles, idesc, steps, kb == kb0 ? 0u : 1u);
+      issue_stage<KIND, 0>(utmem, pd + off, qd + off, base + kPBytes + p.q_bytes, base + kPBytes + p.q_bytes + kTileBytes,
+                           utmem + p.acc_cols + s * cols, p.q_tiles, idesc, steps, kb == kb0 ? 0u : 1u);
       umma_commit_w(ctl + O_EMPTY + 8 * s);
       if (++s == p.stages) {
         s = 0;
@@ -312,8 +333,8 @@ __device__ __forceinline__ void pair_tile(const Params& p, int t, int& tp, int& 
 // 256 x 256 tiles, a persistent CTA pair on each: every CTA loads its 128 rows of P, half of Q's 256 and the scales of
 // its P rows and of all of Q (both tensor memories hold Q's scales), the leader issues MMAs of M = 256, and each CTA ends
 // with a 128 x 256 accumulator. 256 accumulator columns and the stages' scales fill tensor memory, so there is one
-// accumulator: the epilogue's eight warps bring it into registers, already rounded, and free it at once (a few hundred
-// cycles), and store while the next tile's MMAs run.
+// accumulator: the epilogue's eight warps read it into registers and free it before they convert the second half and
+// store, while the next tile's MMAs run.
 template <int KIND>
 __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
     product_pair_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap map_p,
@@ -402,6 +423,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
       const uint64_t pd = sdesc_sw128(ring, 16u, 1024u), qd = sdesc_sw128(ring + kPBytes, 16u, 1024u);
       constexpr uint32_t cols = tiles_of(KIND) * 12u;  // a stage's scales: one tile row of P, two of Q
       const uint32_t empty0 = map_to_rank(ctl + O_EMPTY, 0), empty1 = map_to_rank(ctl + O_EMPTY, 1);
+      const uint32_t utmem = uniform(tmem);
       const uint32_t tfull0 = map_to_rank(ctl + O_TFULL, 0), tfull1 = map_to_rank(ctl + O_TFULL, 1);
       const int last = p.K - (p.num_kb - 1) * stage_k(KIND);
       const int last_steps = (last + step_k(KIND) - 1) / step_k(KIND);
@@ -409,8 +431,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
       for (int t = first; ok && t < p.units; t += step) {
-        if (!mbar_try_wait(ctl + O_TEMPTY, acc_ph ^ 1u) &&
-            !wait_phase(ctl + O_TEMPTY, acc_ph ^ 1u, abort_flag, p.status, kMmaTimeout)) {
+        if (!warp_wait(ctl + O_TEMPTY, acc_ph ^ 1u, abort_flag, p.status, kMmaTimeout)) {
           ok = false;
           break;
         }
@@ -418,13 +439,13 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
         tc_fence_after();
         for (int kb = 0; kb < p.num_kb; ++kb) {
           const uint32_t full = ctl + O_FULL + 8 * s;
-          if (!mbar_try_wait(full, ph) && !wait_phase(full, ph, abort_flag, p.status, kMmaTimeout)) {
+          if (!warp_wait(full, ph, abort_flag, p.status, kMmaTimeout)) {
             ok = false;
             break;
           }
           const uint32_t base = ring + s * p.stage_bytes, off = s * (p.stage_bytes >> 4);
-          issue_stage<KIND, 1>(tmem, pd + off, qd + off, base + kPBytes + p.q_bytes,
-                               base + kPBytes + p.q_bytes + kTileBytes, tmem + p.acc_cols + s * cols, 2, idesc,
+          issue_stage<KIND, 1>(utmem, pd + off, qd + off, base + kPBytes + p.q_bytes,
+                               base + kPBytes + p.q_bytes + kTileBytes, utmem + p.acc_cols + s * cols, 2, idesc,
                                kb + 1 == p.num_kb ? last_steps : kStepsPerStage, kb == 0 ? 0u : 1u);
           umma_commit_pair_w(empty0 + 8 * s);
           umma_commit_pair_w(empty1 + 8 * s);
@@ -455,17 +476,24 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
       tc_fence_after();
       uint32_t w[64];  // the row's 128 columns, rounded
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tmem_ld_32cols(tmem + half * 128 + c * 32 + (static_cast<uint32_t>(q * 32) << 16), v);
-        tmem_ld_wait();
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v[2][32];
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          w[c * 16 + j] = cvt2(__uint_as_float(v[2 * j]) * alpha, __uint_as_float(v[2 * j + 1]) * alpha, p.out_bf16);
+        for (int c = 0; c < 2; ++c)
+          tmem_ld_32cols(tmem + half * 128 + h * 64 + c * 32 + (static_cast<uint32_t>(q * 32) << 16), v[c]);
+        tmem_ld_wait();
+        if (h == 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(tempty);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            w[h * 32 + c * 16 + j] =
+                cvt2(__uint_as_float(v[c][2 * j]) * alpha, __uint_as_float(v[c][2 * j + 1]) * alpha, p.out_bf16);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(tempty);
       const int64_t row0 = static_cast<int64_t>(tp) * 256 + rank * 128 + q * 32;
       const int64_t col0 = static_cast<int64_t>(tq) * 256 + half * 128;
       if (p.vec) {

@@ -9,18 +9,21 @@ namespace b2g {
 // D[tmem] (+)= (A * scale A) * (B * scale B), A and B from shared memory, scales from tensor memory, fp32 accumulators.
 // KIND 1: 8-bit floats, K = 32, one power-of-two scale per row (kind::mxf8f6f4); 2: e2m1, K = 64, two power-of-two
 // scales per row (kind::mxf4); 3: e2m1, K = 64, four e4m3 scales per row (kind::mxf4nvf4). Issued by lane 0 of a
-// converged warp.
+// converged warp. `a`, `b`: the descriptors' low words; `hi`: the high word both share (what varies between stages and K
+// steps is the start address, so only one word is computed).
 template <int KIND, int PAIR>
-__device__ __forceinline__ void umma_scaled_w(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
-                                              uint32_t accumulate) {
-#define B2G_UMMA_SCALED(GROUP, SPEC)                                                              \
-  asm volatile(                                                                                   \
-      "{\n\t.reg .pred p, q;\n\t.reg .u32 l;\n\t"                                                 \
-      "mov.u32 l, %%laneid;\n\t"                                                                  \
-      "setp.eq.u32 q, l, 0;\n\t"                                                                  \
-      "setp.ne.b32 p, %6, 0;\n\t"                                                                 \
-      "@q tcgen05.mma.cta_group::" GROUP "." SPEC " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), \
-      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)                               \
+__device__ __forceinline__ void umma_scaled_w(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t sa,
+                                              uint32_t sb, uint32_t accumulate) {
+#define B2G_UMMA_SCALED(GROUP, SPEC)                                                                 \
+  asm volatile(                                                                                      \
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 l;\n\t.reg .b64 da, db;\n\t"                               \
+      "mov.b64 da, {%1, %3};\n\t"                                                                    \
+      "mov.b64 db, {%2, %3};\n\t"                                                                    \
+      "mov.u32 l, %%laneid;\n\t"                                                                     \
+      "setp.eq.u32 q, l, 0;\n\t"                                                                     \
+      "setp.ne.b32 p, %7, 0;\n\t"                                                                    \
+      "@q tcgen05.mma.cta_group::" GROUP "." SPEC " [%0], da, db, %4, [%5], [%6], p;\n\t}" ::"r"(d), \
+      "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)                         \
       : "memory")
   if constexpr (KIND == 1) {
     if constexpr (PAIR) B2G_UMMA_SCALED("2", "kind::mxf8f6f4.block_scale.scale_vec::1X");
@@ -35,26 +38,22 @@ __device__ __forceinline__ void umma_scaled_w(uint32_t d, uint64_t a, uint64_t b
 #undef B2G_UMMA_SCALED
 }
 
-// A 512-byte scale tile (32 rows of 16 bytes) into four tensor-memory columns, repeated in each quarter of the lanes.
+// A 512-byte scale tile (32 rows of 16 bytes) at shared address `from` into four tensor-memory columns, repeated in each
+// quarter of the lanes. The descriptor has no swizzle: 8-row groups of 16 bytes a row, 128 bytes apart.
 template <int PAIR>
-__device__ __forceinline__ void scales_to_tmem_w(uint32_t tmem, uint64_t desc) {
-#define B2G_SCALE_COPY(GROUP)                                                        \
-  asm volatile(                                                                      \
-      "{\n\t.reg .pred q;\n\t.reg .u32 l;\n\t"                                       \
-      "mov.u32 l, %%laneid;\n\t"                                                     \
-      "setp.eq.u32 q, l, 0;\n\t"                                                     \
-      "@q tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [%0], %1;\n\t}" ::"r"(tmem), \
-      "l"(desc)                                                                      \
+__device__ __forceinline__ void scales_to_tmem_w(uint32_t tmem, uint32_t from) {
+#define B2G_SCALE_COPY(GROUP)                                                           \
+  asm volatile(                                                                         \
+      "{\n\t.reg .pred q;\n\t.reg .u32 l;\n\t.reg .b64 da;\n\t"                         \
+      "mov.b64 da, {%1, %2};\n\t"                                                       \
+      "mov.u32 l, %%laneid;\n\t"                                                        \
+      "setp.eq.u32 q, l, 0;\n\t"                                                        \
+      "@q tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [%0], da;\n\t}" ::"r"(tmem),   \
+      "r"(from >> 4 | 1u << 16), "r"(8u | 1u << 14)                                     \
       : "memory")
   if constexpr (PAIR) B2G_SCALE_COPY("2");
   else B2G_SCALE_COPY("1");
 #undef B2G_SCALE_COPY
-}
-
-// Shared-memory descriptor without a swizzle: 8-row groups of 16 bytes a row, 128 bytes apart.
-__device__ __forceinline__ uint64_t sdesc_plain(uint32_t saddr) {
-  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | static_cast<uint64_t>(1) << 16 | static_cast<uint64_t>(8) << 32 |
-         static_cast<uint64_t>(1) << 46;
 }
 
 // Instruction descriptor of the block-scaled kinds: both operands K-major, scale factor ids `id` (the byte of a 32-bit
