@@ -339,7 +339,7 @@ template <int KIND>
 __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
     product_pair_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap map_p,
                         const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_sp,
-                        const __grid_constant__ CUtensorMap map_sq) {
+                        const __grid_constant__ CUtensorMap map_sq, const __grid_constant__ CUtensorMap map_c) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr uint32_t kPBytes = 128 * 128, kTileBytes = 512u * tiles_of(KIND);
@@ -497,33 +497,19 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
       const int64_t row0 = static_cast<int64_t>(tp) * 256 + rank * 128 + q * 32;
       const int64_t col0 = static_cast<int64_t>(tq) * 256 + half * 128;
       if (p.vec) {
-        // 32 rows x 64 columns at a time through shared memory (16-byte pieces XOR-ed by the row), so that a store
-        // instruction writes four whole 128-byte row segments
+        // 32 rows x 64 columns at a time through the warp's 4 KB of shared memory (16-byte pieces XOR-ed by the row, the
+        // 128-byte swizzle) and out by TMA, which writes whole lines and drops what lies outside C
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          if (lane == 0) tma_store_wait_read();  // the last store has read the buffer
+          __syncwarp();
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             st_shared_v4(stg + lane * 128 + ((j ^ (lane & 7)) << 4),
                          make_uint4(w[h * 32 + 4 * j], w[h * 32 + 4 * j + 1], w[h * 32 + 4 * j + 2], w[h * 32 + 4 * j + 3]));
+          fence_async_shared();
           __syncwarp();
-          const int64_t col = col0 + h * 64 + (lane & 7) * 8;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = 4 * i + (lane >> 3);
-            const uint4 x = ld_shared_v4(stg + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-            if (row0 + r < p.rows_p) {
-              uint16_t* o = out + (row0 + r) * p.ldc + col;
-              if (col + 8 <= p.rows_q) {
-                *reinterpret_cast<uint4*>(o) = x;
-              } else {
-                const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                  if (col + k < p.rows_q) o[k] = static_cast<uint16_t>(u[k / 2] >> (16 * (k & 1)));
-              }
-            }
-          }
-          __syncwarp();
+          if (lane == 0) tma_store_2d(&map_c, stg, static_cast<int32_t>(col0) + h * 64, static_cast<int32_t>(row0));
         }
       } else if (row0 + lane < p.rows_p) {
         uint16_t* o = out + (row0 + lane) * p.ldc + col0;
@@ -532,6 +518,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
           if (col0 + k < p.rows_q) o[k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
       }
     }
+    if (lane == 0) tma_store_wait();
   }
   __syncwarp();
   cluster_sync();  // the pair's MMAs and signals are done in both CTAs
@@ -592,6 +579,20 @@ int32_t encode_scales(CUtensorMap* map, const b2g_micro_tensor* t, int ktiles, i
   return record_error(B2G_ERR_CUDA, "cuTensorMapEncodeTiled (scales): error " + std::to_string(static_cast<int>(r)));
 }
 
+// C in boxes of 32 rows x 64 columns for the pairs' stores (16-byte aligned rows only).
+int32_t encode_out(CUtensorMap* map, const Params& p) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return record_error(B2G_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.rows_q), static_cast<cuuint64_t>(p.rows_p)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.ldc) * 2};
+  const cuuint32_t box[2] = {64u, 32u};
+  const cuuint32_t elem[2] = {1u, 1u};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.out, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return B2G_OK;
+  return record_error(B2G_ERR_CUDA, "cuTensorMapEncodeTiled (C): error " + std::to_string(static_cast<int>(r)));
+}
+
 // Function attributes, once per device.
 int32_t init_device(int dev) {
   static std::mutex mu;
@@ -626,7 +627,7 @@ bool use_pairs(int64_t M, int64_t N) { return M > 128 && ceil_div(M, 256) * ceil
 
 struct Plan {
   Params p;
-  CUtensorMap map_p, map_q, map_sp, map_sq;
+  CUtensorMap map_p, map_q, map_sp, map_sq, map_c;
   int kind, device, grid;
   bool pair;
   uint32_t smem;
@@ -701,6 +702,9 @@ int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b
     if (stages > 256u / cols) stages = 256u / cols;
     p.stages = static_cast<int32_t>(stages);
     pl.smem = kMaxSmem;
+    std::memset(&pl.map_c, 0, sizeof pl.map_c);
+    if (p.vec)
+      if (const int32_t rc = encode_out(&pl.map_c, p)) return rc;
     if (const int32_t rc = encode_codes(&pl.map_p, a, 128)) return rc;
     if (const int32_t rc = encode_codes(&pl.map_q, b, 128)) return rc;
     if (const int32_t rc = encode_scales(&pl.map_sp, a, T, 1)) return rc;
@@ -780,11 +784,11 @@ int32_t plan_launch(const Plan& pl, cudaStream_t st) {
     attr[1].val.clusterDim.z = 1;
     lc.numAttrs = 2;
   }
-  const auto go = [&](auto kernel) { return cudaLaunchKernelEx(&lc, kernel, pl.p, pl.map_p, pl.map_q, pl.map_sp, pl.map_sq); };
   cudaError_t e = cudaSuccess;
   by_format(pl.kind, [&](auto f) -> int32_t {
     constexpr int F = decltype(f)::value;
-    e = pl.pair ? go(product_pair_kernel<F>) : go(product_kernel<F>);
+    e = pl.pair ? cudaLaunchKernelEx(&lc, product_pair_kernel<F>, pl.p, pl.map_p, pl.map_q, pl.map_sp, pl.map_sq, pl.map_c)
+                : cudaLaunchKernelEx(&lc, product_kernel<F>, pl.p, pl.map_p, pl.map_q, pl.map_sp, pl.map_sq);
     return B2G_OK;
   });
   if (e == cudaSuccess) return B2G_OK;

@@ -56,6 +56,18 @@ __device__ __forceinline__ void scales_to_tmem_w(uint32_t tmem, uint32_t from) {
 #undef B2G_SCALE_COPY
 }
 
+// 2-D tile shared -> global; what lies outside the tensor is not written. The thread that issues it commits and waits.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t from, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n\t"
+               "cp.async.bulk.commit_group;" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(from), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// this thread's shared-memory stores before later reads of the async proxy (TMA)
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // Instruction descriptor of the block-scaled kinds: both operands K-major, scale factor ids `id` (the byte of a 32-bit
 // tensor-memory cell from which a K step's scales start), type fields, N >> 3, scale type (0 e4m3, 1 power of two), M.
 __host__ __device__ constexpr uint32_t idesc_scaled(int kind, uint32_t id, uint32_t m, uint32_t n) {
