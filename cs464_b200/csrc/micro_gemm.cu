@@ -511,11 +511,25 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
           __syncwarp();
           if (lane == 0) tma_store_2d(&map_c, stg, static_cast<int32_t>(col0) + h * 64, static_cast<int32_t>(row0));
         }
-      } else if (row0 + lane < p.rows_p) {
-        uint16_t* o = out + (row0 + lane) * p.ldc + col0;
+      } else {  // rows of C that are not 16-byte aligned: through the same buffer, 32 consecutive values an instruction
 #pragma unroll
-        for (int k = 0; k < 128; ++k)
-          if (col0 + k < p.rows_q) o[k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            st_shared_v4(stg + lane * 128 + ((j ^ (lane & 7)) << 4),
+                         make_uint4(w[h * 32 + 4 * j], w[h * 32 + 4 * j + 1], w[h * 32 + 4 * j + 2], w[h * 32 + 4 * j + 3]));
+          __syncwarp();
+          const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.rows_p - row0));
+          for (int r = 0; r < rows; ++r) {
+            uint16_t* o = out + (row0 + r) * p.ldc + col0 + h * 64;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int c = k * 32 + lane;
+              if (col0 + h * 64 + c < p.rows_q) o[c] = ld_shared_u16(stg + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+            }
+          }
+          __syncwarp();
+        }
       }
     }
     if (lane == 0) tma_store_wait();
@@ -622,8 +636,23 @@ constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
 
 constexpr int kPairs = 74;  // CTA pairs resident at once
 
-// Pairs where their 256 x 256 tiles fill the GPU.
-bool use_pairs(int64_t M, int64_t N) { return M > 128 && ceil_div(M, 256) * ceil_div(N, 256) >= kPairs / 2; }
+// K splits of a single-CTA product of `tiles` tiles: one cluster a tile, as many splits as keep every cluster resident at
+// once and leave each split two stages.
+int splits(int64_t tiles, int num_kb) {
+  int split = 1;
+  for (int s = 2; s <= 8; ++s)
+    if (tiles <= kClusters[s] && num_kb >= 2 * s) split = s;
+  return split;
+}
+
+// Pairs, unless a side fits one 128-row tile, or there are so few 128 x 128 tiles that single CTAs split K over the GPU
+// and K is long enough to gain by it. Measured, pairs against single CTAs (us): nvfp4 512x4096x4096 (no split) 11.0, 13.6;
+// 256x28672x4096 22.1, 30.3; 256x4096x4096 (two splits of 16 stages) 10.6, 9.9; 256x4096x14336 23.9, 15.7; 1024^3 (two
+// splits of 4 stages) 6.2, 7.6; mxfp8 512x2048x2048 (of 16) 9.9, 9.2; 1024^3 (of 8) 7.2, 8.0.
+bool use_pairs(int64_t M, int64_t N, int num_kb) {
+  if (M <= 128 || N <= 128) return false;
+  return num_kb <= 8 || splits(ceil_div(M, 128) * ceil_div(N, 128), num_kb) == 1;
+}
 
 struct Plan {
   Params p;
@@ -677,7 +706,7 @@ int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b
   p.K = static_cast<int32_t>(a->cols);
   p.num_kb = static_cast<int32_t>(ceil_div(a->cols, stage_k(pl.kind)));
   const int T = tiles_of(pl.kind);
-  pl.pair = use_pairs(pl.M, pl.N);
+  pl.pair = use_pairs(pl.M, pl.N, p.num_kb);
   if (pl.pair) {  // rows run over A, columns over B: C's rows are stored as they lie
     p.rows_p = static_cast<int32_t>(pl.M);
     p.rows_q = static_cast<int32_t>(pl.N);
@@ -688,7 +717,7 @@ int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b
     const int64_t tiles = static_cast<int64_t>(p.tiles_p) * p.tiles_q;
     if (tiles > kMaxGrid / 2) return too_large("product");
     p.units = static_cast<int32_t>(tiles);
-    p.group = 8;
+    p.group = 16;
     p.split = 1;
     pl.grid = 2 * (tiles < kPairs ? static_cast<int>(tiles) : kPairs);
     p.q_bytes = 128u * 128u;
@@ -718,10 +747,7 @@ int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b
   p.tiles_p = static_cast<int32_t>(ceil_div(p.rows_p, 128));
   p.tiles_q = static_cast<int32_t>(ceil_div(p.rows_q, p.tile_q));
   const int64_t tiles = static_cast<int64_t>(p.tiles_p) * p.tiles_q;
-  // K splits, one cluster: as many as keep every cluster resident at once and leave each split two stages
-  p.split = 1;
-  for (int s = 2; s <= 8; ++s)
-    if (tiles <= kClusters[s] && p.num_kb >= 2 * s) p.split = s;
+  p.split = splits(tiles, p.num_kb);
   if (tiles * p.split > kMaxGrid) return too_large("product");
   p.units = static_cast<int32_t>(tiles * p.split);
   pl.grid = p.units;

@@ -56,6 +56,12 @@ __device__ __forceinline__ void scales_to_tmem_w(uint32_t tmem, uint32_t from) {
 #undef B2G_SCALE_COPY
 }
 
+__device__ __forceinline__ uint16_t ld_shared_u16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 // 2-D tile shared -> global; what lies outside the tensor is not written. The thread that issues it commits and waits.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t from, int32_t x, int32_t y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n\t"
