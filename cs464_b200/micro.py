@@ -31,6 +31,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 import weakref
 
 import torch
@@ -43,7 +44,51 @@ FORMATS = {"mxfp8": _abi.FMT_MXFP8, "mxfp4": _abi.FMT_MXFP4, "nvfp4": _abi.FMT_N
 BLOCK = {"mxfp8": 32, "mxfp4": 32, "nvfp4": 16}
 
 _VALUES = {torch.float16: _abi.VALUE_F16, torch.bfloat16: _abi.VALUE_BF16, torch.float32: _abi.VALUE_F32}
-_HALF = (torch.float16, torch.bfloat16)
+_HALF = {torch.float16: _abi.VALUE_F16, torch.bfloat16: _abi.VALUE_BF16}
+
+# A call of a few microseconds on the GPU is paid for on the host, so the calls below keep it short: structures go to the
+# library as packed bytes, one allocation holds a tensor's codes and scales, and the checks that pass are the cheap ones
+# (those that fail repeat at leisure to say why).
+_pack_tensor = struct.Struct("=iiqqQqQQ").pack   # b2g_micro_tensor
+_pack_matrix = struct.Struct("=Qqq").pack        # b2g_micro_matrix
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+class _Entry:
+    """The entry points that enqueue work, bound with plain pointers for the structures, on first use."""
+
+    _ARGS = {"tensor_scale": "pqqipp", "quantize": "pipp", "dequantize": "ppip", "matmul": "pppqipp", "plan_launch": "pp",
+             "rms_norm": "ppppppqqfip", "rms_norm_backward": "pppppppzqqfip", "silu_mul": "pppqqip",
+             "silu_mul_backward": "pppqqip"}
+    _KIND = {"p": ctypes.c_void_p, "q": ctypes.c_int64, "i": ctypes.c_int32, "f": ctypes.c_float, "z": ctypes.c_size_t}
+
+    def __getattr__(self, name: str):
+        fn = _abi.load()["b2g_micro_" + name]
+        fn.argtypes = [self._KIND[k] for k in self._ARGS[name]]
+        fn.restype = ctypes.c_int32
+        fn.what = "b2g_micro_" + name
+        setattr(self, name, fn)
+        return fn
+
+
+_entry = _Entry()
+
+
+def _call(index: int, fn, *args) -> None:
+    """Enqueue an entry point on the current stream of device `index`, with it the current device."""
+    if _get_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _abi.check(rc, fn.what)
+
+
+def _matrix(t: torch.Tensor) -> bytes:
+    return _pack_matrix(t.data_ptr(), *t.stride())
 
 
 def _format(fmt: str) -> int:
@@ -53,49 +98,39 @@ def _format(fmt: str) -> int:
         raise ValueError(f"format must be one of {', '.join(FORMATS)}, not {fmt!r}") from None
 
 
-def _matrix(t: torch.Tensor) -> _abi.MicroMatrix:
-    return _abi.MicroMatrix(t.data_ptr(), *t.stride())
-
-
-def _device(t: torch.Tensor, what: str) -> torch.device:
+def _check(t: torch.Tensor, what: str, dtypes, like: torch.Tensor | None = None) -> None:
+    """Raise unless t is a CUDA tensor of one of `dtypes`, on the device of `like`."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor (there is no CPU path)")
-    return t.device
-
-
-def _values(t: torch.Tensor, what: str, dtypes, dev: torch.device | None = None) -> None:
-    _device(t, what)
     if t.dtype not in dtypes:
         raise TypeError(f"{what} must be {' or '.join(str(d)[6:] for d in dtypes)}, not {str(t.dtype)[6:]}")
-    if dev is not None and t.device != dev:
-        raise ValueError(f"{what} is on {t.device}, the other tensors on {dev}")
+    if like is not None and t.get_device() != like.get_device():
+        raise ValueError(f"{what} is on {t.device}, the other tensors on {like.device}")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t as a matrix of rows (its last dimension)."""
-    return t if t.ndim == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+    return t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
 
 
-def _call(dev: torch.device, what: str, *args) -> None:
-    """Enqueue an entry point on the current stream of `dev`, with `dev` the current device."""
-    fn = getattr(_abi.load(), what)
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    if rc:
-        _abi.check(rc, what)
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """Uninitialised contiguous storage of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
-def _tensor_scale(scale, dev: torch.device) -> torch.Tensor:
-    if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or scale.numel() != 1 or scale.device != dev:
-        raise ValueError(f"scale must be a float32 tensor of one element on {dev}")
-    return scale
+def _check_scale(scale, like: torch.Tensor) -> None:
+    if (not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or scale.numel() != 1
+            or scale.get_device() != like.get_device()):
+        raise ValueError(f"scale must be a float32 tensor of one element on {like.device}")
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    return t.data_ptr() % 16 == 0
+def _layout(fmt: int, rows: int, cols: int) -> tuple[int, int]:
+    """(pitch, scale bytes) of a tensor: b2g_micro_layout."""
+    if fmt == _abi.FMT_MXFP8:
+        return (cols + 31) // 32 * 32, (rows + 127) // 128 * ((cols + 127) // 128) * 512
+    if fmt == _abi.FMT_MXFP4:
+        return (cols + 31) // 32 * 16, (rows + 127) // 128 * ((cols + 127) // 128) * 512
+    return (cols + 31) // 32 * 16, (rows + 127) // 128 * ((cols + 63) // 64) * 512
 
 
 class MicroTensor:
@@ -107,47 +142,69 @@ class MicroTensor:
     zero where rows or blocks do not exist. `scale`: nvfp4's fp32 scale of the tensor (one element on the device), which
     other formats do not have. The constructor checks and takes the tensors as they are."""
 
-    __slots__ = ("codes", "scales", "shape", "format", "scale", "_abi")
+    __slots__ = ("_codes", "_scales", "shape", "format", "scale", "_buf", "_raw", "__weakref__")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, format: str, scale: torch.Tensor | None = None):
         fmt = _format(format)
-        rows, cols = (int(n) for n in shape)
+        rows, cols = map(int, shape)
         if rows < 0 or cols < 0:
             raise ValueError(f"bad shape {tuple(shape)}")
-        dev = _device(codes, "codes")
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or scales.device != dev:
-            raise ValueError(f"codes and scales must be uint8 tensors on one device, not {codes.dtype} on {dev} and "
-                             f"{scales.dtype} on {scales.device}")
+        _check(codes, "codes", (torch.uint8,))
+        _check(scales, "scales", (torch.uint8,), codes)
         pitch, scale_bytes = _layout(fmt, rows, cols)
-        step = 32 if fmt == _abi.FMT_MXFP8 else 16
+        at, sat = codes.data_ptr(), scales.data_ptr()
+        row = pitch
         if rows and cols:
-            if (codes.ndim != 2 or codes.shape[0] != rows or codes.shape[1] < pitch or codes.stride(1) != 1
-                    or (rows > 1 and (codes.stride(0) < pitch or codes.stride(0) % step)) or not _aligned(codes)):
+            step = 32 if fmt == _abi.FMT_MXFP8 else 16
+            if rows > 1 and codes.dim() == 2:
+                row = codes.stride(0)
+            if (codes.dim() != 2 or codes.shape[0] != rows or codes.shape[1] < pitch or codes.stride(1) != 1
+                    or row < pitch or row % step or at % 16):
                 raise ValueError(f"codes of a {rows}x{cols} {format} tensor must be [{rows}, >= {pitch}] bytes, 16-byte "
                                  f"aligned, rows a multiple of {step} bytes apart, not {tuple(codes.shape)} with strides "
                                  f"{codes.stride()}")
-            if scales.numel() != scale_bytes or not scales.is_contiguous() or not _aligned(scales):
+            if scales.numel() != scale_bytes or not scales.is_contiguous() or sat % 16:
                 raise ValueError(f"scales of a {rows}x{cols} {format} tensor must be {scale_bytes} contiguous, 16-byte "
                                  f"aligned bytes, not {tuple(scales.shape)} with strides {scales.stride()}")
         if fmt == _abi.FMT_NVFP4:
-            _tensor_scale(scale, dev)
+            _check_scale(scale, codes)
         elif scale is not None:
             raise ValueError(f"{format} has no tensor scale")
-        self.codes, self.scales, self.shape, self.format, self.scale = codes, scales, (rows, cols), format, scale
-        self._abi = _abi.MicroTensor(fmt, 0, rows, cols, codes.data_ptr(), codes.stride(0) if rows > 1 else pitch,
-                                     scales.data_ptr(), scale.data_ptr() if scale is not None else None)
+        self._codes, self._scales, self._buf = codes, scales, codes
+        self.shape, self.format, self.scale = (rows, cols), format, scale
+        self._raw = _pack_tensor(fmt, 0, rows, cols, at, row, sat, scale.data_ptr() if scale is not None else 0)
 
     @classmethod
-    def empty(cls, shape, format: str, device, scale: torch.Tensor | None = None) -> "MicroTensor":
-        """Uninitialised storage for a [rows, cols] tensor, for a kernel to fill."""
-        rows, cols = shape
-        pitch, scale_bytes = _layout(_format(format), rows, cols)
-        codes = torch.empty((rows, pitch), dtype=torch.uint8, device=device)
-        return cls(codes, torch.empty(scale_bytes, dtype=torch.uint8, device=device), shape, format, scale)
+    def _new(cls, like: torch.Tensor, fmt: int, format: str, rows: int, cols: int, scale) -> "MicroTensor":
+        """Uninitialised storage (codes, then scales) on the device of `like`, for a kernel to fill."""
+        self = cls.__new__(cls)
+        pitch, scale_bytes = _layout(fmt, rows, cols)
+        buf = self._buf = like.new_empty((rows * pitch + scale_bytes,), dtype=torch.uint8)
+        at = buf.data_ptr()
+        self._codes = self._scales = None
+        self.shape, self.format, self.scale = (rows, cols), format, scale
+        self._raw = _pack_tensor(fmt, 0, rows, cols, at, pitch, at + rows * pitch,
+                                 scale.data_ptr() if scale is not None else 0)
+        return self
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            rows, cols = self.shape
+            pitch = _layout(FORMATS[self.format], rows, cols)[0]
+            self._codes = self._buf[:rows * pitch].view(rows, pitch)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            rows, cols = self.shape
+            self._scales = self._buf[rows * _layout(FORMATS[self.format], rows, cols)[0]:]
+        return self._scales
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._buf.device
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         return dequantize(self, dtype)
@@ -156,25 +213,25 @@ class MicroTensor:
         """mxfp8's codes as float8_e4m3fn [rows, cols], a view. (4-bit codes have no torch type: `dequantize`.)"""
         if self.format != "mxfp8":
             raise TypeError(f"{self.format} codes are packed; dequantize() gives their values")
-        return self.codes[:, :self.shape[1]].view(torch.float8_e4m3fn)
+        rows, cols = self.shape
+        if self._codes is None:
+            return self._buf.view(torch.float8_e4m3fn).as_strided((rows, cols), ((cols + 31) // 32 * 32, 1))
+        return self._codes[:, :cols].view(torch.float8_e4m3fn)
 
     def scale_tiles(self) -> torch.Tensor:
         """The block scales as float8_e8m0fnu (nvfp4: float8_e4m3fn), a view [row tile, 4, 32, block tile, 4]: row
         128 t + 32 i + j and block 4 u + v at [t, i, j, u, v]."""
         rows, cols = self.shape
-        tiles = self.scales.view(-(-rows // 128), -(-cols // (4 * BLOCK[self.format])), 32, 4, 4)
+        tiles = -(-cols // (4 * BLOCK[self.format]))
         kind = torch.float8_e4m3fn if self.format == "nvfp4" else torch.float8_e8m0fnu
-        return tiles.permute(0, 3, 2, 1, 4).view(kind)
+        if self._scales is None:
+            buf, start = self._buf, rows * _layout(FORMATS[self.format], rows, cols)[0]
+        else:
+            buf, start = self._scales, self._scales.storage_offset()
+        return buf.view(kind).as_strided((-(-rows // 128), 4, 32, tiles, 4), (tiles * 512, 4, 16, 512, 1), start)
 
     def __repr__(self) -> str:
         return f"MicroTensor({self.shape[0]}x{self.shape[1]}, {self.format}, {self.device})"
-
-
-def _layout(fmt: int, rows: int, cols: int) -> tuple[int, int]:
-    """(pitch, scale bytes) of a tensor: b2g_micro_layout."""
-    block = 16 if fmt == _abi.FMT_NVFP4 else 32
-    return (-(-cols // 32) * (32 if fmt == _abi.FMT_MXFP8 else 16),
-            -(-rows // 128) * -(-cols // (4 * block)) * 512)
 
 
 def quantize(x: torch.Tensor, format: str = "mxfp8", scale: torch.Tensor | None = None) -> MicroTensor:
@@ -183,22 +240,21 @@ def quantize(x: torch.Tensor, format: str = "mxfp8", scale: torch.Tensor | None 
     nvfp4: `scale` is the tensor's fp32 scale, one positive element on the device; values past 2688 times it saturate.
     Without it, x is read twice: its scale becomes the smallest power of two at which nothing saturates."""
     fmt = _format(format)
-    _values(x, "x", tuple(_VALUES))
-    if x.ndim != 2:
+    _check(x, "x", _VALUES)
+    if x.dim() != 2:
         raise ValueError(f"x must be a matrix, not {tuple(x.shape)}")
-    x = x.detach()
-    dev = x.device
-    mat = _matrix(x)
+    rows, cols = x.shape
+    mat, kind, index = _matrix(x), _VALUES[x.dtype], x.get_device()
     if fmt == _abi.FMT_NVFP4:
         if scale is None:
-            scale = torch.empty(1, dtype=torch.float32, device=dev)
-            _call(dev, "b2g_micro_tensor_scale", mat, x.shape[0], x.shape[1], _VALUES[x.dtype], scale.data_ptr())
+            scale = x.new_empty((1,), dtype=torch.float32)
+            _call(index, _entry.tensor_scale, mat, rows, cols, kind, scale.data_ptr())
         else:
-            _tensor_scale(scale, dev)
+            _check_scale(scale, x)
     elif scale is not None:
         raise ValueError(f"{format} has no tensor scale")
-    q = MicroTensor.empty(tuple(x.shape), format, dev, scale)
-    _call(dev, "b2g_micro_quantize", mat, _VALUES[x.dtype], q._abi)
+    q = MicroTensor._new(x, fmt, format, rows, cols, scale)
+    _call(index, _entry.quantize, mat, kind, q._raw)
     return q
 
 
@@ -208,27 +264,33 @@ def dequantize(q: MicroTensor, dtype: torch.dtype = torch.bfloat16, out: torch.T
     if out is None:
         if dtype not in _VALUES:
             raise TypeError(f"dtype must be float16, bfloat16 or float32, not {dtype}")
-        out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        out = q._buf.new_empty(q.shape, dtype=dtype)
     else:
-        _values(out, "out", tuple(_VALUES), q.device)
+        _check(out, "out", _VALUES, q._buf)
         if tuple(out.shape) != q.shape:
             raise ValueError(f"out must be {q.shape[0]}x{q.shape[1]}, not {tuple(out.shape)}")
-    _call(q.device, "b2g_micro_dequantize", q._abi, _matrix(out), _VALUES[out.dtype])
+    _call(q._buf.get_device(), _entry.dequantize, q._raw, _matrix(out), _VALUES[out.dtype])
     return out
 
 
 # ---------------------------------------------------------------- products
-def _status(dev: torch.device) -> torch.Tensor:
-    if dev.index not in _STATUS and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"the first product on {dev} makes the device's status word, which a stream capture cannot "
-                           "hold: run a product there once before the capture")
-    return status_word(dev)
+_STATUS_AT: dict[int, int] = {}  # address of each device's status word (the words live as long as the process)
+
+
+def _status(index: int) -> int:
+    at = _STATUS_AT.get(index)
+    if at is None:
+        if index not in _STATUS and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"the first product on cuda:{index} makes the device's status word, which a stream capture "
+                               "cannot hold: run a product there once before the capture")
+        at = _STATUS_AT[index] = status_word(torch.device("cuda", index)).data_ptr()
+    return at
 
 
 def _output(a: MicroTensor, b: MicroTensor, out: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor:
     if not isinstance(a, MicroTensor) or not isinstance(b, MicroTensor):
         raise TypeError("a and b must be MicroTensors (quantize makes them)")
-    if a.device != b.device:
+    if a._buf.get_device() != b._buf.get_device():
         raise ValueError(f"a is on {a.device}, b on {b.device}")
     if a.format != b.format:
         raise ValueError(f"a is {a.format}, b {b.format}: a product needs one format")
@@ -239,8 +301,8 @@ def _output(a: MicroTensor, b: MicroTensor, out: torch.Tensor | None, dtype: tor
     if out is None:
         if dtype not in _HALF:
             raise TypeError(f"dtype must be float16 or bfloat16, not {dtype}")
-        return torch.empty((M, N), dtype=dtype, device=a.device)
-    _values(out, "out", _HALF, a.device)
+        return a._buf.new_empty((M, N), dtype=dtype)
+    _check(out, "out", _HALF, a._buf)
     if tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
         raise ValueError(f"out must be a {M}x{N} tensor with unit column stride and rows that do not overlap, not "
                          f"{tuple(out.shape)} with strides {out.stride()}")
@@ -256,8 +318,8 @@ def micro_matmul(a: MicroTensor, b: MicroTensor, out: torch.Tensor | None = None
     """C[M, N] = A[M, K] @ B[N, K].T on the current stream, C in `dtype` (fp16 or bf16), or into `out` (unit column
     stride, any row stride) in its type."""
     c = _output(a, b, out, dtype)
-    dev = a.device
-    _call(dev, "b2g_micro_matmul", a._abi, b._abi, c.data_ptr(), _ldc(c), _VALUES[c.dtype], _status(dev).data_ptr())
+    index = c.get_device()
+    _call(index, _entry.matmul, a._raw, b._raw, c.data_ptr(), _ldc(c), _HALF[c.dtype], _status(index))
     return c
 
 
@@ -267,11 +329,11 @@ class _MicroRunner:
     __slots__ = ("_plan", "_device", "c", "status", "_keep", "_fin", "__weakref__")
 
     def __init__(self, plan: ctypes.c_void_p, c: torch.Tensor, status: torch.Tensor, keep):
-        self._plan, self._device, self.c, self.status, self._keep = plan, c.device, c, status, keep
+        self._plan, self._device, self.c, self.status, self._keep = plan, c.get_device(), c, status, keep
         self._fin = weakref.finalize(self, _abi.load().b2g_micro_plan_destroy, plan)
 
     def __call__(self) -> torch.Tensor:
-        _call(self._device, "b2g_micro_plan_launch", self._plan)
+        _call(self._device, _entry.plan_launch, self._plan)
         return self.c
 
     def device_status(self) -> int:
@@ -300,8 +362,9 @@ class MicroMatmul:
         plan = ctypes.c_void_p()
         with torch.cuda.device(a.device):
             status = torch.zeros(1, dtype=torch.int32, device=a.device)
-            _abi.check(_abi.load().b2g_micro_plan_create(a._abi, b._abi, c.data_ptr(), _ldc(c), _VALUES[c.dtype],
-                                                         status.data_ptr(), ctypes.byref(plan)), "b2g_micro_plan_create")
+            _abi.check(_abi.load().b2g_micro_plan_create(
+                _abi.MicroTensor.from_buffer_copy(a._raw), _abi.MicroTensor.from_buffer_copy(b._raw), c.data_ptr(), _ldc(c),
+                _HALF[c.dtype], status.data_ptr(), ctypes.byref(plan)), "b2g_micro_plan_create")
         return _MicroRunner(plan, c, status, (a, b))
 
 
@@ -329,44 +392,37 @@ def micro_linear(x: torch.Tensor, w: torch.Tensor, format: str = "mxfp8") -> tor
     gradient passed through the quantisations dx = q(dy) q(w^T)^T and dw = q(dy^T) q(x^T)^T. Each product's operands are
     quantised along the dimension it sums over, so the backward pass quantises x, w and dy anew from their values."""
     _format(format)
-    _values(x, "x", _HALF)
-    _values(w, "w", (x.dtype,), x.device)
-    if w.ndim != 2 or x.ndim < 1 or x.shape[-1] != w.shape[1]:
+    _check(x, "x", _HALF)
+    _check(w, "w", (x.dtype,), x)
+    if w.ndim != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"x must be [..., K] and w [N, K], not {tuple(x.shape)} and {tuple(w.shape)}")
     y = _Linear.apply(_rows(x), w, format)
-    return y if x.ndim == 2 else y.reshape(*x.shape[:-1], w.shape[0])
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.shape[0])
 
 
 # ---------------------------------------------------------------- the layers between two products
-def _coded(x: torch.Tensor, cols: int, format: str | None, scale, tensors) -> MicroTensor | None:
-    """The MicroTensor a layer writes to, or None for values."""
-    if format is None:
-        if scale is not None:
-            raise ValueError("scale belongs to format='nvfp4'")
-        return None
+def _coded(x: torch.Tensor, cols: int, format: str, scale, grad: bool) -> MicroTensor:
+    """The MicroTensor [rows of x, cols] a layer writes to."""
     fmt = _format(format)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if grad:
         raise ValueError("an output in a microscaled format has no gradient: detach the inputs, or leave format out and "
                          "let micro_linear quantise")
     if fmt == _abi.FMT_NVFP4:
         if scale is None:
             raise ValueError("nvfp4 needs the tensor's scale (calibrated: the output is not known before it is written)")
-        _tensor_scale(scale, x.device)
+        _check_scale(scale, x)
     elif scale is not None:
         raise ValueError(f"{format} has no tensor scale")
-    return MicroTensor.empty((x.shape[0], cols), format, x.device, scale)
-
-
-def _ref(m: torch.Tensor | None):
-    return None if m is None else _matrix(m)
+    return MicroTensor._new(x, fmt, format, x.shape[0], cols, scale)
 
 
 def _norm_forward(x, residual, weight, eps, q):
-    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if q is None else None
-    _call(x.device, "b2g_micro_rms_norm", _matrix(x), _ref(residual), weight.data_ptr(),
-          None if residual is None else _matrix(h), _ref(y), None if q is None else q._abi, x.shape[0], x.shape[1], eps,
-          _VALUES[x.dtype])
+    h = x if residual is None else _like(x)
+    y = _like(x) if q is None else None
+    rows, cols = x.shape
+    _call(x.get_device(), _entry.rms_norm, _matrix(x), None if residual is None else _matrix(residual), weight.data_ptr(),
+          None if residual is None else _matrix(h), None if y is None else _matrix(y), None if q is None else q._raw, rows,
+          cols, eps, _HALF[x.dtype])
     return (y if q is None else q), h
 
 
@@ -397,28 +453,33 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     sum rounded to the type, the next layer's residual. Without `format` y has x's type and shape and both outputs are
     differentiable. With one, y is a MicroTensor [rows, cols], the next product's operand; nvfp4 then needs the tensor's
     `scale`."""
-    _values(x, "x", _HALF)
-    _values(weight, "weight", (x.dtype,), x.device)
-    if x.ndim < 1 or weight.shape != x.shape[-1:]:
-        raise ValueError(f"weight must be [{x.shape[-1] if x.ndim else '?'}], not {tuple(weight.shape)}")
+    _check(x, "x", _HALF)
+    _check(weight, "weight", (x.dtype,), x)
+    if x.dim() < 1 or weight.shape != x.shape[-1:]:
+        raise ValueError(f"weight must be [{x.shape[-1] if x.dim() else '?'}], not {tuple(weight.shape)}")
+    x2, r2, grad = _rows(x), None, x.requires_grad or weight.requires_grad
     if residual is not None:
-        _values(residual, "residual", (x.dtype,), x.device)
+        _check(residual, "residual", (x.dtype,), x)
         if residual.shape != x.shape:
             raise ValueError(f"residual is {tuple(residual.shape)}, x {tuple(x.shape)}")
-    x2 = _rows(x)
-    r2 = None if residual is None else _rows(residual)
+        r2 = _rows(residual)
+        grad = grad or residual.requires_grad
+    grad = grad and torch.is_grad_enabled()
     if not weight.is_contiguous():
         weight = weight.contiguous()
-    q = _coded(x2, x2.shape[1], format, scale, (x, weight, residual))
-    if q is None and torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (
-            residual is not None and residual.requires_grad)):
+    if format is not None:
+        y, h = _norm_forward(x2, r2, weight, eps, _coded(x2, x2.shape[1], format, scale, grad))
+    elif scale is not None:
+        raise ValueError("scale belongs to format='nvfp4'")
+    elif grad:
         out = _Norm.apply(x2, r2, weight, eps)
         y, h = (out, x2) if residual is None else out
     else:
-        y, h = _norm_forward(x2, r2, weight, eps, q)
-    if q is None and x.ndim != 2:
-        y = y.reshape(x.shape)
-    return y, (x if residual is None else h if x.ndim == 2 else h.reshape(x.shape))
+        y, h = _norm_forward(x2, r2, weight, eps, None)
+    if x.dim() != 2:
+        y = y if format is not None else y.reshape(x.shape)
+        h = h.reshape(x.shape)
+    return y, (x if residual is None else h)
 
 
 def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
@@ -426,33 +487,33 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, e
     """(dx, dweight) of rms_norm from the gradient of y and h, the sum it normalised. `dh`: the gradient that arrives at
     h itself (along the residual), added to dx. dx is the gradient of both x and the residual. The sums' order is fixed:
     results repeat bit for bit."""
-    _values(h, "h", _HALF)
-    for t, what in ((dy, "dy"), (weight, "weight"), (dh, "dh")):
-        if t is not None:
-            _values(t, what, (h.dtype,), h.device)
-    if h.ndim < 1 or weight.shape != h.shape[-1:] or dy.shape != h.shape or (dh is not None and dh.shape != h.shape):
+    _check(h, "h", _HALF)
+    _check(dy, "dy", (h.dtype,), h)
+    _check(weight, "weight", (h.dtype,), h)
+    if dh is not None:
+        _check(dh, "dh", (h.dtype,), h)
+    if h.dim() < 1 or weight.shape != h.shape[-1:] or dy.shape != h.shape or (dh is not None and dh.shape != h.shape):
         raise ValueError(f"dy {tuple(dy.shape)}, dh and h {tuple(h.shape)} must have one shape, weight "
                          f"{tuple(weight.shape)} its last dimension")
-    dy2, h2 = _rows(dy.detach()), _rows(h.detach())
-    dh2 = None if dh is None else _rows(dh.detach())
-    weight = weight.detach().contiguous()
+    dy2, h2, dh2 = _rows(dy), _rows(h), None if dh is None else _rows(dh)  # held until the launch: some may be copies
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
     rows, cols = h2.shape
-    dev = h.device
     n = ctypes.c_size_t(0)
-    _abi.check(_abi.load().b2g_micro_rms_norm_workspace(rows, cols, ctypes.byref(n)), "b2g_micro_rms_norm_workspace")
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-    dx = torch.empty((rows, cols), dtype=h.dtype, device=dev)
-    dw = torch.empty(cols, dtype=h.dtype, device=dev)
-    _call(dev, "b2g_micro_rms_norm_backward", _matrix(dy2), _matrix(h2), weight.data_ptr(), _ref(dh2), _matrix(dx),
-          dw.data_ptr(), ws.data_ptr(), n.value, rows, cols, eps, _VALUES[h.dtype])
-    return (dx if h.ndim == 2 else dx.reshape(h.shape)), dw
+    _abi.check(_abi.load().b2g_micro_rms_norm_workspace(rows, cols, n), "b2g_micro_rms_norm_workspace")
+    dx, dw = _like(h2), _like(weight)
+    ws = h2.new_empty((n.value,), dtype=torch.uint8)
+    _call(h.get_device(), _entry.rms_norm_backward, _matrix(dy2), _matrix(h2), weight.data_ptr(),
+          None if dh is None else _matrix(dh2), _matrix(dx), dw.data_ptr(), ws.data_ptr(), n.value, rows, cols, eps,
+          _HALF[h.dtype])
+    return (dx if h.dim() == 2 else dx.reshape(h.shape)), dw
 
 
 def _gate_forward(x, q):
-    cols = x.shape[1] // 2
-    y = torch.empty((x.shape[0], cols), dtype=x.dtype, device=x.device) if q is None else None
-    _call(x.device, "b2g_micro_silu_mul", _matrix(x), _ref(y), None if q is None else q._abi, x.shape[0], cols,
-          _VALUES[x.dtype])
+    rows, cols = x.shape[0], x.shape[1] // 2
+    y = x.new_empty((rows, cols)) if q is None else None
+    _call(x.get_device(), _entry.silu_mul, _matrix(x), None if y is None else _matrix(y), None if q is None else q._raw,
+          rows, cols, _HALF[x.dtype])
     return y if q is None else q
 
 
@@ -469,8 +530,8 @@ class _Gate(torch.autograd.Function):
 
 
 def _gate_input(x: torch.Tensor) -> None:
-    _values(x, "gate_up", _HALF)
-    if x.ndim < 1 or x.shape[-1] % 2:
+    _check(x, "gate_up", _HALF)
+    if x.dim() < 1 or x.shape[-1] % 2:
         raise ValueError(f"gate_up must be [..., 2 * cols] = [gate | up], not {tuple(x.shape)}")
 
 
@@ -479,23 +540,27 @@ def silu_mul(gate_up: torch.Tensor, format: str | None = None, scale: torch.Tens
     same type, differentiable, or with `format` a MicroTensor [rows, cols] for the next product (nvfp4 needs `scale`)."""
     _gate_input(gate_up)
     x = _rows(gate_up)
-    q = _coded(x, x.shape[1] // 2, format, scale, (gate_up,))
-    y = _Gate.apply(x) if q is None and torch.is_grad_enabled() and gate_up.requires_grad else _gate_forward(x, q)
-    return y if q is not None or gate_up.ndim == 2 else y.reshape(*gate_up.shape[:-1], x.shape[1] // 2)
+    grad = gate_up.requires_grad and torch.is_grad_enabled()
+    if format is not None:
+        return _gate_forward(x, _coded(x, x.shape[1] // 2, format, scale, grad))
+    if scale is not None:
+        raise ValueError("scale belongs to format='nvfp4'")
+    y = _Gate.apply(x) if grad else _gate_forward(x, None)
+    return y if gate_up.dim() == 2 else y.reshape(*gate_up.shape[:-1], x.shape[1] // 2)
 
 
 def silu_mul_backward(dy: torch.Tensor, gate_up: torch.Tensor) -> torch.Tensor:
     """The gradient of silu_mul's input [..., 2 * cols] from that of its output."""
     _gate_input(gate_up)
-    _values(dy, "dy", (gate_up.dtype,), gate_up.device)
+    _check(dy, "dy", (gate_up.dtype,), gate_up)
     cols = gate_up.shape[-1] // 2
     if dy.shape != (*gate_up.shape[:-1], cols):
         raise ValueError(f"dy is {tuple(dy.shape)}, gate_up {tuple(gate_up.shape)}")
-    dy2, x = _rows(dy.detach()), _rows(gate_up.detach())
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _call(x.device, "b2g_micro_silu_mul_backward", _matrix(dy2), _matrix(x), _matrix(dx), x.shape[0], cols,
-          _VALUES[x.dtype])
-    return dx if gate_up.ndim == 2 else dx.reshape(gate_up.shape)
+    x, dy2 = _rows(gate_up), _rows(dy)  # held until the launch: some may be copies
+    dx = _like(x)
+    _call(x.get_device(), _entry.silu_mul_backward, _matrix(dy2), _matrix(x), _matrix(dx), x.shape[0], cols,
+          _HALF[x.dtype])
+    return dx if gate_up.dim() == 2 else dx.reshape(gate_up.shape)
 
 
 def micro_mlp(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: torch.Tensor, w_gate_up: MicroTensor,
@@ -510,4 +575,4 @@ def micro_mlp(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: torch
     n, h = rms_norm(x, norm_weight, residual=residual, eps=eps, format=w_gate_up.format, scale=s[0])
     g = silu_mul(micro_matmul(n, w_gate_up, dtype=x.dtype), format=w_down.format, scale=s[1])
     y = micro_matmul(g, w_down, dtype=x.dtype)
-    return (y if x.ndim == 2 else y.reshape(*x.shape[:-1], w_down.shape[0])), h
+    return (y if x.dim() == 2 else y.reshape(*x.shape[:-1], w_down.shape[0])), h
