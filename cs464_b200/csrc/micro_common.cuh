@@ -268,42 +268,71 @@ __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7fffffffu) : byte ? __uint_as_float(byte << 23) : __uint_as_float(0x00400000u);
 }
 
+// Bits of the largest magnitude among eight values, as an fp32's; at least 0x7f800000 where an infinity or a NaN is among
+// them. The integer pipe is what bounds the quantising kernels, so 16-bit values are compared as they lie, two at a time
+// (magnitudes order as their bits do), and fp32 values by a maximum that takes the magnitude on the way, with a product
+// by zero on the otherwise idle multiply-add pipe to catch what is not finite.
+__device__ __forceinline__ uint32_t amax8(const Raw8<__nv_bfloat16>& r) {
+  const uint32_t k = 0x7fff7fffu;
+  const uint32_t m = __vmaxu2(__vmaxu2(r.v.x & k, r.v.y & k), __vmaxu2(r.v.z & k, r.v.w & k));
+  return max(m & 0xffff0000u, m << 16);
+}
+__device__ __forceinline__ uint32_t amax8(const Raw8<__half>& r) {
+  const uint32_t k = 0x7fff7fffu;
+  const uint32_t m = __vmaxu2(__vmaxu2(r.v.x & k, r.v.y & k), __vmaxu2(r.v.z & k, r.v.w & k));
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(max(m >> 16, m & 0xffffu)))));
+}
+__device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
+  float m = 0.f, p = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    m = fmaxf(m, fabsf(v[i]));
+    p = fmaf(v[i], 0.f, p);
+  }
+  return p == 0.f ? __float_as_uint(m) : 0x7fffffffu;
+}
+__device__ __forceinline__ uint32_t amax8(const Raw8<float>& r) {
+  float v[8];
+  unpack8(r, v);
+  return amax8(v);
+}
+
 // One block's quantiser: its scale byte, and how an element becomes a code's value.
 //   MX: x * 2^-e, exact unless it leaves fp32's range at the bottom, where the code is zero anyway.
 //   NVFP4: x / u, u = block scale * tensor scale, correctly rounded as a division's quotient so that values on the
 //   border between two codes fall as the definition says: one reciprocal a block, then per element the quotient's
 //   estimate corrected by its residual (Markstein, "Computation of elementary functions on the IBM RISC System/6000
-//   processor", 1990). A block whose scale rounds to zero is zero; zeros keep the value's sign.
+//   processor", 1990). The residual is taken negated, so that zeros keep the value's sign. A block whose scale rounds to
+//   zero is zero.
+// The codes of a NaN block are cleared by `keep`.
 template <int FMT>
 struct BlockQuant {
   uint32_t byte;
-  float mul;   // MX: 2^-e; NVFP4: 1 / u; 0: every code is zero
-  float unit;  // NVFP4: u
-  uint32_t sign;  // NVFP4: the sign bit, 0 in a NaN block
+  uint32_t keep;  // all ones; 0 in a NaN block
+  float mul;      // MX: 2^-e; NVFP4: 1 / u, or 0
+  float unit;     // NVFP4: u
   __device__ __forceinline__ void init(uint32_t amax_bits, float tensor_scale) {
+    const bool bad = amax_bits >= 0x7f800000u;
+    keep = bad ? 0u : 0xffffffffu;
     if constexpr (FMT == FMT_NVFP4) {
       const float s = __fdiv_rn(__uint_as_float(amax_bits), 6.f * tensor_scale);
-      byte = amax_bits >= 0x7f800000u ? 0x7fu : __nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3);
+      byte = bad ? 0x7fu : __nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3);
       unit = e4m3_to_f32(byte) * tensor_scale;
-      mul = (byte == 0u || byte == 0x7fu) ? 0.f : __frcp_rn(unit);
-      sign = byte == 0x7fu ? 0u : 0x80000000u;
+      mul = byte == 0u ? 0.f : __frcp_rn(unit);
     } else {
       byte = mx_scale_byte<FMT>(amax_bits);
-      mul = byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
+      mul = __uint_as_float((254u - byte) << 23);
     }
   }
   __device__ __forceinline__ float scaled(float x) const {
     if constexpr (FMT == FMT_NVFP4) {
       const float q = x * mul;
-      const float r = mul == 0.f ? 0.f : fmaf(fmaf(-q, unit, x), mul, q);
-      return __uint_as_float((__float_as_uint(r) & 0x7fffffffu) | (__float_as_uint(x) & sign));
+      return fmaf(-fmaf(q, unit, -x), mul, q);
     } else {
-      return mul == 0.f ? 0.f : x * mul;
+      return x * mul;
     }
   }
 };
-
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
@@ -311,10 +340,18 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return lo | hi << 16;
 }
 
-__device__ __forceinline__ uint32_t e2m1x4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp4x2(make_float2(a, b), __NV_E2M1, cudaRoundNearest);
-  const uint32_t hi = __nv_cvt_float2_to_fp4x2(make_float2(c, d), __NV_E2M1, cudaRoundNearest);
-  return lo | hi << 8;
+// Eight e2m1 codes, the lowest value in the lowest bits: four conversions of two values to a byte and one packing move.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
 }
 
 // Eight values' codes: .x (and .y for MXFP8), lowest column in the lowest bits.
@@ -323,22 +360,20 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], const BlockQuant<FM
   float s[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) s[i] = b.scaled(v[i]);
-  if constexpr (FMT == FMT_MXFP8) return make_uint2(e4m3x4(s[0], s[1], s[2], s[3]), e4m3x4(s[4], s[5], s[6], s[7]));
-  else return make_uint2(e2m1x4(s[0], s[1], s[2], s[3]) | e2m1x4(s[4], s[5], s[6], s[7]) << 16, 0u);
+  if constexpr (FMT == FMT_MXFP8)
+    return make_uint2(e4m3x4(s[0], s[1], s[2], s[3]) & b.keep, e4m3x4(s[4], s[5], s[6], s[7]) & b.keep);
+  else return make_uint2(e2m1x8(s) & b.keep, 0u);
 }
 
 // Quantise eight consecutive columns per lane, the warp's 32 lanes holding 256 consecutive columns from `col` (lane 0's
 // first, a multiple of 256 past the row's start), and store them: the codes of columns below `code_cols` (a multiple of
-// 32), and the scale words of tile columns below `ktiles`. A block's lanes (4 for blocks of 32, 2 for 16) share its
-// largest magnitude by shuffles; the four scale bytes of one tile row are gathered into one 4-byte store. Called by a
-// converged warp.
+// 32), and the scale words of tile columns below `ktiles`. `m`: the eight values' amax8. A block's lanes (4 for blocks of
+// 32, 2 for 16) share their largest magnitude by shuffles; the four scale bytes of one tile row are gathered into one
+// 4-byte store. Called by a converged warp.
 template <int FMT>
-__device__ __forceinline__ void quantize_store(const float (&v)[8], int lane, int64_t c, int64_t code_cols,
+__device__ __forceinline__ void quantize_store(const float (&v)[8], uint32_t m, int lane, int64_t c, int64_t code_cols,
                                                uint8_t* code_row, uint8_t* scale_row0, int64_t ktiles, float tensor_scale) {
   constexpr int kLanes = block_of(FMT) / 8;
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
 #pragma unroll
   for (int d = 1; d < kLanes; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
   BlockQuant<FMT> b;

@@ -105,14 +105,19 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
 
   const int64_t cover = FMT == FMT_NONE ? cols : q.ktiles * 4 * block_of(FMT);  // whole scale tiles
   auto finish = [&](float(&f)[8], int64_t c) {
-    float g[8];
-    unpack8(load8<T, VEC>(w, 1, c, cols), g);
+    if (c < lim) {  // a chunk that ends past the row: its further values and weights were read as zero
+      float g[8];
+      unpack8(load8<T, VEC>(w, 1, c, cols), g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = live && c + i < cols ? f[i] * r * g[i] : 0.f;
+      for (int i = 0; i < 8; ++i) f[i] = f[i] * r * g[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    }
     if constexpr (FMT == FMT_NONE) {
       if (c < lim) store8<T, VEC>(y + row * syr, syc, c, lim, pack8<T>(f));
     } else {
-      quantize_store<FMT>(f, threadIdx.x & 31, c, live ? q.code_cols : 0, q.codes + row * q.pitch,
+      quantize_store<FMT>(f, amax8(f), threadIdx.x & 31, c, live ? q.code_cols : 0, q.codes + row * q.pitch,
                           q.scales + scale_row(row, q.ktiles), q.ktiles, ts);
     }
   };

@@ -14,31 +14,38 @@ constexpr int kWarps = 8;  // per block
 // ---------------------------------------------------------------- largest magnitude -> NVFP4 tensor scale
 // The smallest power of two 2^e >= 2^-100 with amax <= 2688 * 2^e (2688 = 6 * 448 = 1.3125 * 2^11). Every block takes
 // the maximum of its own candidate: the order does not matter. Infinities and NaN do not count.
+// A row's eight-column chunks are numbered across rows; a thread steps by the whole grid, four chunks in flight, and
+// carries (row, chunk) along instead of dividing.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32) tensor_scale_kernel(Mat x, int64_t rows, int64_t cols, float* scale) {
-  const int64_t chunks = (cols + 7) / 8;
-  const int64_t total = rows * chunks;
-  uint32_t m = 0;
+__global__ void __launch_bounds__(kWarps * 32)
+    tensor_scale_kernel(Mat x, int64_t rows, int64_t cols, int64_t chunks, int64_t step_rows, int64_t step_chunks, float* scale) {
+  const int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
+  int64_t row = first / chunks, k = first - row * chunks;
   const T* p = static_cast<const T*>(x.p);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total; i += 4 * step) {
+  uint32_t m = 0;
+  while (row < rows) {
     Raw8<T> r[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int64_t k = i + u * step;
-      const int64_t row = k < total ? k / chunks : 0;
-      const int64_t c = k < total ? (k - row * chunks) * 8 : cols;
-      r[u] = load8<T, VEC>(p + row * x.sr, x.sc, c, cols);
+      r[u] = load8<T, VEC>(p + row * x.sr, x.sc, k * 8, row < rows ? cols : 0);
+      row += step_rows;
+      k += step_chunks;
+      if (k >= chunks) {
+        k -= chunks;
+        ++row;
+      }
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      float v[8];
-      unpack8(r[u], v);
+      uint32_t a = amax8(r[u]);
+      if (a >= 0x7f800000u) {  // something is not finite: take the others one by one
+        float v[8];
+        unpack8(r[u], v);
+        a = 0;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const uint32_t a = abs_bits(v[q]);
-        m = max(m, a >= 0x7f800000u ? 0u : a);
+        for (int i = 0; i < 8; ++i) a = max(a, isfinite(v[i]) ? __float_as_uint(fabsf(v[i])) : 0u);
       }
+      m = max(m, a);
     }
   }
   m = __reduce_max_sync(0xffffffffu, m);
@@ -58,7 +65,10 @@ __global__ void __launch_bounds__(kWarps * 32) tensor_scale_kernel(Mat x, int64_
 template <typename T>
 struct ValueSource {
   static constexpr int kLoads = 1;
-  __device__ __forceinline__ static void value(const Raw8<T> (&r)[1], float (&v)[8]) { unpack8(r[0], v); }
+  __device__ __forceinline__ static uint32_t value(const Raw8<T> (&r)[1], float (&v)[8]) {  // and their amax8
+    unpack8(r[0], v);
+    return amax8(r[0]);
+  }
 };
 
 // 1 / (1 + exp(-x)), the exponential and the division in their fast forms: their errors (2 + 1.173 |x| and 2 ulps) are far
@@ -69,12 +79,13 @@ __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f +
 template <typename T>
 struct GateSource {
   static constexpr int kLoads = 2;
-  __device__ __forceinline__ static void value(const Raw8<T> (&r)[2], float (&v)[8]) {
+  __device__ __forceinline__ static uint32_t value(const Raw8<T> (&r)[2], float (&v)[8]) {
     float g[8], u[8];
     unpack8(r[0], g);
     unpack8(r[1], u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = g[i] * sigmoid(g[i]) * u[i];
+    return amax8(v);
   }
 };
 
@@ -104,9 +115,9 @@ __global__ void __launch_bounds__(kWarps * 32)
   for (int i = 0; i < 4; ++i) {
     const int64_t row = row0 + 32 * i;
     float v[8];
-    S::value(r[i], v);
+    const uint32_t m = S::value(r[i], v);
     // rows past the last get zero scales and no codes
-    quantize_store<FMT>(v, lane, c, row < rows ? q.code_cols : 0, q.codes + row * q.pitch,
+    quantize_store<FMT>(v, m, lane, c, row < rows ? q.code_cols : 0, q.codes + row * q.pitch,
                         q.scales + scale_row(row, q.ktiles), q.ktiles, ts);
   }
 }
@@ -180,16 +191,17 @@ __global__ void __launch_bounds__(128) quantize_cols_kernel(Mat x, int64_t rows,
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
       float v[kBlk];
-      uint32_t m = 0;
+      float m = 0.f, bad = 0.f;  // as amax8 of values
 #pragma unroll
       for (int i = 0; i < kBlk; ++i) {
         float f[4];
         unpack4(raw[s * kBlk + i], f);
         v[i] = f[k];
-        m = max(m, abs_bits(v[i]));
+        m = fmaxf(m, fabsf(v[i]));
+        bad = fmaf(v[i], 0.f, bad);
       }
       BlockQuant<FMT> b;
-      b.init(m, ts);
+      b.init(bad == 0.f ? __float_as_uint(m) : 0x7fffffffu, ts);
 #pragma unroll
       for (int g = 0; g < kBlk / 8; ++g) {
         float e[8];
@@ -228,7 +240,8 @@ __global__ void __launch_bounds__(128) quantize_cols_kernel(Mat x, int64_t rows,
 }
 
 // ---------------------------------------------------------------- codes and scales -> values
-// A lane reads 16 columns' codes of four rows (16 bytes each of e4m3, 8 of e2m1) and each row's one scale byte.
+// A lane reads eight columns' codes of four rows, twice (256 columns apart), with each block's one scale byte, and stores
+// 16 bytes a row (fp32: 32), a warp 512 consecutive ones.
 template <typename T, int FMT, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32)
     dequantize_kernel(const uint8_t* codes, int64_t pitch, const uint8_t* scales, const float* scale, int64_t rows,
@@ -237,45 +250,43 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int64_t task = blockIdx.x * static_cast<int64_t>(kWarps) + (threadIdx.x >> 5);
   if (task >= tasks) return;
   const int64_t rj = task / col_chunks;
-  const int64_t c = (task - rj * col_chunks) * 512 + lane * 16;
-  if (c >= cols) return;
+  const int64_t c0 = (task - rj * col_chunks) * 512 + lane * 8;
   const int64_t row0 = (rj >> 5) * 128 + (rj & 31);
   const float ts = FMT == FMT_NVFP4 ? *scale : 1.f;
-  const int64_t blk = c / block_of(FMT);
-  const uint8_t* sp = scales + scale_row(row0, ktiles) + (blk >> 2) * 512 + (blk & 3);
-  uint4 q[4];
-  uint32_t s[4];
+  uint2 q[2][4];
+  uint32_t s[2][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = row0 + 32 * i;
-    if (row < rows) {  // a row's codes are readable up to a multiple of 32 columns
-      if constexpr (FMT == FMT_MXFP8) {
-        q[i] = __ldg(reinterpret_cast<const uint4*>(codes + row * pitch + c));
-      } else {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + row * pitch + (c >> 1)));
-        q[i] = make_uint4(w.x, w.y, 0u, 0u);
+  for (int h = 0; h < 2; ++h) {
+    const int64_t c = c0 + 256 * h, blk = c / block_of(FMT);
+    const uint8_t* sp = scales + scale_row(row0, ktiles) + (blk >> 2) * 512 + (blk & 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = row0 + 32 * i;
+      if (row < rows && c < cols) {  // a row's codes are readable up to a multiple of 32 columns
+        if constexpr (FMT == FMT_MXFP8) q[h][i] = __ldg(reinterpret_cast<const uint2*>(codes + row * pitch + c));
+        else q[h][i].x = __ldg(reinterpret_cast<const uint32_t*>(codes + row * pitch + (c >> 1)));
+        s[h][i] = __ldg(sp + i * 4);
       }
-      s[i] = __ldg(sp + i * 4);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = row0 + 32 * i;
-    if (row >= rows) break;
-    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-    float bs;
-    if constexpr (FMT == FMT_NVFP4) bs = e4m3_to_f32(s[i]);
-    else bs = mx_scale_value(s[i]);
+  for (int h = 0; h < 2; ++h) {
+    const int64_t c = c0 + 256 * h;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = row0 + 32 * i;
+      if (row >= rows || c >= cols) break;
+      float bs;
+      if constexpr (FMT == FMT_NVFP4) bs = e4m3_to_f32(s[h][i]);
+      else bs = mx_scale_value(s[h][i]);
       float v[8];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         __half2_raw p;
         if constexpr (FMT == FMT_MXFP8)
-          p = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[2 * h + k / 2] >> (16 * (k & 1))), __NV_E4M3);
+          p = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((k < 2 ? q[h][i].x : q[h][i].y) >> (16 * (k & 1))), __NV_E4M3);
         else
-          p = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(w[h] >> (8 * k)), __NV_E2M1);
+          p = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(q[h][i].x >> (8 * k)), __NV_E2M1);
         const float2 f = __half22float2(__half2(p));
         // code * block scale is exact in fp32 (4 bits of e4m3 with a power of two, 2 bits of e2m1 with 4 of e4m3)
         v[2 * k] = f.x * bs;
@@ -285,18 +296,18 @@ __global__ void __launch_bounds__(kWarps * 32)
           v[2 * k + 1] *= ts;
         }
       }
-      store8<T, VEC>(out + row * sr, sc, c + 8 * h, cols, pack8<T>(v));
+      store8<T, VEC>(out + row * sr, sc, c, cols, pack8<T>(v));
     }
   }
 }
 
 // ---------------------------------------------------------------- the gate as values, and its gradient
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) gate_kernel(Mat x, T* y, int64_t syr, int64_t syc, int64_t rows, int64_t cols) {
-  const int64_t chunks = (cols + 7) / 8, total = rows * chunks;
-  const int64_t k = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x;
-  if (k >= total) return;
-  const int64_t row = k / chunks, c = (k - row * chunks) * 8;
+__global__ void __launch_bounds__(256) gate_kernel(Mat x, T* y, int64_t syr, int64_t syc, int64_t rows, int64_t cols, uint32_t row_blocks) {
+  // blockDim.y rows of blockDim.x chunks of eight columns; row_blocks blocks along a row
+  const uint32_t k = blockIdx.x % row_blocks * blockDim.x + threadIdx.x;
+  const int64_t row = static_cast<int64_t>(blockIdx.x / row_blocks) * blockDim.y + threadIdx.y, c = static_cast<int64_t>(k) * 8;
+  if (row >= rows || c >= cols) return;
   const T* p = static_cast<const T*>(x.p) + row * x.sr;
   Raw8<T> r[2] = {load8<T, VEC>(p, x.sc, c, cols), load8<T, VEC>(p + cols * x.sc, x.sc, c, cols)};
   float v[8];
@@ -308,11 +319,12 @@ __global__ void __launch_bounds__(256) gate_kernel(Mat x, T* y, int64_t syr, int
 // keeps its digits where s is near one.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-    gate_backward_kernel(Mat dy, Mat x, T* dx, int64_t sxr, int64_t sxc, int64_t rows, int64_t cols) {
-  const int64_t chunks = (cols + 7) / 8, total = rows * chunks;
-  const int64_t k = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x;
-  if (k >= total) return;
-  const int64_t row = k / chunks, c = (k - row * chunks) * 8;
+    gate_backward_kernel(Mat dy, Mat x, T* dx, int64_t sxr, int64_t sxc, int64_t rows, int64_t cols,
+                         uint32_t row_blocks) {
+  // blockDim.y rows of blockDim.x chunks of eight columns; row_blocks blocks along a row
+  const uint32_t k = blockIdx.x % row_blocks * blockDim.x + threadIdx.x;
+  const int64_t row = static_cast<int64_t>(blockIdx.x / row_blocks) * blockDim.y + threadIdx.y, c = static_cast<int64_t>(k) * 8;
+  if (row >= rows || c >= cols) return;
   const T* p = static_cast<const T*>(x.p) + row * x.sr;
   const Raw8<T> rg = load8<T, VEC>(p, x.sc, c, cols), ru = load8<T, VEC>(p + cols * x.sc, x.sc, c, cols);
   const Raw8<T> rd = load8<T, VEC>(static_cast<const T*>(dy.p) + row * dy.sr, dy.sc, c, cols);
@@ -333,6 +345,22 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------- host side
+// Blocks of 256 threads over rows of eight-column chunks: several rows a block where they are short.
+struct RowBlocks {
+  dim3 block;
+  uint32_t along;
+  int64_t grid;
+};
+
+RowBlocks row_blocks(int64_t rows, int64_t cols) {
+  const int64_t chunks = ceil_div(cols, 8);
+  unsigned x = 1;
+  while (x < chunks && x < 256) x *= 2;
+  RowBlocks b{dim3(x, 256 / x), static_cast<uint32_t>(ceil_div(chunks, x)), 0};
+  b.grid = ceil_div(rows, b.block.y) * b.along;
+  return b;
+}
+
 template <typename T, int FMT, bool VEC, template <typename> class SRC>
 int32_t run_rows(const Mat& x, int64_t rows, int64_t cols, const Quant& q, cudaStream_t st) {
   const int64_t col_chunks = ceil_div(q.ktiles * 4 * block_of(FMT), 256);  // whole scale tiles, so that all are written
@@ -405,10 +433,14 @@ int32_t b2g_micro_tensor_scale(const b2g_micro_matrix* x, int64_t rows, int64_t 
         std::swap(r, c);
       }
       const b2g_micro_matrix view = {const_cast<void*>(m.p), m.sr, m.sc};
-      const int64_t want = ceil_div(r * ceil_div(c, 8), kWarps * 32 * 4);
+      const int64_t chunks = c > 0 ? ceil_div(c, 8) : 1;
+      const int64_t want = ceil_div(r * chunks, kWarps * 32 * 4);
       const unsigned grid = static_cast<unsigned>(want < 1 ? 1 : want > 148 * 8 ? 148 * 8 : want);
-      if (vec_ok(&view, r, sizeof(T))) tensor_scale_kernel<T, true><<<grid, kWarps * 32, 0, st>>>(m, r, c, scale);
-      else tensor_scale_kernel<T, false><<<grid, kWarps * 32, 0, st>>>(m, r, c, scale);
+      const int64_t step = static_cast<int64_t>(grid) * kWarps * 32;
+      if (vec_ok(&view, r, sizeof(T)))
+        tensor_scale_kernel<T, true><<<grid, kWarps * 32, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
+      else
+        tensor_scale_kernel<T, false><<<grid, kWarps * 32, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
       return launched("tensor_scale launch");
     });
   });
@@ -481,12 +513,13 @@ int32_t b2g_micro_silu_mul(const b2g_micro_matrix* gate_up, const b2g_micro_matr
           });
         }
         if (const int32_t rc = check_matrix(y, "y")) return rc;
-        const int64_t grid = ceil_div(rows * ceil_div(cols, 8), 256);
+        const RowBlocks rb = row_blocks(rows, cols);
+    const int64_t grid = rb.grid;
         if (grid > kMaxGrid) return too_large("silu_mul");
         if (vec && vec_ok(y, rows, 2))
-          gate_kernel<T, true><<<static_cast<unsigned>(grid), 256, 0, st>>>(mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols);
+          gate_kernel<T, true><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols, rb.along);
         else
-          gate_kernel<T, false><<<static_cast<unsigned>(grid), 256, 0, st>>>(mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols);
+          gate_kernel<T, false><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols, rb.along);
         return launched("silu_mul launch");
       }
     });
@@ -503,7 +536,8 @@ int32_t b2g_micro_silu_mul_backward(const b2g_micro_matrix* dy, const b2g_micro_
     if (const int32_t rc = check_matrix(dy, "dy")) return rc;
     if (const int32_t rc = check_matrix(gate_up, "gate_up")) return rc;
     if (const int32_t rc = check_matrix(dgate_up, "dgate_up")) return rc;
-    const int64_t grid = ceil_div(rows * ceil_div(cols, 8), 256);
+    const RowBlocks rb = row_blocks(rows, cols);
+    const int64_t grid = rb.grid;
     if (grid > kMaxGrid) return too_large("silu_mul_backward");
     return by_type(dtype, [&](auto t) -> int32_t {
       using T = decltype(t);
@@ -513,9 +547,9 @@ int32_t b2g_micro_silu_mul_backward(const b2g_micro_matrix* dy, const b2g_micro_
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         T* out = static_cast<T*>(dgate_up->ptr);
         if (vec_ok(dy, rows, 2) && vec_ok(gate_up, rows, 2) && vec_ok(dgate_up, rows, 2) && cols % 8 == 0)
-          gate_backward_kernel<T, true><<<static_cast<unsigned>(grid), 256, 0, st>>>(mat(dy), mat(gate_up), out, dgate_up->stride_r, dgate_up->stride_c, rows, cols);
+          gate_backward_kernel<T, true><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(dy), mat(gate_up), out, dgate_up->stride_r, dgate_up->stride_c, rows, cols, rb.along);
         else
-          gate_backward_kernel<T, false><<<static_cast<unsigned>(grid), 256, 0, st>>>(mat(dy), mat(gate_up), out, dgate_up->stride_r, dgate_up->stride_c, rows, cols);
+          gate_backward_kernel<T, false><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(dy), mat(gate_up), out, dgate_up->stride_r, dgate_up->stride_c, rows, cols, rb.along);
         return launched("silu_mul_backward launch");
       }
     });
