@@ -79,9 +79,9 @@ struct Quant {  // where a microscaled tensor goes
   int64_t pitch, ktiles, code_cols;
 };
 
-// Whether rows of `m` can be read and written in 16-byte pieces.
-inline bool vec_ok(const b2g_micro_matrix* m, int64_t rows, int64_t size) {
-  return m->stride_c == 1 && aligned16(m->ptr) && (rows <= 1 || (m->stride_r * size) % 16 == 0);
+// Whether rows of `cols` values of `m` can be read and written in whole 16-byte pieces of eight columns.
+inline bool vec_ok(const b2g_micro_matrix* m, int64_t rows, int64_t cols, int64_t size) {
+  return m->stride_c == 1 && cols % 8 == 0 && aligned16(m->ptr) && (rows <= 1 || (m->stride_r * size) % 16 == 0);
 }
 
 inline Mat mat(const b2g_micro_matrix* m) { return Mat{m->ptr, m->stride_r, m->stride_c}; }
@@ -216,36 +216,43 @@ __device__ __forceinline__ Raw8<float> pack8<float>(const float (&v)[8]) {
                      make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]))};
 }
 
-// Columns c .. c+7 of a row that starts at `row`; columns at or past `cols` read as zero. VEC: unit column stride and
-// 16-byte aligned rows, so eight columns that all exist are one or two 16-byte loads.
+// Columns c .. c+7 of a row that starts at `row`; columns at or past `cols` read as zero. VEC: unit column stride, 16-byte
+// aligned rows and `cols` a multiple of 8, so that eight columns exist or do not, and are one or two 16-byte loads.
 template <typename T, bool VEC>
 __device__ __forceinline__ Raw8<T> load8(const T* row, int64_t stride_c, int64_t c, int64_t cols) {
-  if (VEC && c + 8 <= cols) {
-    Raw8<T> r;
-    const uint4* p = reinterpret_cast<const uint4*>(row + c);
-    r.v = __ldg(p);
-    if constexpr (sizeof(T) == 4) r.w = __ldg(p + 1);
-    return r;
-  }
-  float v[8];
+  Raw8<T> r;
+  if constexpr (VEC) {
+    r.v = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (sizeof(T) == 4) r.w = r.v;
+    if (c < cols) {
+      const uint4* p = reinterpret_cast<const uint4*>(row + c);
+      r.v = __ldg(p);
+      if constexpr (sizeof(T) == 4) r.w = __ldg(p + 1);
+    }
+  } else {
+    float v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f32(row[(c + i) * stride_c]) : 0.f;
-  return pack8<T>(v);
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f32(row[(c + i) * stride_c]) : 0.f;
+    r = pack8<T>(v);
+  }
+  return r;
 }
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* row, int64_t stride_c, int64_t c, int64_t cols, const Raw8<T>& r) {
-  if (VEC && c + 8 <= cols) {
-    uint4* p = reinterpret_cast<uint4*>(row + c);
-    p[0] = r.v;
-    if constexpr (sizeof(T) == 4) p[1] = r.w;
-    return;
-  }
-  float v[8];
-  unpack8(r, v);
+  if constexpr (VEC) {
+    if (c < cols) {
+      uint4* p = reinterpret_cast<uint4*>(row + c);
+      p[0] = r.v;
+      if constexpr (sizeof(T) == 4) p[1] = r.w;
+    }
+  } else {
+    float v[8];
+    unpack8(r, v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (c + i < cols) row[(c + i) * stride_c] = from_f32<T>(v[i]);
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) row[(c + i) * stride_c] = from_f32<T>(v[i]);
+  }
 }
 
 // The byte of a block's power-of-two scale: with amax = m * 2^e, the smallest exponent at which amax is at most the

@@ -17,6 +17,8 @@ constexpr int kMaxThreads = 512;  // per row, and per block where that is more t
 // Blocks of kMaxThreads an SM holds at once, by rounds held in registers.
 constexpr int blocks_per_sm(int rounds) { return rounds <= 2 ? 2 : 1; }
 
+constexpr int backward_blocks_per_sm(int rounds) { return rounds == 1 ? 2 : 1; }
+
 // Sum over the `tpr` threads of each row of the block (tpr a multiple of 32; rows of a block are consecutive groups of
 // warps), the same bits in every thread: warps by shuffles, then the row's warps in order through `part` (one float2
 // per warp). `buf` alternates so that one barrier per call is enough.
@@ -39,66 +41,61 @@ __device__ __forceinline__ float2 row_sum(float2 v, int tpr, float2 (*part)[32],
 }
 
 // FMT_NONE writes values (y), the formats write q; rows from `rows` to the end of their 128-row scale tile get zero
-// scales. RES: h = x + residual, else h = x.
+// scales. RES: h = x + residual, else h = x. Columns fit 31 bits.
 template <typename T, int FMT, bool RES, bool VEC, int ROUNDS>
 __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
     norm_kernel(Mat x, Mat res, const T* w, T* h, int64_t shr, int64_t shc, T* y, int64_t syr, int64_t syc, Quant q,
-                int64_t rows, int64_t cols, float eps, int tpr) {
+                int64_t rows, int cols, float eps, int tpr) {
   __shared__ float2 part[2][32];
   const int t = threadIdx.x % tpr;
   const int64_t row = blockIdx.x * static_cast<int64_t>(blockDim.x / tpr) + threadIdx.x / tpr;
   const bool live = row < rows;
-  const int64_t width = tpr * 8;
+  const int width = tpr * 8;
+  if (FMT != FMT_NONE && blockIdx.x * static_cast<int64_t>(blockDim.x / tpr) >= rows) {  // a block without rows
+    for (int64_t kt = t; kt < q.ktiles; kt += tpr)
+      *reinterpret_cast<uint32_t*>(q.scales + scale_row(row, q.ktiles) + kt * 512) = 0u;
+    return;
+  }
   const T* xr = static_cast<const T*>(x.p) + row * x.sr;
   const T* rr = RES ? static_cast<const T*>(res.p) + row * res.sr : nullptr;
-  const int64_t lim = live ? cols : 0;
+  T* hr = h + row * shr;
+  const int lim = live ? cols : 0;
   const float ts = FMT == FMT_NVFP4 ? *q.scale : 0.f;
 
-  auto sum8 = [&](const Raw8<T>& a, const Raw8<T>& b, float(&v)[8]) {
+  float2 s = make_float2(0.f, 0.f);
+  // v = the row's values from their loads; stores h and adds up the squares
+  auto take = [&](const Raw8<T>& a, const Raw8<T>& b, int c, float(&v)[8]) {
     unpack8(a, v);
     if (RES) {
       float f[8];
       unpack8(b, f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += f[i];
+      if (h) store8<T, VEC>(hr, shc, c, lim, pack8<T>(v));
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s.x = fmaf(v[i], v[i], s.x);
   };
-
   float v[ROUNDS][8];
-  float2 s = make_float2(0.f, 0.f);
   {
     Raw8<T> a[ROUNDS], b[ROUNDS];
 #pragma unroll
     for (int k = 0; k < ROUNDS; ++k) {
-      const int64_t c = k * width + t * 8;
-      if (k * width < cols) {
-        a[k] = load8<T, VEC>(xr, x.sc, c, lim);
-        if (RES) b[k] = load8<T, VEC>(rr, res.sc, c, lim);
-      }
+      const int c = k * width + t * 8;
+      a[k] = load8<T, VEC>(xr, x.sc, c, lim);
+      if (RES) b[k] = load8<T, VEC>(rr, res.sc, c, lim);
     }
 #pragma unroll
-    for (int k = 0; k < ROUNDS; ++k) {
-      const int64_t c = k * width + t * 8;
-      if (k * width < cols) {
-        sum8(a[k], b[k], v[k]);
-        if (RES && h && c < lim) store8<T, VEC>(h + row * shr, shc, c, lim, pack8<T>(v[k]));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s.x = fmaf(v[k][i], v[k][i], s.x);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
-      }
-    }
+    for (int k = 0; k < ROUNDS; ++k) take(a[k], b[k], k * width + t * 8, v[k]);
   }
-  if constexpr (ROUNDS == kMostRounds) for (int64_t c0 = ROUNDS * width; c0 < cols; c0 += width) {
-    const int64_t c = c0 + t * 8;
-    Raw8<T> a = load8<T, VEC>(xr, x.sc, c, lim), b = a;
-    if (RES) b = load8<T, VEC>(rr, res.sc, c, lim);
-    float f[8];
-    sum8(a, b, f);
-    if (RES && h && c < lim) store8<T, VEC>(h + row * shr, shc, c, lim, pack8<T>(f));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s.x = fmaf(f[i], f[i], s.x);
+  if constexpr (ROUNDS == kMostRounds) {
+    for (int64_t c = ROUNDS * width + t * 8; c - t * 8 < cols; c += width) {
+      const Raw8<T> a = load8<T, VEC>(xr, x.sc, c, lim);
+      Raw8<T> b = a;
+      if (RES) b = load8<T, VEC>(rr, res.sc, c, lim);
+      float f[8];
+      take(a, b, static_cast<int>(c), f);
+    }
   }
   s = row_sum(s, tpr, part, 0);
   const float r = rsqrtf(s.x / static_cast<float>(cols) + eps);
@@ -115,7 +112,7 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
       for (int i = 0; i < 8; ++i) f[i] = 0.f;
     }
     if constexpr (FMT == FMT_NONE) {
-      if (c < lim) store8<T, VEC>(y + row * syr, syc, c, lim, pack8<T>(f));
+      store8<T, VEC>(y + row * syr, syc, c, lim, pack8<T>(f));
     } else {
       quantize_store<FMT>(f, amax8(f), threadIdx.x & 31, c, live ? q.code_cols : 0, q.codes + row * q.pitch,
                           q.scales + scale_row(row, q.ktiles), q.ktiles, ts);
@@ -124,142 +121,201 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
 #pragma unroll
   for (int k = 0; k < ROUNDS; ++k)
     if (k * width < cover) finish(v[k], k * width + t * 8);
-  if constexpr (ROUNDS == kMostRounds) for (int64_t c0 = ROUNDS * width; c0 < cover; c0 += width) {
-    const int64_t c = c0 + t * 8;
-    Raw8<T> a = load8<T, VEC>(xr, x.sc, c, lim), b = a;
-    if (RES) b = load8<T, VEC>(rr, res.sc, c, lim);
-    float f[8];
-    sum8(a, b, f);
-    finish(f, c);
+  if constexpr (ROUNDS == kMostRounds) {
+    for (int64_t c = ROUNDS * width + t * 8; c - t * 8 < cover; c += width) {
+      float f[8];
+      unpack8(load8<T, VEC>(xr, x.sc, c, lim), f);
+      if (RES) {
+        float g[8];
+        unpack8(load8<T, VEC>(rr, res.sc, c, lim), g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] += g[i];
+      }
+      finish(f, c);
+    }
   }
 }
 
-// Gradient: a block walks rows blockIdx.x * rpb + k * gridDim.x * rpb, so its threads keep their columns and add up the
-// weight's gradient in registers (rounds past the fourth: in the block's own row of the workspace). Each group of tpr
-// threads leaves one fp32 row of partial sums in the workspace; norm_dweight_kernel adds them in a fixed order.
+// Gradient: a block walks rows, `rpb` groups of tpr threads a row each, so its threads keep their columns and add up the
+// weight's gradient in registers (rounds past the fourth: in the group's own row of the workspace, from column
+// ROUNDS * width on). At the end the block's groups add theirs up in shared memory, in order, and the block leaves one
+// fp32 row in the workspace; norm_dweight_kernel adds the rows in a fixed order. With one or two
+// rounds the weight stays in registers and a row's loads are one row ahead, in flight across the row sum's barrier; four
+// leave no room for either.
 template <typename T, bool DH, bool VEC, int ROUNDS>
-__global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
+__global__ void __launch_bounds__(kMaxThreads, backward_blocks_per_sm(ROUNDS))
     norm_backward_kernel(Mat dy, Mat h, const T* w, Mat dh, T* dx, int64_t sxr, int64_t sxc, float* partial,
-                         int64_t rows, int64_t cols, float eps, int tpr) {
+                         int64_t rows, int cols, float eps, int tpr) {
   __shared__ float2 part[2][32];
-  const int t = threadIdx.x % tpr;
+  extern __shared__ float sums[];  // [rpb][cols] where rpb > 1
+  constexpr bool kAhead = ROUNDS < kMostRounds;
+  const int t = threadIdx.x % tpr, g = threadIdx.x / tpr;
   const int rpb = blockDim.x / tpr;
-  const int64_t group = blockIdx.x * static_cast<int64_t>(rpb) + threadIdx.x / tpr;
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * rpb;
-  const int64_t width = tpr * 8;
-  float* mine = partial + group * cols;
-  float acc[ROUNDS][8];
+  const int width = tpr * 8;
+  const float n = static_cast<float>(cols);
+  float* mine = partial + blockIdx.x * static_cast<int64_t>(cols);
+  float acc[ROUNDS][8], wf[kAhead ? ROUNDS : 1][8];
+  auto weight = [&](int k, float(&wt)[8]) {
+    if constexpr (kAhead) {
 #pragma unroll
-  for (int k = 0; k < ROUNDS; ++k)
+      for (int i = 0; i < 8; ++i) wt[i] = wf[k][i];
+    } else {
+      unpack8(load8<T, VEC>(w, 1, k * width + t * 8, cols), wt);
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    if constexpr (kAhead) unpack8(load8<T, VEC>(w, 1, k * width + t * 8, cols), wf[k]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[k][i] = 0.f;
-  const int64_t trips = (rows + groups - 1) / groups;
-  int buf = 0;
-  for (int64_t trip = 0; trip < trips; ++trip) {
-    const int64_t row = trip * groups + group;
-    const int64_t lim = row < rows ? cols : 0;  // every thread of the block reaches the barrier
+  }
+  Raw8<T> a[ROUNDS], b[ROUNDS];
+  auto fetch = [&](int64_t row) {
+    const int lim = row < rows ? cols : 0;
     const T* dyr = static_cast<const T*>(dy.p) + row * dy.sr;
     const T* hr = static_cast<const T*>(h.p) + row * h.sr;
-    Raw8<T> a[ROUNDS], b[ROUNDS];
 #pragma unroll
     for (int k = 0; k < ROUNDS; ++k) {
-      const int64_t c = k * width + t * 8;
-      if (k * width < cols) {
-        a[k] = load8<T, VEC>(dyr, dy.sc, c, lim);
-        b[k] = load8<T, VEC>(hr, h.sc, c, lim);
-      }
+      const int c = k * width + t * 8;
+      a[k] = load8<T, VEC>(dyr, dy.sc, c, lim);
+      b[k] = load8<T, VEC>(hr, h.sc, c, lim);
     }
+  };
+  // dx, and the weight's terms into `sum`
+  auto finish = [&](const float(&d)[8], const float(&v)[8], const float(&wt)[8], int64_t row, int64_t c, int lim, float r,
+                    float rm, float(&sum)[8]) {
+    float o[8], e[8];
+    if (DH) unpack8(load8<T, VEC>(static_cast<const T*>(dh.p) + row * dh.sr, dh.sc, c, lim), e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      o[i] = fmaf(v[i], -rm, d[i] * wt[i] * r);
+      if (DH) o[i] += e[i];
+      sum[i] = fmaf(d[i] * v[i], r, sum[i]);
+    }
+    store8<T, VEC>(dx + row * sxr, sxc, c, lim, pack8<T>(o));
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * rpb;
+  const int64_t trips = (rows - static_cast<int64_t>(blockIdx.x) * rpb + step - 1) / step;  // the block's; at least one
+  int64_t row = blockIdx.x * static_cast<int64_t>(rpb) + g;
+  int buf = 0;
+  if (kAhead) fetch(row);
+  for (int64_t trip = 0; trip < trips; ++trip, row += step) {
+    const int lim = row < rows ? cols : 0;  // every thread of the block reaches the barrier
     float2 s = make_float2(0.f, 0.f);
-    auto add = [&](const Raw8<T>& ra, const Raw8<T>& rb, int64_t c) {
-      float d[8], v[8], g[8];
-      unpack8(ra, d);
-      unpack8(rb, v);
-      unpack8(load8<T, VEC>(w, 1, c, cols), g);
+    auto add = [&](const float(&d)[8], const float(&v)[8], const float(&wt)[8]) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         s.x = fmaf(v[i], v[i], s.x);
-        s.y = fmaf(d[i] * g[i], v[i], s.y);
+        s.y = fmaf(d[i] * wt[i], v[i], s.y);
       }
     };
+    if (!kAhead) fetch(row);
+    Raw8<T> ca[ROUNDS], cb[ROUNDS];
 #pragma unroll
-    for (int k = 0; k < ROUNDS; ++k)
-      if (k * width < cols) add(a[k], b[k], k * width + t * 8);
-    if constexpr (ROUNDS == kMostRounds) for (int64_t c0 = ROUNDS * width; c0 < cols; c0 += width) {
-      const int64_t c = c0 + t * 8;
-      add(load8<T, VEC>(dyr, dy.sc, c, lim), load8<T, VEC>(hr, h.sc, c, lim), c);
+    for (int k = 0; k < ROUNDS; ++k) {
+      ca[k] = a[k];
+      cb[k] = b[k];
+      float d[8], v[8], wt[8];
+      unpack8(ca[k], d);
+      unpack8(cb[k], v);
+      weight(k, wt);
+      add(d, v, wt);
     }
+    const T* dyr = static_cast<const T*>(dy.p) + row * dy.sr;
+    const T* hr = static_cast<const T*>(h.p) + row * h.sr;
+    if constexpr (ROUNDS == kMostRounds) {
+      for (int64_t c = ROUNDS * width + t * 8; c - t * 8 < cols; c += width) {
+        float d[8], v[8], wt[8];
+        unpack8(load8<T, VEC>(dyr, dy.sc, c, lim), d);
+        unpack8(load8<T, VEC>(hr, h.sc, c, lim), v);
+        unpack8(load8<T, VEC>(w, 1, c, cols), wt);
+        add(d, v, wt);
+      }
+    }
+    if (kAhead && trip + 1 < trips) fetch(row + step);
     s = row_sum(s, tpr, part, buf);
     buf ^= 1;
-    const float n = static_cast<float>(cols);
     const float r = rsqrtf(s.x / n + eps);
-    const float m = r * r * (s.y / n);  // dx = r * (dy * w - h * m)
-    auto finish = [&](const Raw8<T>& ra, const Raw8<T>& rb, int64_t c, float(&sum)[8]) {
-      float d[8], v[8], g[8], e[8], o[8];
-      unpack8(ra, d);
-      unpack8(rb, v);
-      unpack8(load8<T, VEC>(w, 1, c, cols), g);
-      if (DH) unpack8(load8<T, VEC>(static_cast<const T*>(dh.p) + row * dh.sr, dh.sc, c, lim), e);
+    const float rm = r * r * r * (s.y / n);  // dx = r * dy * w - h * rm
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        o[i] = r * (d[i] * g[i] - v[i] * m);
-        if (DH) o[i] += e[i];
-        sum[i] = fmaf(d[i] * r, v[i], sum[i]);
+    for (int k = 0; k < ROUNDS; ++k) {
+      const int c = k * width + t * 8;
+      if (c < lim) {
+        float d[8], v[8], wt[8];
+        unpack8(ca[k], d);
+        unpack8(cb[k], v);
+        weight(k, wt);
+        finish(d, v, wt, row, c, lim, r, rm, acc[k]);
       }
-      if (c < lim) store8<T, VEC>(dx + row * sxr, sxc, c, lim, pack8<T>(o));
-    };
+    }
+    if constexpr (ROUNDS == kMostRounds) {  // such rows are long: one group a block, whose columns are this thread's own
+      for (int64_t c = ROUNDS * width + t * 8; c < lim; c += width) {
+        float d[8], v[8], wt[8], sum[8];
+        unpack8(load8<T, VEC>(dyr, dy.sc, c, lim), d);
+        unpack8(load8<T, VEC>(hr, h.sc, c, lim), v);
+        unpack8(load8<T, VEC>(w, 1, c, cols), wt);
 #pragma unroll
-    for (int k = 0; k < ROUNDS; ++k)
-      if (k * width < cols && lim) finish(a[k], b[k], k * width + t * 8, acc[k]);
-    if constexpr (ROUNDS == kMostRounds) for (int64_t c0 = ROUNDS * width; c0 < cols && lim; c0 += width) {
-      const int64_t c = c0 + t * 8;
-      float sum[8];
+        for (int i = 0; i < 8; ++i) sum[i] = trip > 0 && c + i < cols ? mine[c + i] : 0.f;
+        finish(d, v, wt, row, c, lim, r, rm, sum);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] = trip > 0 && c + i < cols ? mine[c + i] : 0.f;
-      finish(load8<T, VEC>(dyr, dy.sc, c, lim), load8<T, VEC>(hr, h.sc, c, lim), c, sum);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < cols) mine[c + i] = sum[i];
+        for (int i = 0; i < 8; ++i)
+          if (c + i < cols) mine[c + i] = sum[i];
+      }
     }
   }
-  if (group >= rows)  // a group without rows: its sums are zero
-    for (int64_t c = ROUNDS * width + t; c < cols; c += tpr) mine[c] = 0.f;
+  if (rpb > 1) {
 #pragma unroll
-  for (int k = 0; k < ROUNDS; ++k) {
-    const int64_t c = k * width + t * 8;
-    if (c + 8 <= cols && cols % 4 == 0) {
-      reinterpret_cast<float4*>(mine + c)[0] = make_float4(acc[k][0], acc[k][1], acc[k][2], acc[k][3]);
-      reinterpret_cast<float4*>(mine + c)[1] = make_float4(acc[k][4], acc[k][5], acc[k][6], acc[k][7]);
-    } else {
+    for (int k = 0; k < ROUNDS; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (c + i < cols) mine[c + i] = acc[k][i];
+        if (k * width + t * 8 + i < cols) sums[g * cols + k * width + t * 8 + i] = acc[k][i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+      float f = sums[c];
+      for (int i = 1; i < rpb; ++i) f += sums[i * cols + c];
+      mine[c] = f;
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    const int c = k * width + t * 8;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      if (c + i + 4 <= cols && cols % 4 == 0) {
+        *reinterpret_cast<float4*>(mine + c + i) = make_float4(acc[k][i], acc[k][i + 1], acc[k][i + 2], acc[k][i + 3]);
+      } else {
+#pragma unroll
+        for (int j = i; j < i + 4; ++j)
+          if (c + j < cols) mine[c + j] = acc[k][j];
+      }
     }
   }
 }
 
-// dweight[c] = sum over the groups' partial rows, in order within each of 8 strands, then the strands in order.
+// dweight[c] = sum over the blocks' partial rows: 32 strands, each its rows in order, then the strands in order.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_dweight_kernel(const float* partial, int64_t groups, int64_t cols, T* dw) {
-  __shared__ float part[8][33];
+__global__ void __launch_bounds__(1024) norm_dweight_kernel(const float* partial, int groups, int64_t cols, T* dw) {
+  __shared__ float part[32][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t c = blockIdx.x * int64_t(32) + x;
   float s = 0.f;
   if (c < cols) {
-    int64_t g = y;
-    for (; g + 24 < groups; g += 32) {
+    int g = y;
+    for (; g + 96 < groups; g += 128) {
       float f[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) f[u] = partial[(g + 8 * u) * cols + c];
+      for (int u = 0; u < 4; ++u) f[u] = partial[static_cast<int64_t>(g + 32 * u) * cols + c];
 #pragma unroll
       for (int u = 0; u < 4; ++u) s += f[u];
     }
-    for (; g < groups; g += 8) s += partial[g * cols + c];
+    for (; g < groups; g += 32) s += partial[static_cast<int64_t>(g) * cols + c];
   }
   part[y][x] = s;
   __syncthreads();
   if (y == 0 && c < cols) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += part[i][x];
+    for (int i = 1; i < 32; ++i) s += part[i][x];
     dw[c] = from_f32<T>(s);
   }
 }
@@ -293,17 +349,18 @@ Split forward_split(int64_t rows, int64_t cols) {
   return s;
 }
 
-// The gradient's blocks stay for many rows: as many as the GPU holds at once, fewer where there are fewer rows.
+// The gradient's blocks stay for many rows: as many as the GPU holds at once, fewer where there are fewer rows. Blocks of
+// kMaxThreads, several rows at a time where rows are short.
 Split backward_split(int64_t rows, int64_t cols) {
   Split s;
   s.tpr = pow2_threads(ceil_div(cols, 8), kMaxThreads);
-  s.threads = s.tpr < 128 ? 128 : s.tpr;
+  s.threads = kMaxThreads;
+  while (s.threads > s.tpr && s.threads > 128 && (s.threads / s.tpr) / 2 >= rows) s.threads /= 2;
   s.rounds = rounds_of(cols, s.tpr);
-  const int rpb = s.threads / s.tpr;
-  const int64_t most = 148 * blocks_per_sm(s.rounds) * (kMaxThreads / s.threads);
-  s.blocks = ceil_div(rows, rpb);
+  const int64_t most = 148 * backward_blocks_per_sm(s.rounds);
+  s.blocks = ceil_div(rows, s.threads / s.tpr);
   if (s.blocks > most) s.blocks = most;
-  s.groups = s.blocks * rpb;
+  s.groups = s.blocks;
   return s;
 }
 
@@ -336,8 +393,8 @@ int32_t b2g_micro_rms_norm(const b2g_micro_matrix* x, const b2g_micro_matrix* re
     if (!weight) return record_error(B2G_ERR_INVALID_ARG, "null weight");
     const Split s = forward_split(q ? ceil_div(rows, 128) * 128 : rows, cols);
     if (s.blocks > kMaxGrid) return too_large("rms_norm");
-    const bool vec = vec_ok(x, rows, 2) && (!residual || vec_ok(residual, rows, 2)) && (!h || vec_ok(h, rows, 2)) &&
-                     (!y || vec_ok(y, rows, 2)) && aligned16(weight);
+    const bool vec = vec_ok(x, rows, cols, 2) && (!residual || vec_ok(residual, rows, cols, 2)) &&
+                     (!h || vec_ok(h, rows, cols, 2)) && (!y || vec_ok(y, rows, cols, 2)) && aligned16(weight);
     return by_type(dtype, [&](auto t) -> int32_t {
       using T = decltype(t);
       if constexpr (sizeof(T) == 4) {
@@ -348,7 +405,7 @@ int32_t b2g_micro_rms_norm(const b2g_micro_matrix* x, const b2g_micro_matrix* re
           kernel<<<static_cast<unsigned>(s.blocks), s.threads, 0, static_cast<cudaStream_t>(stream)>>>(
               mat(x), residual ? mat(residual) : none, static_cast<const T*>(weight), h ? static_cast<T*>(h->ptr) : nullptr,
               h ? h->stride_r : 0, h ? h->stride_c : 1, y ? static_cast<T*>(y->ptr) : nullptr, y ? y->stride_r : 0,
-              y ? y->stride_c : 1, q ? quant(q) : Quant{}, rows, cols, eps, s.tpr);
+              y ? y->stride_c : 1, q ? quant(q) : Quant{}, rows, static_cast<int>(cols), eps, s.tpr);
           return launched("rms_norm launch");
         };
         const auto pick = [&](auto f) -> int32_t {
@@ -400,8 +457,8 @@ int32_t b2g_micro_rms_norm_backward(const b2g_micro_matrix* dy, const b2g_micro_
       return record_error(B2G_ERR_WORKSPACE, "rms_norm_backward: workspace missing, misaligned or too small");
     const int64_t wgrid = ceil_div(cols, 32);
     if (wgrid > kMaxGrid) return too_large("rms_norm_backward");
-    const bool vec = vec_ok(dy, rows, 2) && vec_ok(h, rows, 2) && vec_ok(dx, rows, 2) && (!dh || vec_ok(dh, rows, 2)) &&
-                     aligned16(weight);
+    const bool vec = vec_ok(dy, rows, cols, 2) && vec_ok(h, rows, cols, 2) && vec_ok(dx, rows, cols, 2) &&
+                     (!dh || vec_ok(dh, rows, cols, 2)) && aligned16(weight);
     return by_type(dtype, [&](auto t) -> int32_t {
       using T = decltype(t);
       if constexpr (sizeof(T) == 4) {
@@ -409,9 +466,10 @@ int32_t b2g_micro_rms_norm_backward(const b2g_micro_matrix* dy, const b2g_micro_
       } else {
         const Mat none{nullptr, 0, 1};
         const auto go = [&](auto kernel) {
-          kernel<<<static_cast<unsigned>(s.blocks), s.threads, 0, st>>>(
+          const size_t smem = s.threads > s.tpr ? size_t(s.threads / s.tpr) * cols * sizeof(float) : 0;
+          kernel<<<static_cast<unsigned>(s.blocks), s.threads, smem, st>>>(
               mat(dy), mat(h), static_cast<const T*>(weight), dh ? mat(dh) : none, static_cast<T*>(dx->ptr), dx->stride_r,
-              dx->stride_c, static_cast<float*>(workspace), rows, cols, eps, s.tpr);
+              dx->stride_c, static_cast<float*>(workspace), rows, static_cast<int>(cols), eps, s.tpr);
           return launched("rms_norm_backward launch");
         };
         const int32_t rc = by_flag(dh, [&](auto f) {
@@ -421,7 +479,8 @@ int32_t b2g_micro_rms_norm_backward(const b2g_micro_matrix* dy, const b2g_micro_
                                : s.rounds == 2 ? go(norm_backward_kernel<T, D, true, 2>) : go(norm_backward_kernel<T, D, true, kMostRounds>);
         });
         if (rc) return rc;
-        norm_dweight_kernel<T><<<static_cast<unsigned>(wgrid), 256, 0, st>>>(static_cast<const float*>(workspace), s.groups, cols,
+        norm_dweight_kernel<T><<<static_cast<unsigned>(wgrid), 1024, 0, st>>>(static_cast<const float*>(workspace),
+                                                                           static_cast<int>(s.groups), cols,
                                                                            static_cast<T*>(dweight));
         return launched("rms_norm_backward reduce launch");
       }

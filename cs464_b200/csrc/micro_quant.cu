@@ -99,6 +99,16 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int64_t rj = task / col_chunks;
   const int64_t c = (task - rj * col_chunks) * 256 + lane * 8;
   const int64_t row0 = (rj >> 5) * 128 + (rj & 31);
+  const bool leads = (lane & (block_of(FMT) / 2 - 1)) == 0;  // of the lanes that share a scale word
+  const int64_t kt = c / (4 * block_of(FMT));
+  auto no_row = [&](int64_t row) {  // a row past the last: zero scales and no codes
+    if (leads && kt < q.ktiles) *reinterpret_cast<uint32_t*>(q.scales + scale_row(row, q.ktiles) + kt * 512) = 0u;
+  };
+  if (row0 >= rows) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) no_row(row0 + 32 * i);
+    return;
+  }
   const float ts = FMT == FMT_NVFP4 ? *q.scale : 0.f;
   using S = SRC<T>;
   Raw8<T> r[4][S::kLoads];
@@ -114,11 +124,13 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t row = row0 + 32 * i;
+    if (row >= rows) {
+      no_row(row);
+      continue;
+    }
     float v[8];
     const uint32_t m = S::value(r[i], v);
-    // rows past the last get zero scales and no codes
-    quantize_store<FMT>(v, m, lane, c, row < rows ? q.code_cols : 0, q.codes + row * q.pitch,
-                        q.scales + scale_row(row, q.ktiles), q.ktiles, ts);
+    quantize_store<FMT>(v, m, lane, c, q.code_cols, q.codes + row * q.pitch, q.scales + scale_row(row, q.ktiles), q.ktiles, ts);
   }
 }
 
@@ -387,7 +399,7 @@ int32_t run_quantize(const b2g_micro_matrix* x, const b2g_micro_tensor* t, cudaS
       return launched("quantize launch");
     }
   }
-  if (vec_ok(x, t->rows, sizeof(T))) return run_rows<T, FMT, true, ValueSource>(m, t->rows, t->cols, q, st);
+  if (vec_ok(x, t->rows, t->cols, sizeof(T))) return run_rows<T, FMT, true, ValueSource>(m, t->rows, t->cols, q, st);
   return run_rows<T, FMT, false, ValueSource>(m, t->rows, t->cols, q, st);
 }
 
@@ -437,7 +449,7 @@ int32_t b2g_micro_tensor_scale(const b2g_micro_matrix* x, int64_t rows, int64_t 
       const int64_t want = ceil_div(r * chunks, kWarps * 32 * 4);
       const unsigned grid = static_cast<unsigned>(want < 1 ? 1 : want > 148 * 8 ? 148 * 8 : want);
       const int64_t step = static_cast<int64_t>(grid) * kWarps * 32;
-      if (vec_ok(&view, r, sizeof(T)))
+      if (vec_ok(&view, r, c, sizeof(T)))
         tensor_scale_kernel<T, true><<<grid, kWarps * 32, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
       else
         tensor_scale_kernel<T, false><<<grid, kWarps * 32, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
@@ -479,7 +491,7 @@ int32_t b2g_micro_dequantize(const b2g_micro_tensor* q, const b2g_micro_matrix* 
               q->cols, ceil_div(q->cols, 4 * block_of(F)), static_cast<T*>(out->ptr), out->stride_r, out->stride_c,
               col_chunks, tasks);
         };
-        if (vec_ok(out, q->rows, sizeof(T))) go(dequantize_kernel<T, F, true>);
+        if (vec_ok(out, q->rows, q->cols, sizeof(T))) go(dequantize_kernel<T, F, true>);
         else go(dequantize_kernel<T, F, false>);
         return launched("dequantize launch");
       });
@@ -504,7 +516,7 @@ int32_t b2g_micro_silu_mul(const b2g_micro_matrix* gate_up, const b2g_micro_matr
       if constexpr (sizeof(T) == 4) {
         return B2G_ERR_INVALID_ARG;
       } else {
-        const bool vec = vec_ok(gate_up, rows, 2) && cols % 8 == 0;  // the up half starts `cols` values into the row
+        const bool vec = vec_ok(gate_up, rows, cols, 2);  // the up half starts `cols` values into the row
         if (q) {
           return by_format(q->format, [&](auto f) {
             constexpr int F = decltype(f)::value;
@@ -516,7 +528,7 @@ int32_t b2g_micro_silu_mul(const b2g_micro_matrix* gate_up, const b2g_micro_matr
         const RowBlocks rb = row_blocks(rows, cols);
     const int64_t grid = rb.grid;
         if (grid > kMaxGrid) return too_large("silu_mul");
-        if (vec && vec_ok(y, rows, 2))
+        if (vec && vec_ok(y, rows, cols, 2))
           gate_kernel<T, true><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols, rb.along);
         else
           gate_kernel<T, false><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols, rb.along);
@@ -546,7 +558,7 @@ int32_t b2g_micro_silu_mul_backward(const b2g_micro_matrix* dy, const b2g_micro_
       } else {
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         T* out = static_cast<T*>(dgate_up->ptr);
-        if (vec_ok(dy, rows, 2) && vec_ok(gate_up, rows, 2) && vec_ok(dgate_up, rows, 2) && cols % 8 == 0)
+        if (vec_ok(dy, rows, cols, 2) && vec_ok(gate_up, rows, cols, 2) && vec_ok(dgate_up, rows, cols, 2))
           gate_backward_kernel<T, true><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(dy), mat(gate_up), out, dgate_up->stride_r, dgate_up->stride_c, rows, cols, rb.along);
         else
           gate_backward_kernel<T, false><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(dy), mat(gate_up), out, dgate_up->stride_r, dgate_up->stride_c, rows, cols, rb.along);
