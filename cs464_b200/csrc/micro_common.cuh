@@ -312,24 +312,41 @@ __device__ __forceinline__ uint32_t amax8(const Raw8<float>& r) {
 //   processor", 1990). The residual is taken negated, so that zeros keep the value's sign. A block whose scale rounds to
 //   zero is zero.
 // The codes of a NaN block are cleared by `keep`.
+// NVFP4's tensor scale g as a thread uses it: 6 g and its reciprocal, once, so that a block's scale amax / (6 g) is three
+// operations of the same kind. (Below 2^-60 the residual would leave fp32's range: the division is done as such.)
+struct TensorScale {
+  float g, six, inv;
+  __device__ __forceinline__ explicit TensorScale(float scale) : g(scale), six(6.f * scale), inv(1.f / (6.f * scale)) {}
+  __device__ __forceinline__ float block(float amax) const {
+    if (g < 8.67361738e-19f) return amax / six;
+    const float q = amax * inv;
+    return fmaf(-fmaf(q, six, -amax), inv, q);
+  }
+};
+
 template <int FMT>
 struct BlockQuant {
   uint32_t byte;
   uint32_t keep;  // all ones; 0 in a NaN block
   float mul;      // MX: 2^-e; NVFP4: 1 / u, or 0
   float unit;     // NVFP4: u
-  __device__ __forceinline__ void init(uint32_t amax_bits, float tensor_scale) {
+  __device__ __forceinline__ void init(uint32_t amax_bits, const TensorScale& ts) {
     const bool bad = amax_bits >= 0x7f800000u;
     keep = bad ? 0u : 0xffffffffu;
     if constexpr (FMT == FMT_NVFP4) {
-      const float s = __fdiv_rn(__uint_as_float(amax_bits), 6.f * tensor_scale);
-      byte = bad ? 0x7fu : __nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3);
-      unit = e4m3_to_f32(byte) * tensor_scale;
-      mul = byte == 0u ? 0.f : __frcp_rn(unit);
+      byte = bad ? 0x7fu : __nv_cvt_float_to_fp8(ts.block(__uint_as_float(amax_bits)), __NV_SATFINITE, __NV_E4M3);
+      unit = e4m3_to_f32(byte) * ts.g;
+      mul = byte == 0u ? 0.f : reciprocal(unit);
     } else {
       byte = mx_scale_byte<FMT>(amax_bits);
       mul = __uint_as_float((254u - byte) << 23);
     }
+  }
+  // 1 / u, the hardware's estimate corrected by its residual (Markstein, as above).
+  __device__ __forceinline__ static float reciprocal(float u) {
+    float y;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(u));
+    return fmaf(-fmaf(u, y, -1.f), y, y);
   }
   __device__ __forceinline__ float scaled(float x) const {
     if constexpr (FMT == FMT_NVFP4) {
@@ -379,12 +396,12 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], const BlockQuant<FM
 // 4-byte store. Called by a converged warp.
 template <int FMT>
 __device__ __forceinline__ void quantize_store(const float (&v)[8], uint32_t m, int lane, int64_t c, int64_t code_cols,
-                                               uint8_t* code_row, uint8_t* scale_row0, int64_t ktiles, float tensor_scale) {
+                                               uint8_t* code_row, uint8_t* scale_row0, int64_t ktiles, const TensorScale& ts) {
   constexpr int kLanes = block_of(FMT) / 8;
 #pragma unroll
   for (int d = 1; d < kLanes; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
   BlockQuant<FMT> b;
-  b.init(m, tensor_scale);
+  b.init(m, ts);
   const uint2 q = codes8<FMT>(v, b);
   if (c < code_cols) {
     if constexpr (FMT == FMT_MXFP8) *reinterpret_cast<uint2*>(code_row + c) = q;

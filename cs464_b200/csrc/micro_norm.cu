@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
   const T* rr = RES ? static_cast<const T*>(res.p) + row * res.sr : nullptr;
   T* hr = h + row * shr;
   const int lim = live ? cols : 0;
-  const float ts = FMT == FMT_NVFP4 ? *q.scale : 0.f;
+  const TensorScale ts(FMT == FMT_NVFP4 ? *q.scale : 1.f);
 
   float2 s = make_float2(0.f, 0.f);
   // v = the row's values from their loads; stores h and adds up the squares
@@ -349,15 +349,14 @@ Split forward_split(int64_t rows, int64_t cols) {
   return s;
 }
 
-// The gradient's blocks stay for many rows: as many as the GPU holds at once, fewer where there are fewer rows. Blocks of
-// kMaxThreads, several rows at a time where rows are short.
+// The gradient's blocks stay for many rows: as many as the GPU holds at once, fewer where there are fewer rows. Two
+// rounds of eight columns a thread where there are that many; blocks of one row, or of 128 threads and several short rows.
 Split backward_split(int64_t rows, int64_t cols) {
   Split s;
-  s.tpr = pow2_threads(ceil_div(cols, 8), kMaxThreads);
-  s.threads = kMaxThreads;
-  while (s.threads > s.tpr && s.threads > 128 && (s.threads / s.tpr) / 2 >= rows) s.threads /= 2;
+  s.tpr = pow2_threads(ceil_div(ceil_div(cols, 8), 2), kMaxThreads);
+  s.threads = s.tpr < 128 ? 128 : s.tpr;
   s.rounds = rounds_of(cols, s.tpr);
-  const int64_t most = 148 * backward_blocks_per_sm(s.rounds);
+  const int64_t most = 148 * backward_blocks_per_sm(s.rounds) * (kMaxThreads / s.threads);
   s.blocks = ceil_div(rows, s.threads / s.tpr);
   if (s.blocks > most) s.blocks = most;
   s.groups = s.blocks;
