@@ -279,14 +279,21 @@ __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
 // them. The integer pipe is what bounds the quantising kernels, so 16-bit values are compared as they lie, two at a time
 // (magnitudes order as their bits do), and fp32 values by a maximum that takes the magnitude on the way, with a product
 // by zero on the otherwise idle multiply-add pipe to catch what is not finite.
-__device__ __forceinline__ uint32_t amax8(const Raw8<__nv_bfloat16>& r) {
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
+__device__ __forceinline__ uint32_t max_magnitudes(const uint4& w) {  // of the even and the odd ones
   const uint32_t k = 0x7fff7fffu;
-  const uint32_t m = __vmaxu2(__vmaxu2(r.v.x & k, r.v.y & k), __vmaxu2(r.v.z & k, r.v.w & k));
+  return max_u16x2(max_u16x2(w.x & k, w.y & k), max_u16x2(w.z & k, w.w & k));
+}
+__device__ __forceinline__ uint32_t amax8(const Raw8<__nv_bfloat16>& r) {
+  const uint32_t m = max_magnitudes(r.v);
   return max(m & 0xffff0000u, m << 16);
 }
 __device__ __forceinline__ uint32_t amax8(const Raw8<__half>& r) {
-  const uint32_t k = 0x7fff7fffu;
-  const uint32_t m = __vmaxu2(__vmaxu2(r.v.x & k, r.v.y & k), __vmaxu2(r.v.z & k, r.v.w & k));
+  const uint32_t m = max_magnitudes(r.v);
   return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(max(m >> 16, m & 0xffffu)))));
 }
 __device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
@@ -359,9 +366,14 @@ struct BlockQuant {
 };
 
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-  return lo | hi << 16;
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
 }
 
 // Eight e2m1 codes, the lowest value in the lowest bits: four conversions of two values to a byte and one packing move.
@@ -389,29 +401,43 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], const BlockQuant<FM
   else return make_uint2(e2m1x8(s) & b.keep, 0u);
 }
 
-// Quantise eight consecutive columns per lane, the warp's 32 lanes holding 256 consecutive columns from `col` (lane 0's
-// first, a multiple of 256 past the row's start), and store them: the codes of columns below `code_cols` (a multiple of
-// 32), and the scale words of tile columns below `ktiles`. `m`: the eight values' amax8. A block's lanes (4 for blocks of
-// 32, 2 for 16) share their largest magnitude by shuffles; the four scale bytes of one tile row are gathered into one
-// 4-byte store. Called by a converged warp.
+// Where a lane's eight columns of a row go: eight consecutive columns per lane, the warp's 32 lanes holding 256 of one row
+// (lane 0's first, a multiple of 256 past the row's start).
 template <int FMT>
-__device__ __forceinline__ void quantize_store(const float (&v)[8], uint32_t m, int lane, int64_t c, int64_t code_cols,
-                                               uint8_t* code_row, uint8_t* scale_row0, int64_t ktiles, const TensorScale& ts) {
+struct CodePlace {
+  uint8_t* codes;   // the lane's codes in the row
+  uint8_t* word;    // the scale word its block is in
+  bool has_codes;   // the columns exist in the codes (below code_cols)
+  bool leads;       // this lane stores the word, and the word exists
+  __device__ __forceinline__ CodePlace(const Quant& q, int64_t row, int64_t c, int lane) {
+    constexpr int kLanes = block_of(FMT) / 2;  // lanes that share a word: four blocks
+    const int64_t kt = c / (4 * block_of(FMT));
+    codes = q.codes + row * q.pitch + (FMT == FMT_MXFP8 ? c : c >> 1);
+    word = q.scales + scale_row(row, q.ktiles) + kt * 512;
+    has_codes = c < q.code_cols;
+    leads = (lane & (kLanes - 1)) == 0 && kt < q.ktiles;
+  }
+};
+
+// Quantise them. `m`: the eight values' amax8. A block's lanes (4 for blocks of 32, 2 for 16) share their largest magnitude
+// by shuffles; the four scale bytes of one tile row are gathered into one 4-byte store. Called by a converged warp.
+template <int FMT>
+__device__ __forceinline__ void quantize_store(const float (&v)[8], uint32_t m, int lane, const CodePlace<FMT>& to,
+                                               const TensorScale& ts) {
   constexpr int kLanes = block_of(FMT) / 8;
 #pragma unroll
   for (int d = 1; d < kLanes; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
   BlockQuant<FMT> b;
   b.init(m, ts);
   const uint2 q = codes8<FMT>(v, b);
-  if (c < code_cols) {
-    if constexpr (FMT == FMT_MXFP8) *reinterpret_cast<uint2*>(code_row + c) = q;
-    else *reinterpret_cast<uint32_t*>(code_row + (c >> 1)) = q.x;
+  if (to.has_codes) {
+    if constexpr (FMT == FMT_MXFP8) *reinterpret_cast<uint2*>(to.codes) = q;
+    else *reinterpret_cast<uint32_t*>(to.codes) = q.x;
   }
   uint32_t w = b.byte << (8 * ((lane / kLanes) & 3));
   w |= __shfl_xor_sync(0xffffffffu, w, kLanes);
   w |= __shfl_xor_sync(0xffffffffu, w, 2 * kLanes);
-  const int64_t kt = c / (4 * block_of(FMT));
-  if ((lane & (4 * kLanes - 1)) == 0 && kt < ktiles) *reinterpret_cast<uint32_t*>(scale_row0 + kt * 512) = w;
+  if (to.leads) *reinterpret_cast<uint32_t*>(to.word) = w;
 }
 
 }  // namespace micro

@@ -114,8 +114,9 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
     if constexpr (FMT == FMT_NONE) {
       store8<T, VEC>(y + row * syr, syc, c, lim, pack8<T>(f));
     } else {
-      quantize_store<FMT>(f, amax8(f), threadIdx.x & 31, c, live ? q.code_cols : 0, q.codes + row * q.pitch,
-                          q.scales + scale_row(row, q.ktiles), q.ktiles, ts);
+      CodePlace<FMT> to(q, row, c, threadIdx.x & 31);
+      to.has_codes = to.has_codes && live;
+      quantize_store<FMT>(f, amax8(f), threadIdx.x & 31, to, ts);
     }
   };
 #pragma unroll

@@ -103,38 +103,29 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int64_t rj = task / col_chunks;
   const int64_t c = (task - rj * col_chunks) * 256 + lane * 8;
   const int64_t row0 = (rj >> 5) * 128 + (rj & 31);
-  const bool leads = (lane & (block_of(FMT) / 2 - 1)) == 0;  // of the lanes that share a scale word
-  const int64_t kt = c / (4 * block_of(FMT));
-  auto no_row = [&](int64_t row) {  // a row past the last: zero scales and no codes
-    if (leads && kt < q.ktiles) *reinterpret_cast<uint32_t*>(q.scales + scale_row(row, q.ktiles) + kt * 512) = 0u;
-  };
-  if (row0 >= rows) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) no_row(row0 + 32 * i);
-    return;
-  }
-  const TensorScale ts(FMT == FMT_NVFP4 ? *q.scale : 1.f);
+  CodePlace<FMT> to(q, row0, c, lane);  // of the first row; row i is 32 i rows and 4 i scale bytes on
+  const int64_t code_step = 32 * q.pitch;
+  const int live = row0 >= rows ? 0 : static_cast<int>(min(static_cast<int64_t>(4), (rows - row0 + 31) / 32));
   using S = SRC<T>;
   Raw8<T> r[4][S::kLoads];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t row = row0 + 32 * i;
 #pragma unroll
-    for (int k = 0; k < S::kLoads; ++k) {
-      const T* p = static_cast<const T*>(x.p) + row * x.sr + k * cols * x.sc;
-      r[i][k] = load8<T, VEC>(p, x.sc, row < rows ? c : cols, cols);
-    }
+    for (int k = 0; k < S::kLoads; ++k)
+      r[i][k] = load8<T, VEC>(static_cast<const T*>(x.p) + (row0 + 32 * i) * x.sr + k * cols * x.sc, x.sc, c, i < live ? cols : 0);
   }
+  const TensorScale ts(FMT == FMT_NVFP4 ? *q.scale : 1.f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t row = row0 + 32 * i;
-    if (row >= rows) {
-      no_row(row);
-      continue;
+    if (i < live) {
+      float v[8];
+      const uint32_t m = S::value(r[i], v);
+      quantize_store<FMT>(v, m, lane, to, ts);
+    } else if (to.leads) {  // a row past the last: zero scales and no codes
+      *reinterpret_cast<uint32_t*>(to.word) = 0u;
     }
-    float v[8];
-    const uint32_t m = S::value(r[i], v);
-    quantize_store<FMT>(v, m, lane, c, q.code_cols, q.codes + row * q.pitch, q.scales + scale_row(row, q.ktiles), q.ktiles, ts);
+    to.codes += code_step;
+    to.word += 4;
   }
 }
 
