@@ -16,38 +16,59 @@ constexpr int64_t kOneBlock = 16384;  // chunks of eight values up to which one 
 // The smallest power of two 2^e >= 2^-100 with amax <= 2688 * 2^e (2688 = 6 * 448 = 1.3125 * 2^11). Every block takes
 // the maximum of its own candidate: the order does not matter. Infinities and NaN do not count. Up to kOneBlock chunks one
 // block does it alone (16x4096: two launches, one of them clearing the scale, and 6 us less).
-// A row's eight-column chunks are numbered across rows; a thread steps by the whole grid, four chunks in flight, and
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t a = __float_as_uint(v) & 0x7fffffffu;
+  return a >= 0x7f800000u ? 0u : a;
+}
+
+// amax8 of the finite ones
+template <typename T>
+__device__ __forceinline__ uint32_t finite_amax8(const Raw8<T>& r) {
+  const uint32_t a = amax8(r);
+  if (a < 0x7f800000u) return a;
+  float v[8];
+  unpack8(r, v);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, finite_bits(v[i]));
+  return m;
+}
+
+// FLAT: rows follow one another without a gap, and are one row of `chunks` chunks. Else a row's eight-column chunks are
+// numbered across rows; a thread steps by the whole grid, four chunks in flight, and
 // carries (row, chunk) along instead of dividing.
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool FLAT>
 __global__ void __launch_bounds__(1024)
     tensor_scale_kernel(Mat x, int64_t rows, int64_t cols, int64_t chunks, int64_t step_rows, int64_t step_chunks, float* scale) {
   const int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-  int64_t row = first / chunks, k = first - row * chunks;
+  int64_t row = FLAT ? 0 : first / chunks, k = FLAT ? first : first - row * chunks;
   const T* p = static_cast<const T*>(x.p);
   uint32_t m = 0;
-  while (row < rows) {
-    Raw8<T> r[4];
+  if constexpr (FLAT) {
+    constexpr int U = sizeof(T) == 4 ? 4 : 8;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    for (k = first; k < chunks; k += U * step) {
+      Raw8<T> r[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      r[u] = load8<T, VEC>(p + row * x.sr, x.sc, k * 8, row < rows ? cols : 0);
-      row += step_rows;
-      k += step_chunks;
-      if (k >= chunks) {
-        k -= chunks;
-        ++row;
-      }
+      for (int u = 0; u < U; ++u) r[u] = load8<T, true>(p, 1, (k + u * step) * 8, chunks * 8);
+#pragma unroll
+      for (int u = 0; u < U; ++u) m = max(m, finite_amax8(r[u]));
     }
+  } else {
+    while (row < rows) {
+      Raw8<T> r[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      uint32_t a = amax8(r[u]);
-      if (a >= 0x7f800000u) {  // something is not finite: take the others one by one
-        float v[8];
-        unpack8(r[u], v);
-        a = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a = max(a, isfinite(v[i]) ? __float_as_uint(fabsf(v[i])) : 0u);
+      for (int u = 0; u < 4; ++u) {
+        r[u] = load8<T, VEC>(p + row * x.sr, x.sc, k * 8, row < rows ? cols : 0);
+        row += step_rows;
+        k += step_chunks;
+        if (k >= chunks) {
+          k -= chunks;
+          ++row;
+        }
       }
-      m = max(m, a);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) m = max(m, finite_amax8(r[u]));
     }
   }
   m = __reduce_max_sync(0xffffffffu, m);
@@ -435,7 +456,11 @@ int32_t b2g_micro_tensor_scale(const b2g_micro_matrix* x, int64_t rows, int64_t 
         std::swap(r, c);
       }
       const b2g_micro_matrix view = {const_cast<void*>(m.p), m.sr, m.sc};
-      const int64_t chunks = c > 0 ? ceil_div(c, 8) : 1;
+      if (!rows || !cols) {  // no values: one flat row of no chunks, nothing is read
+        r = 1;
+        c = 0;
+      }
+      const int64_t chunks = ceil_div(c, 8);
       unsigned threads = 1024, grid = 1;
       if (r * chunks > kOneBlock) {
         const int64_t want = ceil_div(r * chunks, kWarps * 32 * 4);
@@ -448,10 +473,13 @@ int32_t b2g_micro_tensor_scale(const b2g_micro_matrix* x, int64_t rows, int64_t 
         }
       }
       const int64_t step = static_cast<int64_t>(grid) * threads;
-      if (vec_ok(&view, r, c, sizeof(T)))
-        tensor_scale_kernel<T, true><<<grid, threads, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
+      const bool vec = vec_ok(&view, r, c, sizeof(T));
+      if (vec && (r == 1 || m.sr == c))
+        tensor_scale_kernel<T, true, true><<<grid, threads, 0, st>>>(m, 1, r * c, r * chunks, 0, 0, scale);
+      else if (vec)
+        tensor_scale_kernel<T, true, false><<<grid, threads, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
       else
-        tensor_scale_kernel<T, false><<<grid, threads, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
+        tensor_scale_kernel<T, false, false><<<grid, threads, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
       return launched("tensor_scale launch");
     });
   });
