@@ -10,6 +10,7 @@
 #include <stdint.h>
 
 #include <cstdio>
+#include <algorithm>
 #include <exception>
 #include <type_traits>
 #include <utility>
@@ -79,9 +80,19 @@ struct Quant {  // where a microscaled tensor goes
   int64_t pitch, ktiles, code_cols;
 };
 
-// Whether rows of `cols` values of `m` can be read and written in whole 16-byte pieces of eight columns.
-inline bool vec_ok(const b2g_micro_matrix* m, int64_t rows, int64_t cols, int64_t size) {
-  return m->stride_c == 1 && cols % 8 == 0 && aligned16(m->ptr) && (rows <= 1 || (m->stride_r * size) % 16 == 0);
+// How rows of `cols` values of `m` can be moved (Mode).
+inline int mode_of(const b2g_micro_matrix* m, int64_t rows, int64_t cols, int64_t size) {
+  if (m->stride_c != 1) return 2;
+  return cols % 8 == 0 && aligned16(m->ptr) && (rows <= 1 || (m->stride_r * size) % 16 == 0) ? 0 : 1;
+}
+
+template <typename F>
+int32_t by_mode(int mode, F&& f) {
+  switch (mode) {
+    case 0: return f(std::integral_constant<int, 0>{});
+    case 1: return f(std::integral_constant<int, 1>{});
+    default: return f(std::integral_constant<int, 2>{});
+  }
 }
 
 inline Mat mat(const b2g_micro_matrix* m) { return Mat{m->ptr, m->stride_r, m->stride_c}; }
@@ -216,42 +227,104 @@ __device__ __forceinline__ Raw8<float> pack8<float>(const float (&v)[8]) {
                      make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]))};
 }
 
-// Columns c .. c+7 of a row that starts at `row`; columns at or past `cols` read as zero. VEC: unit column stride, 16-byte
-// aligned rows and `cols` a multiple of 8, so that eight columns exist or do not, and are one or two 16-byte loads.
-template <typename T, bool VEC>
-__device__ __forceinline__ Raw8<T> load8(const T* row, int64_t stride_c, int64_t c, int64_t cols) {
+// How a row's values lie. kVec: unit column stride, 16-byte aligned rows and a multiple of 8 columns, so that eight
+// columns exist or do not and are one or two 16-byte accesses. kUnit: unit column stride, any alignment and width: a warp
+// moves 32 consecutive values an instruction and shared memory turns them to eight a lane (through strided scalars an odd
+// width ran at a fifth of an even one's rate). kAny: any strides, a value at a time.
+enum Mode : int { kVec = 0, kUnit = 1, kAny = 2 };
+
+// A lane's eight columns c .. c+7 on their way from a row, columns at or past `cols` zero: `fetch` issues the loads,
+// `settle` gives the values. In kUnit both are called by a converged warp whose lanes hold 256 consecutive columns, with a
+// scratch of 256 values of the warp's own.
+template <typename T, int MODE>
+struct Frag {
   Raw8<T> r;
-  if constexpr (VEC) {
-    r.v = make_uint4(0u, 0u, 0u, 0u);
-    if constexpr (sizeof(T) == 4) r.w = r.v;
+};
+template <typename T>
+struct Frag<T, kUnit> {
+  T e[8];
+};
+
+template <typename T, int MODE>
+__device__ __forceinline__ Frag<T, MODE> fetch8(const T* row, int64_t stride_c, int64_t c, int64_t cols) {
+  Frag<T, MODE> f;
+  if constexpr (MODE == kVec) {
+    f.r.v = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (sizeof(T) == 4) f.r.w = f.r.v;
     if (c < cols) {
       const uint4* p = reinterpret_cast<const uint4*>(row + c);
-      r.v = __ldg(p);
-      if constexpr (sizeof(T) == 4) r.w = __ldg(p + 1);
+      f.r.v = __ldg(p);
+      if constexpr (sizeof(T) == 4) f.r.w = __ldg(p + 1);
     }
+  } else if constexpr (MODE == kUnit) {
+    const int lane = threadIdx.x & 31;
+    const int64_t first = c - 7 * lane;  // c0 + lane of the warp's first column c0
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.e[i] = first + 32 * i < cols ? row[first + 32 * i] : from_f32<T>(0.f);
   } else {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f32(row[(c + i) * stride_c]) : 0.f;
-    r = pack8<T>(v);
+    f.r = pack8<T>(v);
   }
-  return r;
+  return f;
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* row, int64_t stride_c, int64_t c, int64_t cols, const Raw8<T>& r) {
-  if constexpr (VEC) {
+template <typename T, int MODE>
+__device__ __forceinline__ Raw8<T> settle8(const Frag<T, MODE>& f, T* scratch) {
+  if constexpr (MODE == kUnit) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) scratch[32 * i + lane] = f.e[i];
+    __syncwarp();
+    const Raw8<T> r = reinterpret_cast<const Raw8<T>*>(scratch)[lane];
+    __syncwarp();
+    return r;
+  } else {
+    return f.r;
+  }
+}
+
+template <typename T, int MODE>
+__device__ __forceinline__ Raw8<T> load8(const T* row, int64_t stride_c, int64_t c, int64_t cols, T* scratch) {
+  return settle8<T, MODE>(fetch8<T, MODE>(row, stride_c, c, cols), scratch);
+}
+
+template <typename T, int MODE>
+__device__ __forceinline__ void store8(T* row, int64_t stride_c, int64_t c, int64_t cols, const Raw8<T>& r, T* scratch) {
+  if constexpr (MODE == kVec) {
     if (c < cols) {
       uint4* p = reinterpret_cast<uint4*>(row + c);
       p[0] = r.v;
       if constexpr (sizeof(T) == 4) p[1] = r.w;
     }
+  } else if constexpr (MODE == kUnit) {
+    const int lane = threadIdx.x & 31;
+    reinterpret_cast<Raw8<T>*>(scratch)[lane] = r;
+    __syncwarp();
+    const int64_t first = c - 7 * lane;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (first + 32 * i < cols) row[first + 32 * i] = scratch[32 * i + lane];
+    __syncwarp();
   } else {
     float v[8];
     unpack8(r, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (c + i < cols) row[(c + i) * stride_c] = from_f32<T>(v[i]);
+  }
+}
+
+// The calling warp's scratch for kUnit (WARPS warps a block).
+template <typename T, int MODE, int WARPS>
+__device__ __forceinline__ T* warp_scratch() {
+  if constexpr (MODE == kUnit) {
+    __shared__ __align__(16) unsigned char scratch[WARPS * 256 * sizeof(T)];
+    const int warp = (threadIdx.y * blockDim.x + threadIdx.x) >> 5;
+    return reinterpret_cast<T*>(scratch) + warp * 256;
+  } else {
+    return nullptr;
   }
 }
 

@@ -42,7 +42,7 @@ __device__ __forceinline__ float2 row_sum(float2 v, int tpr, float2 (*part)[32],
 
 // FMT_NONE writes values (y), the formats write q; rows from `rows` to the end of their 128-row scale tile get zero
 // scales. RES: h = x + residual, else h = x. Columns fit 31 bits.
-template <typename T, int FMT, bool RES, bool VEC, int ROUNDS>
+template <typename T, int FMT, bool RES, int MODE, int ROUNDS>
 __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
     norm_kernel(Mat x, Mat res, const T* w, T* h, int64_t shr, int64_t shc, T* y, int64_t syr, int64_t syc, Quant q,
                 int64_t rows, int cols, float eps, int tpr) {
@@ -61,6 +61,8 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
   T* hr = h + row * shr;
   const int lim = live ? cols : 0;
   const TensorScale ts(FMT == FMT_NVFP4 ? *q.scale : 1.f);
+  T* scratch = warp_scratch<T, MODE, kMaxThreads / 32>();
+  const int lane8 = (threadIdx.x & 31) * 8;  // a lane's columns past its warp's first
 
   float2 s = make_float2(0.f, 0.f);
   // v = the row's values from their loads; stores h and adds up the squares
@@ -71,28 +73,31 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
       unpack8(b, f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += f[i];
-      if (h) store8<T, VEC>(hr, shc, c, lim, pack8<T>(v));
+      if (h) store8<T, MODE>(hr, shc, c, lim, pack8<T>(v), scratch);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) s.x = fmaf(v[i], v[i], s.x);
   };
   float v[ROUNDS][8];
   {
-    Raw8<T> a[ROUNDS], b[ROUNDS];
+    Frag<T, MODE> a[ROUNDS], b[ROUNDS];
 #pragma unroll
     for (int k = 0; k < ROUNDS; ++k) {
       const int c = k * width + t * 8;
-      a[k] = load8<T, VEC>(xr, x.sc, c, lim);
-      if (RES) b[k] = load8<T, VEC>(rr, res.sc, c, lim);
+      a[k] = fetch8<T, MODE>(xr, x.sc, c, lim);
+      if (RES) b[k] = fetch8<T, MODE>(rr, res.sc, c, lim);
     }
 #pragma unroll
-    for (int k = 0; k < ROUNDS; ++k) take(a[k], b[k], k * width + t * 8, v[k]);
+    for (int k = 0; k < ROUNDS; ++k) {
+      const Raw8<T> ra = settle8<T, MODE>(a[k], scratch);
+      take(ra, RES ? settle8<T, MODE>(b[k], scratch) : ra, k * width + t * 8, v[k]);
+    }
   }
   if constexpr (ROUNDS == kMostRounds) {
     for (int64_t c = ROUNDS * width + t * 8; c - t * 8 < cols; c += width) {
-      const Raw8<T> a = load8<T, VEC>(xr, x.sc, c, lim);
+      const Raw8<T> a = load8<T, MODE>(xr, x.sc, c, lim, scratch);
       Raw8<T> b = a;
-      if (RES) b = load8<T, VEC>(rr, res.sc, c, lim);
+      if (RES) b = load8<T, MODE>(rr, res.sc, c, lim, scratch);
       float f[8];
       take(a, b, static_cast<int>(c), f);
     }
@@ -102,17 +107,18 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
 
   const int64_t cover = FMT == FMT_NONE ? cols : q.ktiles * 4 * block_of(FMT);  // whole scale tiles
   auto finish = [&](float(&f)[8], int64_t c) {
-    if (c < lim) {  // a chunk that ends past the row: its further values and weights were read as zero
+    // Past the row's end values and weights are read as zero; a warp wholly past it has zeros whatever the row's norm is.
+    if (c - lane8 < lim) {
       float g[8];
-      unpack8(load8<T, VEC>(w, 1, c, cols), g);
+      unpack8(load8<T, MODE>(w, 1, c, cols, scratch), g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = f[i] * r * g[i];
+      for (int i = 0; i < 8; ++i) f[i] = c < lim ? f[i] * r * g[i] : 0.f;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = 0.f;
     }
     if constexpr (FMT == FMT_NONE) {
-      store8<T, VEC>(y + row * syr, syc, c, lim, pack8<T>(f));
+      store8<T, MODE>(y + row * syr, syc, c, lim, pack8<T>(f), scratch);
     } else {
       CodePlace<FMT> to(q, row, c, threadIdx.x & 31);
       to.has_codes = to.has_codes && live;
@@ -125,10 +131,10 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
   if constexpr (ROUNDS == kMostRounds) {
     for (int64_t c = ROUNDS * width + t * 8; c - t * 8 < cover; c += width) {
       float f[8];
-      unpack8(load8<T, VEC>(xr, x.sc, c, lim), f);
+      unpack8(load8<T, MODE>(xr, x.sc, c, lim, scratch), f);
       if (RES) {
         float g[8];
-        unpack8(load8<T, VEC>(rr, res.sc, c, lim), g);
+        unpack8(load8<T, MODE>(rr, res.sc, c, lim, scratch), g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] += g[i];
       }
@@ -138,39 +144,37 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
 }
 
 // Gradient: a block walks rows, `rpb` groups of tpr threads a row each, so its threads keep their columns and add up the
-// weight's gradient in registers (rounds past the fourth: in the group's own row of the workspace, from column
+// weight's gradient in registers (rounds past the fourth: in the block's own row of the workspace, from column
 // ROUNDS * width on). At the end the block's groups add theirs up in shared memory, in order, and the block leaves one
-// fp32 row in the workspace; norm_dweight_kernel adds the rows in a fixed order. With one or two
-// rounds the weight stays in registers and a row's loads are one row ahead, in flight across the row sum's barrier; four
-// leave no room for either.
-template <typename T, bool DH, bool VEC, int ROUNDS>
+// fp32 row in the workspace; norm_dweight_kernel adds the rows in a fixed order. With one or two rounds of aligned rows the
+// weight stays in registers and a row's loads are one row ahead, in flight across the row sum's barrier; four leave no room
+// for either.
+template <typename T, bool DH, int MODE, int ROUNDS>
 __global__ void __launch_bounds__(kMaxThreads, backward_blocks_per_sm(ROUNDS))
     norm_backward_kernel(Mat dy, Mat h, const T* w, Mat dh, T* dx, int64_t sxr, int64_t sxc, float* partial,
                          int64_t rows, int cols, float eps, int tpr) {
   __shared__ float2 part[2][32];
   extern __shared__ float sums[];  // [rpb][cols] where rpb > 1
-  constexpr bool kAhead = ROUNDS < kMostRounds;
+  constexpr bool kAhead = MODE == kVec && ROUNDS < kMostRounds;
+  T* scratch = warp_scratch<T, MODE, kMaxThreads / 32>();
   const int t = threadIdx.x % tpr, g = threadIdx.x / tpr;
   const int rpb = blockDim.x / tpr;
-  const int width = tpr * 8;
+  const int width = tpr * 8, lane8 = (threadIdx.x & 31) * 8;
   const float n = static_cast<float>(cols);
   float* mine = partial + blockIdx.x * static_cast<int64_t>(cols);
-  float acc[ROUNDS][8], wf[kAhead ? ROUNDS : 1][8];
+  float acc[ROUNDS][8];
+  Raw8<T> wr[kAhead ? ROUNDS : 1];
   auto weight = [&](int k, float(&wt)[8]) {
-    if constexpr (kAhead) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) wt[i] = wf[k][i];
-    } else {
-      unpack8(load8<T, VEC>(w, 1, k * width + t * 8, cols), wt);
-    }
+    if constexpr (kAhead) unpack8(wr[k], wt);
+    else unpack8(load8<T, MODE>(w, 1, k * width + t * 8, cols, scratch), wt);
   };
 #pragma unroll
   for (int k = 0; k < ROUNDS; ++k) {
-    if constexpr (kAhead) unpack8(load8<T, VEC>(w, 1, k * width + t * 8, cols), wf[k]);
+    if constexpr (kAhead) wr[k] = load8<T, MODE>(w, 1, k * width + t * 8, cols, scratch);
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[k][i] = 0.f;
   }
-  Raw8<T> a[ROUNDS], b[ROUNDS];
+  Frag<T, MODE> a[ROUNDS], b[ROUNDS], e[DH ? ROUNDS : 1];
   auto fetch = [&](int64_t row) {
     const int lim = row < rows ? cols : 0;
     const T* dyr = static_cast<const T*>(dy.p) + row * dy.sr;
@@ -178,22 +182,28 @@ __global__ void __launch_bounds__(kMaxThreads, backward_blocks_per_sm(ROUNDS))
 #pragma unroll
     for (int k = 0; k < ROUNDS; ++k) {
       const int c = k * width + t * 8;
-      a[k] = load8<T, VEC>(dyr, dy.sc, c, lim);
-      b[k] = load8<T, VEC>(hr, h.sc, c, lim);
+      a[k] = fetch8<T, MODE>(dyr, dy.sc, c, lim);
+      b[k] = fetch8<T, MODE>(hr, h.sc, c, lim);
+      if (DH) e[k] = fetch8<T, MODE>(static_cast<const T*>(dh.p) + row * dh.sr, dh.sc, c, lim);
     }
   };
   // dx, and the weight's terms into `sum`
-  auto finish = [&](const float(&d)[8], const float(&v)[8], const float(&wt)[8], int64_t row, int64_t c, int lim, float r,
-                    float rm, float(&sum)[8]) {
-    float o[8], e[8];
-    if (DH) unpack8(load8<T, VEC>(static_cast<const T*>(dh.p) + row * dh.sr, dh.sc, c, lim), e);
+  auto finish = [&](const Raw8<T>& rd, const Raw8<T>& rv, const Raw8<T>& re, const float(&wt)[8], int64_t row, int64_t c,
+                    int lim, float r, float rm, float(&sum)[8]) {
+    float d[8], v[8], o[8];
+    unpack8(rd, d);
+    unpack8(rv, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       o[i] = fmaf(v[i], -rm, d[i] * wt[i] * r);
-      if (DH) o[i] += e[i];
       sum[i] = fmaf(d[i] * v[i], r, sum[i]);
     }
-    store8<T, VEC>(dx + row * sxr, sxc, c, lim, pack8<T>(o));
+    if (DH) {
+      unpack8(re, d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] += d[i];
+    }
+    store8<T, MODE>(dx + row * sxr, sxc, c, lim, pack8<T>(o), scratch);
   };
   const int64_t step = static_cast<int64_t>(gridDim.x) * rpb;
   const int64_t trips = (rows - static_cast<int64_t>(blockIdx.x) * rpb + step - 1) / step;  // the block's; at least one
@@ -203,7 +213,10 @@ __global__ void __launch_bounds__(kMaxThreads, backward_blocks_per_sm(ROUNDS))
   for (int64_t trip = 0; trip < trips; ++trip, row += step) {
     const int lim = row < rows ? cols : 0;  // every thread of the block reaches the barrier
     float2 s = make_float2(0.f, 0.f);
-    auto add = [&](const float(&d)[8], const float(&v)[8], const float(&wt)[8]) {
+    auto add = [&](const Raw8<T>& rd, const Raw8<T>& rv, const float(&wt)[8]) {
+      float d[8], v[8];
+      unpack8(rd, d);
+      unpack8(rv, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         s.x = fmaf(v[i], v[i], s.x);
@@ -211,26 +224,24 @@ __global__ void __launch_bounds__(kMaxThreads, backward_blocks_per_sm(ROUNDS))
       }
     };
     if (!kAhead) fetch(row);
-    Raw8<T> ca[ROUNDS], cb[ROUNDS];
+    Raw8<T> ca[ROUNDS], cb[ROUNDS], ce[DH ? ROUNDS : 1];
 #pragma unroll
     for (int k = 0; k < ROUNDS; ++k) {
-      ca[k] = a[k];
-      cb[k] = b[k];
-      float d[8], v[8], wt[8];
-      unpack8(ca[k], d);
-      unpack8(cb[k], v);
+      ca[k] = settle8<T, MODE>(a[k], scratch);
+      cb[k] = settle8<T, MODE>(b[k], scratch);
+      if (DH) ce[k] = settle8<T, MODE>(e[k], scratch);
+      float wt[8];
       weight(k, wt);
-      add(d, v, wt);
+      add(ca[k], cb[k], wt);
     }
     const T* dyr = static_cast<const T*>(dy.p) + row * dy.sr;
     const T* hr = static_cast<const T*>(h.p) + row * h.sr;
     if constexpr (ROUNDS == kMostRounds) {
       for (int64_t c = ROUNDS * width + t * 8; c - t * 8 < cols; c += width) {
-        float d[8], v[8], wt[8];
-        unpack8(load8<T, VEC>(dyr, dy.sc, c, lim), d);
-        unpack8(load8<T, VEC>(hr, h.sc, c, lim), v);
-        unpack8(load8<T, VEC>(w, 1, c, cols), wt);
-        add(d, v, wt);
+        float wt[8];
+        unpack8(load8<T, MODE>(w, 1, c, cols, scratch), wt);
+        const Raw8<T> rd = load8<T, MODE>(dyr, dy.sc, c, lim, scratch);
+        add(rd, load8<T, MODE>(hr, h.sc, c, lim, scratch), wt);
       }
     }
     if (kAhead && trip + 1 < trips) fetch(row + step);
@@ -241,23 +252,22 @@ __global__ void __launch_bounds__(kMaxThreads, backward_blocks_per_sm(ROUNDS))
 #pragma unroll
     for (int k = 0; k < ROUNDS; ++k) {
       const int c = k * width + t * 8;
-      if (c < lim) {
-        float d[8], v[8], wt[8];
-        unpack8(ca[k], d);
-        unpack8(cb[k], v);
+      if (c - lane8 < lim) {
+        float wt[8];
         weight(k, wt);
-        finish(d, v, wt, row, c, lim, r, rm, acc[k]);
+        finish(ca[k], cb[k], ce[DH ? k : 0], wt, row, c, lim, r, rm, acc[k]);
       }
     }
     if constexpr (ROUNDS == kMostRounds) {  // such rows are long: one group a block, whose columns are this thread's own
-      for (int64_t c = ROUNDS * width + t * 8; c < lim; c += width) {
-        float d[8], v[8], wt[8], sum[8];
-        unpack8(load8<T, VEC>(dyr, dy.sc, c, lim), d);
-        unpack8(load8<T, VEC>(hr, h.sc, c, lim), v);
-        unpack8(load8<T, VEC>(w, 1, c, cols), wt);
+      for (int64_t c = ROUNDS * width + t * 8; c - lane8 < lim; c += width) {
+        float wt[8], sum[8];
+        unpack8(load8<T, MODE>(w, 1, c, cols, scratch), wt);
+        const Raw8<T> rd = load8<T, MODE>(dyr, dy.sc, c, lim, scratch), rv = load8<T, MODE>(hr, h.sc, c, lim, scratch);
+        Raw8<T> re = rd;
+        if (DH) re = load8<T, MODE>(static_cast<const T*>(dh.p) + row * dh.sr, dh.sc, c, lim, scratch);
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[i] = trip > 0 && c + i < cols ? mine[c + i] : 0.f;
-        finish(d, v, wt, row, c, lim, r, rm, sum);
+        finish(rd, rv, re, wt, row, c, lim, r, rm, sum);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (c + i < cols) mine[c + i] = sum[i];
@@ -393,8 +403,10 @@ int32_t b2g_micro_rms_norm(const b2g_micro_matrix* x, const b2g_micro_matrix* re
     if (!weight) return record_error(B2G_ERR_INVALID_ARG, "null weight");
     const Split s = forward_split(q ? ceil_div(rows, 128) * 128 : rows, cols);
     if (s.blocks > kMaxGrid) return too_large("rms_norm");
-    const bool vec = vec_ok(x, rows, cols, 2) && (!residual || vec_ok(residual, rows, cols, 2)) &&
-                     (!h || vec_ok(h, rows, cols, 2)) && (!y || vec_ok(y, rows, cols, 2)) && aligned16(weight);
+    const b2g_micro_matrix w = {const_cast<void*>(weight), cols, 1};
+    int mode = std::max(mode_of(x, rows, cols, 2), mode_of(&w, 1, cols, 2));
+    for (const b2g_micro_matrix* m : {residual, h, y})
+      if (m) mode = std::max(mode, mode_of(m, rows, cols, 2));
     return by_type(dtype, [&](auto t) -> int32_t {
       using T = decltype(t);
       if constexpr (sizeof(T) == 4) {
@@ -412,9 +424,11 @@ int32_t b2g_micro_rms_norm(const b2g_micro_matrix* x, const b2g_micro_matrix* re
           constexpr int F = decltype(f)::value;
           return by_flag(residual, [&](auto res) {
             constexpr bool R = decltype(res)::value;
-            if (!vec) return go(norm_kernel<T, F, R, false, kMostRounds>);
-            return s.rounds == 1 ? go(norm_kernel<T, F, R, true, 1>)
-                                 : s.rounds == 2 ? go(norm_kernel<T, F, R, true, 2>) : go(norm_kernel<T, F, R, true, kMostRounds>);
+            if (mode == kAny) return go(norm_kernel<T, F, R, kAny, kMostRounds>);
+            if (mode == kUnit) return s.rounds <= 2 ? go(norm_kernel<T, F, R, kUnit, 2>) : go(norm_kernel<T, F, R, kUnit, kMostRounds>);
+            return s.rounds == 1   ? go(norm_kernel<T, F, R, kVec, 1>)
+                   : s.rounds == 2 ? go(norm_kernel<T, F, R, kVec, 2>)
+                                   : go(norm_kernel<T, F, R, kVec, kMostRounds>);
           });
         };
         return q ? by_format(q->format, pick) : pick(std::integral_constant<int, FMT_NONE>{});
@@ -457,8 +471,9 @@ int32_t b2g_micro_rms_norm_backward(const b2g_micro_matrix* dy, const b2g_micro_
       return record_error(B2G_ERR_WORKSPACE, "rms_norm_backward: workspace missing, misaligned or too small");
     const int64_t wgrid = ceil_div(cols, 32);
     if (wgrid > kMaxGrid) return too_large("rms_norm_backward");
-    const bool vec = vec_ok(dy, rows, cols, 2) && vec_ok(h, rows, cols, 2) && vec_ok(dx, rows, cols, 2) &&
-                     (!dh || vec_ok(dh, rows, cols, 2)) && aligned16(weight);
+    const b2g_micro_matrix w = {const_cast<void*>(weight), cols, 1};
+    int mode = std::max({mode_of(dy, rows, cols, 2), mode_of(h, rows, cols, 2), mode_of(dx, rows, cols, 2), mode_of(&w, 1, cols, 2)});
+    if (dh) mode = std::max(mode, mode_of(dh, rows, cols, 2));
     return by_type(dtype, [&](auto t) -> int32_t {
       using T = decltype(t);
       if constexpr (sizeof(T) == 4) {
@@ -474,9 +489,12 @@ int32_t b2g_micro_rms_norm_backward(const b2g_micro_matrix* dy, const b2g_micro_
         };
         const int32_t rc = by_flag(dh, [&](auto f) {
           constexpr bool D = decltype(f)::value;
-          if (!vec) return go(norm_backward_kernel<T, D, false, kMostRounds>);
-          return s.rounds == 1 ? go(norm_backward_kernel<T, D, true, 1>)
-                               : s.rounds == 2 ? go(norm_backward_kernel<T, D, true, 2>) : go(norm_backward_kernel<T, D, true, kMostRounds>);
+          if (mode == kAny) return go(norm_backward_kernel<T, D, kAny, kMostRounds>);
+          if (mode == kUnit)
+            return s.rounds <= 2 ? go(norm_backward_kernel<T, D, kUnit, 2>) : go(norm_backward_kernel<T, D, kUnit, kMostRounds>);
+          return s.rounds == 1   ? go(norm_backward_kernel<T, D, kVec, 1>)
+                 : s.rounds == 2 ? go(norm_backward_kernel<T, D, kVec, 2>)
+                                 : go(norm_backward_kernel<T, D, kVec, kMostRounds>);
         });
         if (rc) return rc;
         norm_dweight_kernel<T><<<static_cast<unsigned>(wgrid), 1024, 0, st>>>(static_cast<const float*>(workspace),

@@ -34,10 +34,10 @@ __device__ __forceinline__ uint32_t finite_amax8(const Raw8<T>& r) {
   return m;
 }
 
-// FLAT: rows follow one another without a gap, and are one row of `chunks` chunks. Else a row's eight-column chunks are
+// FLAT: rows follow one another without a gap, and are one row of `cols` values in `chunks` whole chunks and a rest. Else a row's eight-column chunks are
 // numbered across rows; a thread steps by the whole grid, four chunks in flight, and
 // carries (row, chunk) along instead of dividing.
-template <typename T, bool VEC, bool FLAT>
+template <typename T, int MODE, bool FLAT>
 __global__ void __launch_bounds__(1024)
     tensor_scale_kernel(Mat x, int64_t rows, int64_t cols, int64_t chunks, int64_t step_rows, int64_t step_chunks, float* scale) {
   const int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
@@ -50,16 +50,17 @@ __global__ void __launch_bounds__(1024)
     for (k = first; k < chunks; k += U * step) {
       Raw8<T> r[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) r[u] = load8<T, true>(p, 1, (k + u * step) * 8, chunks * 8);
+      for (int u = 0; u < U; ++u) r[u] = load8<T, kVec>(p, 1, (k + u * step) * 8, chunks * 8, nullptr);
 #pragma unroll
       for (int u = 0; u < U; ++u) m = max(m, finite_amax8(r[u]));
     }
+    if (first < cols - chunks * 8) m = max(m, finite_bits(to_f32(p[chunks * 8 + first])));  // the last, fewer than eight
   } else {
     while (row < rows) {
       Raw8<T> r[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        r[u] = load8<T, VEC>(p + row * x.sr, x.sc, k * 8, row < rows ? cols : 0);
+        r[u] = load8<T, MODE>(p + row * x.sr, x.sc, k * 8, row < rows ? cols : 0, nullptr);
         row += step_rows;
         k += step_chunks;
         if (k >= chunks) {
@@ -114,7 +115,7 @@ struct GateSource {
   }
 };
 
-template <typename T, int FMT, bool VEC, template <typename> class SRC>
+template <typename T, int FMT, int MODE, template <typename> class SRC>
 __global__ void __launch_bounds__(kWarps * 32)
     quantize_rows_kernel(Mat x, int64_t rows, int64_t cols, Quant q, int64_t col_chunks, int64_t tasks) {
   const int lane = threadIdx.x & 31;
@@ -128,19 +129,23 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int64_t code_step = 32 * q.pitch;
   const int live = row0 >= rows ? 0 : static_cast<int>(min(static_cast<int64_t>(4), (rows - row0 + 31) / 32));
   using S = SRC<T>;
-  Raw8<T> r[4][S::kLoads];
+  T* scratch = warp_scratch<T, MODE, kWarps>();
+  Frag<T, MODE> f[4][S::kLoads];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
 #pragma unroll
     for (int k = 0; k < S::kLoads; ++k)
-      r[i][k] = load8<T, VEC>(static_cast<const T*>(x.p) + (row0 + 32 * i) * x.sr + k * cols * x.sc, x.sc, c, i < live ? cols : 0);
+      f[i][k] = fetch8<T, MODE>(static_cast<const T*>(x.p) + (row0 + 32 * i) * x.sr + k * cols * x.sc, x.sc, c, i < live ? cols : 0);
   }
   const TensorScale ts(FMT == FMT_NVFP4 ? *q.scale : 1.f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (i < live) {
+      Raw8<T> r[S::kLoads];
+#pragma unroll
+      for (int k = 0; k < S::kLoads; ++k) r[k] = settle8<T, MODE>(f[i][k], scratch);
       float v[8];
-      const uint32_t m = S::value(r[i], v);
+      const uint32_t m = S::value(r, v);
       quantize_store<FMT>(v, m, lane, to, ts);
     } else if (to.leads) {  // a row past the last: zero scales and no codes
       *reinterpret_cast<uint32_t*>(to.word) = 0u;
@@ -270,7 +275,7 @@ __global__ void __launch_bounds__(128) quantize_cols_kernel(Mat x, int64_t rows,
 // ---------------------------------------------------------------- codes and scales -> values
 // A lane reads eight columns' codes of four rows, twice (256 columns apart), with each block's one scale byte, and stores
 // 16 bytes a row (fp32: 32), a warp 512 consecutive ones.
-template <typename T, int FMT, bool VEC>
+template <typename T, int FMT, int MODE>
 __global__ void __launch_bounds__(kWarps * 32)
     dequantize_kernel(const uint8_t* codes, int64_t pitch, const uint8_t* scales, const float* scale, int64_t rows,
                       int64_t cols, int64_t ktiles, T* out, int64_t sr, int64_t sc, int64_t col_chunks, int64_t tasks) {
@@ -281,6 +286,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int64_t c0 = (task - rj * col_chunks) * 512 + lane * 8;
   const int64_t row0 = (rj >> 5) * 128 + (rj & 31);
   const float ts = FMT == FMT_NVFP4 ? *scale : 1.f;
+  T* scratch = warp_scratch<T, MODE, kWarps>();
   uint2 q[2][4];
   uint32_t s[2][4];
 #pragma unroll
@@ -290,6 +296,8 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int64_t row = row0 + 32 * i;
+      q[h][i] = make_uint2(0u, 0u);
+      s[h][i] = 0u;
       if (row < rows && c < cols) {  // a row's codes are readable up to a multiple of 32 columns
         if constexpr (FMT == FMT_MXFP8) q[h][i] = __ldg(reinterpret_cast<const uint2*>(codes + row * pitch + c));
         else q[h][i].x = __ldg(reinterpret_cast<const uint32_t*>(codes + row * pitch + (c >> 1)));
@@ -303,7 +311,7 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int64_t row = row0 + 32 * i;
-      if (row >= rows || c >= cols) break;
+      if (row >= rows || c - lane * 8 >= cols) break;
       float bs;
       if constexpr (FMT == FMT_NVFP4) bs = e4m3_to_f32(s[h][i]);
       else bs = mx_scale_value(s[h][i]);
@@ -324,38 +332,42 @@ __global__ void __launch_bounds__(kWarps * 32)
           v[2 * k + 1] *= ts;
         }
       }
-      store8<T, VEC>(out + row * sr, sc, c, cols, pack8<T>(v));
+      store8<T, MODE>(out + row * sr, sc, c, cols, pack8<T>(v), scratch);
     }
   }
 }
 
 // ---------------------------------------------------------------- the gate as values, and its gradient
-template <typename T, bool VEC>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(256) gate_kernel(Mat x, T* y, int64_t syr, int64_t syc, int64_t rows, int64_t cols, uint32_t row_blocks) {
-  // blockDim.y rows of blockDim.x chunks of eight columns; row_blocks blocks along a row
+  // blockDim.y rows of blockDim.x chunks of eight columns (kUnit: whole warps of them); row_blocks blocks along a row
   const uint32_t k = blockIdx.x % row_blocks * blockDim.x + threadIdx.x;
   const int64_t row = static_cast<int64_t>(blockIdx.x / row_blocks) * blockDim.y + threadIdx.y, c = static_cast<int64_t>(k) * 8;
-  if (row >= rows || c >= cols) return;
+  if (row >= rows || (MODE == kUnit ? c - (threadIdx.x & 31) * 8 : c) >= cols) return;
+  T* scratch = warp_scratch<T, MODE, 8>();
   const T* p = static_cast<const T*>(x.p) + row * x.sr;
-  Raw8<T> r[2] = {load8<T, VEC>(p, x.sc, c, cols), load8<T, VEC>(p + cols * x.sc, x.sc, c, cols)};
+  const Frag<T, MODE> f = fetch8<T, MODE>(p, x.sc, c, cols), g = fetch8<T, MODE>(p + cols * x.sc, x.sc, c, cols);
+  const Raw8<T> r[2] = {settle8<T, MODE>(f, scratch), settle8<T, MODE>(g, scratch)};
   float v[8];
   GateSource<T>::value(r, v);
-  store8<T, VEC>(y + row * syr, syc, c, cols, pack8<T>(v));
+  store8<T, MODE>(y + row * syr, syc, c, cols, pack8<T>(v), scratch);
 }
 
 // With s = sigmoid(g): d gate = dy * up * s * (1 + g * (1 - s)), d up = dy * g * s. 1 - s is taken as sigmoid(-g), which
 // keeps its digits where s is near one.
-template <typename T, bool VEC>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(256)
     gate_backward_kernel(Mat dy, Mat x, T* dx, int64_t sxr, int64_t sxc, int64_t rows, int64_t cols,
                          uint32_t row_blocks) {
-  // blockDim.y rows of blockDim.x chunks of eight columns; row_blocks blocks along a row
+  // blockDim.y rows of blockDim.x chunks of eight columns (kUnit: whole warps of them); row_blocks blocks along a row
   const uint32_t k = blockIdx.x % row_blocks * blockDim.x + threadIdx.x;
   const int64_t row = static_cast<int64_t>(blockIdx.x / row_blocks) * blockDim.y + threadIdx.y, c = static_cast<int64_t>(k) * 8;
-  if (row >= rows || c >= cols) return;
+  if (row >= rows || (MODE == kUnit ? c - (threadIdx.x & 31) * 8 : c) >= cols) return;
+  T* scratch = warp_scratch<T, MODE, 8>();
   const T* p = static_cast<const T*>(x.p) + row * x.sr;
-  const Raw8<T> rg = load8<T, VEC>(p, x.sc, c, cols), ru = load8<T, VEC>(p + cols * x.sc, x.sc, c, cols);
-  const Raw8<T> rd = load8<T, VEC>(static_cast<const T*>(dy.p) + row * dy.sr, dy.sc, c, cols);
+  const Frag<T, MODE> fg = fetch8<T, MODE>(p, x.sc, c, cols), fu = fetch8<T, MODE>(p + cols * x.sc, x.sc, c, cols);
+  const Frag<T, MODE> fd = fetch8<T, MODE>(static_cast<const T*>(dy.p) + row * dy.sr, dy.sc, c, cols);
+  const Raw8<T> rg = settle8<T, MODE>(fg, scratch), ru = settle8<T, MODE>(fu, scratch), rd = settle8<T, MODE>(fd, scratch);
   float g[8], u[8], d[8], dg[8], du[8];
   unpack8(rg, g);
   unpack8(ru, u);
@@ -368,8 +380,8 @@ __global__ void __launch_bounds__(256)
     du[i] = d[i] * g[i] * s;
   }
   T* o = dx + row * sxr;
-  store8<T, VEC>(o, sxc, c, cols, pack8<T>(dg));
-  store8<T, VEC>(o + cols * sxc, sxc, c, cols, pack8<T>(du));
+  store8<T, MODE>(o, sxc, c, cols, pack8<T>(dg), scratch);
+  store8<T, MODE>(o + cols * sxc, sxc, c, cols, pack8<T>(du), scratch);
 }
 
 // ---------------------------------------------------------------- host side
@@ -380,22 +392,22 @@ struct RowBlocks {
   int64_t grid;
 };
 
-RowBlocks row_blocks(int64_t rows, int64_t cols) {
+RowBlocks row_blocks(int64_t rows, int64_t cols, int mode) {
   const int64_t chunks = ceil_div(cols, 8);
-  unsigned x = 1;
+  unsigned x = mode == kUnit ? 32 : 1;
   while (x < chunks && x < 256) x *= 2;
   RowBlocks b{dim3(x, 256 / x), static_cast<uint32_t>(ceil_div(chunks, x)), 0};
   b.grid = ceil_div(rows, b.block.y) * b.along;
   return b;
 }
 
-template <typename T, int FMT, bool VEC, template <typename> class SRC>
+template <typename T, int FMT, int MODE, template <typename> class SRC>
 int32_t run_rows(const Mat& x, int64_t rows, int64_t cols, const Quant& q, cudaStream_t st) {
   const int64_t col_chunks = ceil_div(q.ktiles * 4 * block_of(FMT), 256);  // whole scale tiles, so that all are written
   const int64_t tasks = ceil_div(rows, 128) * 32 * col_chunks;
   const int64_t grid = ceil_div(tasks, kWarps);
   if (grid > kMaxGrid) return too_large("quantisation");
-  quantize_rows_kernel<T, FMT, VEC, SRC><<<static_cast<unsigned>(grid), kWarps * 32, 0, st>>>(x, rows, cols, q, col_chunks, tasks);
+  quantize_rows_kernel<T, FMT, MODE, SRC><<<static_cast<unsigned>(grid), kWarps * 32, 0, st>>>(x, rows, cols, q, col_chunks, tasks);
   return launched("quantize launch");
 }
 
@@ -415,8 +427,9 @@ int32_t run_quantize(const b2g_micro_matrix* x, const b2g_micro_tensor* t, cudaS
       return launched("quantize launch");
     }
   }
-  if (vec_ok(x, t->rows, t->cols, sizeof(T))) return run_rows<T, FMT, true, ValueSource>(m, t->rows, t->cols, q, st);
-  return run_rows<T, FMT, false, ValueSource>(m, t->rows, t->cols, q, st);
+  return by_mode(mode_of(x, t->rows, t->cols, sizeof(T)), [&](auto mode) {
+    return run_rows<T, FMT, decltype(mode)::value, ValueSource>(m, t->rows, t->cols, q, st);
+  });
 }
 
 }  // namespace micro
@@ -473,13 +486,12 @@ int32_t b2g_micro_tensor_scale(const b2g_micro_matrix* x, int64_t rows, int64_t 
         }
       }
       const int64_t step = static_cast<int64_t>(grid) * threads;
-      const bool vec = vec_ok(&view, r, c, sizeof(T));
-      if (vec && (r == 1 || m.sr == c))
-        tensor_scale_kernel<T, true, true><<<grid, threads, 0, st>>>(m, 1, r * c, r * chunks, 0, 0, scale);
-      else if (vec)
-        tensor_scale_kernel<T, true, false><<<grid, threads, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
+      if (m.sc == 1 && aligned16(m.p) && (r == 1 || m.sr == c))
+        tensor_scale_kernel<T, kVec, true><<<grid, threads, 0, st>>>(m, 1, r * c, r * c / 8, 0, 0, scale);
+      else if (mode_of(&view, r, c, sizeof(T)) == kVec)
+        tensor_scale_kernel<T, kVec, false><<<grid, threads, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
       else
-        tensor_scale_kernel<T, false, false><<<grid, threads, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
+        tensor_scale_kernel<T, kAny, false><<<grid, threads, 0, st>>>(m, r, c, chunks, step / chunks, step % chunks, scale);
       return launched("tensor_scale launch");
     });
   });
@@ -518,9 +530,10 @@ int32_t b2g_micro_dequantize(const b2g_micro_tensor* q, const b2g_micro_matrix* 
               q->cols, ceil_div(q->cols, 4 * block_of(F)), static_cast<T*>(out->ptr), out->stride_r, out->stride_c,
               col_chunks, tasks);
         };
-        if (vec_ok(out, q->rows, q->cols, sizeof(T))) go(dequantize_kernel<T, F, true>);
-        else go(dequantize_kernel<T, F, false>);
-        return launched("dequantize launch");
+        return by_mode(mode_of(out, q->rows, q->cols, sizeof(T)), [&](auto mode) {
+          go(dequantize_kernel<T, F, decltype(mode)::value>);
+          return launched("dequantize launch");
+        });
       });
     });
   });
@@ -543,22 +556,23 @@ int32_t b2g_micro_silu_mul(const b2g_micro_matrix* gate_up, const b2g_micro_matr
       if constexpr (sizeof(T) == 4) {
         return B2G_ERR_INVALID_ARG;
       } else {
-        const bool vec = vec_ok(gate_up, rows, cols, 2);  // the up half starts `cols` values into the row
+        int mode = mode_of(gate_up, rows, cols, 2);  // kVec: the up half, `cols` values into the row, is aligned too
         if (q) {
           return by_format(q->format, [&](auto f) {
-            constexpr int F = decltype(f)::value;
-            return vec ? run_rows<T, F, true, GateSource>(mat(gate_up), rows, cols, quant(q), st)
-                       : run_rows<T, F, false, GateSource>(mat(gate_up), rows, cols, quant(q), st);
+            return by_mode(mode, [&](auto md) {
+              return run_rows<T, decltype(f)::value, decltype(md)::value, GateSource>(mat(gate_up), rows, cols, quant(q), st);
+            });
           });
         }
         if (const int32_t rc = check_matrix(y, "y")) return rc;
-        const RowBlocks rb = row_blocks(rows, cols);
-    const int64_t grid = rb.grid;
-        if (grid > kMaxGrid) return too_large("silu_mul");
-        if (vec && vec_ok(y, rows, cols, 2))
-          gate_kernel<T, true><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols, rb.along);
-        else
-          gate_kernel<T, false><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols, rb.along);
+        mode = std::max(mode, mode_of(y, rows, cols, 2));
+        const RowBlocks rb = row_blocks(rows, cols, mode);
+        if (rb.grid > kMaxGrid) return too_large("silu_mul");
+        by_mode(mode, [&](auto md) -> int32_t {
+          gate_kernel<T, decltype(md)::value><<<static_cast<unsigned>(rb.grid), rb.block, 0, st>>>(
+              mat(gate_up), static_cast<T*>(y->ptr), y->stride_r, y->stride_c, rows, cols, rb.along);
+          return B2G_OK;
+        });
         return launched("silu_mul launch");
       }
     });
@@ -575,20 +589,19 @@ int32_t b2g_micro_silu_mul_backward(const b2g_micro_matrix* dy, const b2g_micro_
     if (const int32_t rc = check_matrix(dy, "dy")) return rc;
     if (const int32_t rc = check_matrix(gate_up, "gate_up")) return rc;
     if (const int32_t rc = check_matrix(dgate_up, "dgate_up")) return rc;
-    const RowBlocks rb = row_blocks(rows, cols);
-    const int64_t grid = rb.grid;
-    if (grid > kMaxGrid) return too_large("silu_mul_backward");
     return by_type(dtype, [&](auto t) -> int32_t {
       using T = decltype(t);
       if constexpr (sizeof(T) == 4) {
         return B2G_ERR_INVALID_ARG;
       } else {
-        cudaStream_t st = static_cast<cudaStream_t>(stream);
-        T* out = static_cast<T*>(dgate_up->ptr);
-        if (vec_ok(dy, rows, cols, 2) && vec_ok(gate_up, rows, cols, 2) && vec_ok(dgate_up, rows, cols, 2))
-          gate_backward_kernel<T, true><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(dy), mat(gate_up), out, dgate_up->stride_r, dgate_up->stride_c, rows, cols, rb.along);
-        else
-          gate_backward_kernel<T, false><<<static_cast<unsigned>(grid), rb.block, 0, st>>>(mat(dy), mat(gate_up), out, dgate_up->stride_r, dgate_up->stride_c, rows, cols, rb.along);
+        const int mode = std::max({mode_of(dy, rows, cols, 2), mode_of(gate_up, rows, cols, 2), mode_of(dgate_up, rows, cols, 2)});
+        const RowBlocks rb = row_blocks(rows, cols, mode);
+        if (rb.grid > kMaxGrid) return too_large("silu_mul_backward");
+        by_mode(mode, [&](auto md) -> int32_t {
+          gate_backward_kernel<T, decltype(md)::value><<<static_cast<unsigned>(rb.grid), rb.block, 0, static_cast<cudaStream_t>(stream)>>>(
+              mat(dy), mat(gate_up), static_cast<T*>(dgate_up->ptr), dgate_up->stride_r, dgate_up->stride_c, rows, cols, rb.along);
+          return B2G_OK;
+        });
         return launched("silu_mul_backward launch");
       }
     });
