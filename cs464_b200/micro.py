@@ -91,6 +91,17 @@ def _matrix(t: torch.Tensor) -> bytes:
     return _pack_matrix(t.data_ptr(), *t.stride())
 
 
+_BYTES: dict[int, torch.Tensor] = {}  # an empty uint8 tensor per device: new_empty of it is the cheapest allocation
+
+
+def _new_bytes(n: int, like: torch.Tensor) -> torch.Tensor:
+    index = like.get_device()
+    proto = _BYTES.get(index)
+    if proto is None:
+        proto = _BYTES[index] = torch.empty(0, dtype=torch.uint8, device=like.device)
+    return proto.new_empty(n)
+
+
 def _format(fmt: str) -> int:
     try:
         return FORMATS[fmt]
@@ -179,7 +190,7 @@ class MicroTensor:
         """Uninitialised storage (codes, then scales) on the device of `like`, for a kernel to fill."""
         self = cls.__new__(cls)
         pitch, scale_bytes = _layout(fmt, rows, cols)
-        buf = self._buf = like.new_empty((rows * pitch + scale_bytes,), dtype=torch.uint8)
+        buf = self._buf = _new_bytes(rows * pitch + scale_bytes, like)
         at = buf.data_ptr()
         self._codes = self._scales = None
         self.shape, self.format, self.scale = (rows, cols), format, scale
@@ -239,12 +250,13 @@ def quantize(x: torch.Tensor, format: str = "mxfp8", scale: torch.Tensor | None 
 
     nvfp4: `scale` is the tensor's fp32 scale, one positive element on the device; values past 2688 times it saturate.
     Without it, x is read twice: its scale becomes the smallest power of two at which nothing saturates."""
-    fmt = _format(format)
-    _check(x, "x", _VALUES)
-    if x.dim() != 2:
+    fmt = FORMATS.get(format)
+    if fmt is None or not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _VALUES or x.dim() != 2:
+        _format(format)
+        _check(x, "x", _VALUES)
         raise ValueError(f"x must be a matrix, not {tuple(x.shape)}")
     rows, cols = x.shape
-    mat, kind, index = _matrix(x), _VALUES[x.dtype], x.get_device()
+    mat, kind, index = _pack_matrix(x.data_ptr(), *x.stride()), _VALUES[x.dtype], x.get_device()
     if fmt == _abi.FMT_NVFP4:
         if scale is None:
             scale = x.new_empty((1,), dtype=torch.float32)
@@ -445,6 +457,18 @@ class _Norm(torch.autograd.Function):
         return dx, (dx if ctx.needs_input_grad[1] else None), dw, None
 
 
+def _norm_args(x, weight, residual) -> bool:
+    """Whether rms_norm takes them: the checks that rms_norm repeats one by one where they fail."""
+    try:
+        dtype, index, shape = x.dtype, x.get_device(), x.shape
+        return (dtype in _HALF and index >= 0 and weight.dtype is dtype and weight.get_device() == index
+                and shape[-1:] == weight.shape and weight.dim() == 1
+                and (residual is None or (residual.dtype is dtype and residual.shape == shape
+                                          and residual.get_device() == index)))
+    except (AttributeError, TypeError):
+        return False
+
+
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-5,
              format: str | None = None, scale: torch.Tensor | None = None):
     """(y, h): h = x + residual (x itself without one), y = h * weight / sqrt(mean(h^2) + eps) over the last dimension.
@@ -453,18 +477,17 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     sum rounded to the type, the next layer's residual. Without `format` y has x's type and shape and both outputs are
     differentiable. With one, y is a MicroTensor [rows, cols], the next product's operand; nvfp4 then needs the tensor's
     `scale`."""
-    _check(x, "x", _HALF)
-    _check(weight, "weight", (x.dtype,), x)
-    if x.dim() < 1 or weight.shape != x.shape[-1:]:
-        raise ValueError(f"weight must be [{x.shape[-1] if x.dim() else '?'}], not {tuple(weight.shape)}")
-    x2, r2, grad = _rows(x), None, x.requires_grad or weight.requires_grad
-    if residual is not None:
+    if not _norm_args(x, weight, residual):
+        _check(x, "x", _HALF)
+        _check(weight, "weight", (x.dtype,), x)
+        if x.dim() < 1 or weight.shape != x.shape[-1:]:
+            raise ValueError(f"weight must be [{x.shape[-1] if x.dim() else '?'}], not {tuple(weight.shape)}")
         _check(residual, "residual", (x.dtype,), x)
-        if residual.shape != x.shape:
-            raise ValueError(f"residual is {tuple(residual.shape)}, x {tuple(x.shape)}")
-        r2 = _rows(residual)
-        grad = grad or residual.requires_grad
-    grad = grad and torch.is_grad_enabled()
+        raise ValueError(f"residual is {tuple(residual.shape)}, x {tuple(x.shape)}")
+    x2 = x if x.dim() == 2 else _rows(x)
+    r2 = residual if residual is None or residual.dim() == 2 else _rows(residual)
+    grad = (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)) \
+        and torch.is_grad_enabled()
     if not weight.is_contiguous():
         weight = weight.contiguous()
     if format is not None:

@@ -93,7 +93,7 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.b2g_micro_silu_mul_backward(mat, None, mat, 4, 64, 1, None) == inv
     assert lib.b2g_micro_tensor_scale(mat, 4, 64, 1, None, None) == inv
     n = ctypes.c_size_t()
-    assert lib.b2g_micro_rms_norm_workspace(4, 64, ctypes.byref(n)) == 0 and n.value >= 4 * 64 * 4
+    assert lib.b2g_micro_rms_norm_workspace(4, 64, ctypes.byref(n)) == 0 and n.value >= 64 * 4  # an fp32 row at least
     assert lib.b2g_micro_rms_norm_workspace(-1, 64, ctypes.byref(n)) == inv
 
 
