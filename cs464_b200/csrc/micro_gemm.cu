@@ -115,6 +115,17 @@ __device__ __forceinline__ uint32_t scale_cols(int q_tiles) {
   return tiles_of(KIND) * 4u * (1u + static_cast<uint32_t>(q_tiles));
 }
 
+// Four consecutive values of a row of C, `n` of which exist; `vec`: C's rows are 16-byte aligned.
+__device__ __forceinline__ void store_four(uint16_t* o, uint2 w, bool vec, int n) {
+  if (vec && n >= 4) {
+    *reinterpret_cast<uint2*>(o) = w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < n) o[k] = static_cast<uint16_t>((k < 2 ? w.x : w.y) >> (16 * (k & 1)));
+  }
+}
+
 // Issue one stage: its scales into tensor memory, then up to four MMAs (fewer where K ends inside the stage: codes past
 // K are zero but the scales there may be any bytes). `sp`, `sq`, `cp`, `cq`: shared addresses of P's and Q's codes and of
 // their scales.
@@ -269,45 +280,32 @@ __global__ void __launch_bounds__(192, 1)
     }
   }
   // Part two: CTA r of the cluster adds its share of the tile over the cluster's CTAs in split order, scales, converts
-  // and stores, eight consecutive columns of C at a time. Every thread of every CTA reaches both barriers.
+  // and stores, a lane four consecutive values (a warp's loads of other CTAs' memory are whole lines that way). Every thread of every CTA reaches both barriers.
   __syncwarp();
   if (p.split > 1) cluster_sync();
   else __syncthreads();
   {
     const float alpha = p.scale_a ? *p.scale_a * *p.scale_b : 1.f;
     const int cols = min(p.tile_q, p.rows_q - tq * p.tile_q);  // columns of the tile inside C^T
-    const int groups = cols * 16;
-    const int g0 = groups * split / p.split, g1 = groups * (split + 1) / p.split;
-    uint16_t* out = static_cast<uint16_t*>(p.out);
-    for (int g = g0 + static_cast<int>(threadIdx.x); g < g1; g += 192) {
-      const int j = g >> 4, i = (g & 15) * 8;
-      const int64_t n = static_cast<int64_t>(tp) * 128 + i;
-      if (n >= p.rows_p) continue;
+    const int groups = cols * 32;  // of four values
+    const int g1 = groups * (split + 1) / p.split;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(tq) * p.tile_q * p.ldc + static_cast<int64_t>(tp) * 128;
+    const int rows = p.rows_p - tp * 128;  // the tile's rows inside C^T
+    for (int g = groups * split / p.split + static_cast<int>(threadIdx.x); g < g1; g += 192) {
+      const int j = g >> 5, i = (g & 31) * 4;
+      if (i >= rows) continue;
       const uint32_t off = ring + (j * 132 + i) * 4u;
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int s = 0; s < p.split; ++s) {
-        const uint32_t at = p.split > 1 ? map_to_rank(off, s) : off;
-        const float4 x = ld_cluster_v4(at), y = ld_cluster_v4(at + 16);
-        v[0] += x.x;
-        v[1] += x.y;
-        v[2] += x.z;
-        v[3] += x.w;
-        v[4] += y.x;
-        v[5] += y.y;
-        v[6] += y.z;
-        v[7] += y.w;
+        const float4 x = ld_cluster_v4(p.split > 1 ? map_to_rank(off, s) : off);
+        v.x += x.x;
+        v.y += x.y;
+        v.z += x.z;
+        v.w += x.w;
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= alpha;
-      uint16_t* o = out + (static_cast<int64_t>(tq) * p.tile_q + j) * p.ldc + n;
-      if (p.vec && n + 8 <= p.rows_p) {
-        *reinterpret_cast<uint4*>(o) = make_uint4(cvt2(v[0], v[1], p.out_bf16), cvt2(v[2], v[3], p.out_bf16),
-                                                  cvt2(v[4], v[5], p.out_bf16), cvt2(v[6], v[7], p.out_bf16));
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (n + k < p.rows_p) o[k] = cvt1(v[k], p.out_bf16);
-      }
+      uint16_t* o = out + j * p.ldc + i;
+      const uint2 w = make_uint2(cvt2(v.x * alpha, v.y * alpha, p.out_bf16), cvt2(v.z * alpha, v.w * alpha, p.out_bf16));
+      store_four(o, w, p.vec, rows - i);
     }
   }
   __syncwarp();
@@ -319,6 +317,7 @@ __global__ void __launch_bounds__(192, 1)
 // ---------------------------------------------------------------- CTA pairs
 constexpr int kPairEpilogueWarps = 8;
 constexpr uint32_t kPairStaging = kPairEpilogueWarps * 4096u;
+constexpr int kPartRow = 256 + 4;  // floats a row of a split's part in shared memory
 
 // Tile `t` of the pairs' walk: bands of `group` tile rows, inside a band down the rows first, so that the tiles that run
 // at one time share operands in L2.
@@ -330,7 +329,7 @@ __device__ __forceinline__ void pair_tile(const Params& p, int t, int& tp, int& 
   tp = g * p.group + (r - tq * h);
 }
 
-// 256 x 256 tiles, a persistent CTA pair on each: every CTA loads its 128 rows of P, half of Q's 256 and the scales of
+// 256 x 256 tiles, a persistent CTA pair on each (or, with K split, the pairs of a cluster on one tile, a K range each): every CTA loads its 128 rows of P, half of Q's 256 and the scales of
 // its P rows and of all of Q (both tensor memories hold Q's scales), the leader issues MMAs of M = 256, and each CTA ends
 // with a 128 x 256 accumulator. 256 accumulator columns and the stages' scales fill tensor memory, so there is one
 // accumulator: the epilogue's eight warps read it into registers and free it before they convert the second half and
@@ -347,9 +346,13 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
   const uint32_t ring = (ctl + kCtl + 1023u) & ~1023u;
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem_raw + O_ABORT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(cluster_ctarank());
+  const int cta = static_cast<int>(cluster_ctarank());
+  const int rank = cta & 1, split = cta >> 1;  // within the pair; the pair's K split
+  const uint32_t lead = static_cast<uint32_t>(cta & ~1);
   const bool leader = rank == 0;
   const int first = static_cast<int>(cluster_id_x()), step = static_cast<int>(num_clusters_x());
+  const int kb0 = static_cast<int>(static_cast<int64_t>(split) * p.num_kb / p.split);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(split + 1) * p.num_kb / p.split);
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&map_p);
@@ -379,14 +382,14 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
 
   if (warp == 0) {
     if (lane == 0) {  // TMA producer: each CTA's copies count on the leader's barriers
-      const uint32_t full0 = map_to_rank(ctl + O_FULL, 0);
+      const uint32_t full0 = map_to_rank(ctl + O_FULL, lead);
       int s = 0, issued = 0;
       uint32_t ph = 0;
       bool ok = true;
       for (int t = first; ok && t < p.units; t += step) {
         int tp, tq;
         pair_tile(p, t, tp, tq);
-        for (int kb = 0; kb < p.num_kb; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           const uint32_t empty = ctl + O_EMPTY + 8 * s, full = full0 + 8 * s;
           if (!mbar_try_wait(empty, ph ^ 1u) && !wait_phase(empty, ph ^ 1u, abort_flag, p.status, kProducerTimeout)) {
             ok = false;
@@ -422,9 +425,9 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
       for (int i = 0; i < kStepsPerStage; ++i) idesc[i] = idesc_scaled(KIND, step_id(KIND, i), 256, 256);
       const uint64_t pd = sdesc_sw128(ring, 16u, 1024u), qd = sdesc_sw128(ring + kPBytes, 16u, 1024u);
       constexpr uint32_t cols = tiles_of(KIND) * 12u;  // a stage's scales: one tile row of P, two of Q
-      const uint32_t empty0 = map_to_rank(ctl + O_EMPTY, 0), empty1 = map_to_rank(ctl + O_EMPTY, 1);
+      const uint32_t empty0 = map_to_rank(ctl + O_EMPTY, lead), empty1 = map_to_rank(ctl + O_EMPTY, lead + 1);
       const uint32_t utmem = uniform(tmem);
-      const uint32_t tfull0 = map_to_rank(ctl + O_TFULL, 0), tfull1 = map_to_rank(ctl + O_TFULL, 1);
+      const uint32_t tfull0 = map_to_rank(ctl + O_TFULL, lead), tfull1 = map_to_rank(ctl + O_TFULL, lead + 1);
       const int last = p.K - (p.num_kb - 1) * stage_k(KIND);
       const int last_steps = (last + step_k(KIND) - 1) / step_k(KIND);
       int s = 0;
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
         }
         acc_ph ^= 1u;
         tc_fence_after();
-        for (int kb = 0; kb < p.num_kb; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           const uint32_t full = ctl + O_FULL + 8 * s;
           if (!warp_wait(full, ph, abort_flag, p.status, kMmaTimeout)) {
             ok = false;
@@ -446,7 +449,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
           const uint32_t base = ring + s * p.stage_bytes, off = s * (p.stage_bytes >> 4);
           issue_stage<KIND, 1>(utmem, pd + off, qd + off, base + kPBytes + p.q_bytes,
                                base + kPBytes + p.q_bytes + kTileBytes, utmem + p.acc_cols + s * cols, 2, idesc,
-                               kb + 1 == p.num_kb ? last_steps : kStepsPerStage, kb == 0 ? 0u : 1u);
+                               kb + 1 == p.num_kb ? last_steps : kStepsPerStage, kb == kb0 ? 0u : 1u);
           umma_commit_pair_w(empty0 + 8 * s);
           umma_commit_pair_w(empty1 + 8 * s);
           if (++s == p.stages) {
@@ -458,12 +461,12 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
         umma_commit_pair_w(tfull0);
         umma_commit_pair_w(tfull1);
       }
-      umma_commit_pair_w(map_to_rank(ctl + O_DRAIN, 0));
+      umma_commit_pair_w(map_to_rank(ctl + O_DRAIN, lead));
       drain_phase(ctl + O_DRAIN, 0, ok ? kWaitNs : kDrainNs);
     }
   } else {
     const int e = warp - 2, q = warp & 3, half = e >> 2;  // tensor-memory lane quarter, half of the columns
-    const uint32_t tempty = map_to_rank(ctl + O_TEMPTY, 0);
+    const uint32_t tempty = map_to_rank(ctl + O_TEMPTY, lead);
     const uint32_t stg = ring + p.stages * p.stage_bytes + static_cast<uint32_t>(e) * 4096u;
     const float alpha = p.scale_a ? *p.scale_a * *p.scale_b : 1.f;
     uint16_t* out = static_cast<uint16_t*>(p.out);
@@ -474,6 +477,19 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
       if (!wait_phase(ctl + O_TFULL, ph, abort_flag, p.status, kEpilogueTimeout)) break;
       ph ^= 1u;
       tc_fence_after();
+      if (p.split > 1) {  // the pair's only tile: this split's part of it stays in shared memory, fp32 (below)
+        const uint32_t to = ring + static_cast<uint32_t>((q * 32 + lane) * kPartRow + half * 128) * 4u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          tmem_ld_32cols(tmem + half * 128 + c * 32 + (static_cast<uint32_t>(q * 32) << 16), v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            st_shared_v4(to + (c * 32 + 4 * j) * 4u, make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+        }
+        break;
+      }
       uint32_t w[64];  // the row's 128 columns, rounded
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -535,7 +551,52 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
     if (lane == 0) tma_store_wait();
   }
   __syncwarp();
-  cluster_sync();  // the pair's MMAs and signals are done in both CTAs
+  cluster_sync();  // the pair's MMAs and signals are done in both CTAs; the splits' parts lie in shared memory
+  if (p.split > 1) {
+    // Each CTA adds its share of the columns of its 128 rows over the splits, in split order, from the CTAs of its rank in
+    // every pair; the rows were stored 4 floats apart in banks. Then the cluster's shared memory may go.
+    int tp, tq;
+    pair_tile(p, first, tp, tq);
+    const float alpha = p.scale_a ? *p.scale_a * *p.scale_b : 1.f;
+    const int per0 = 64 * split / p.split, per = 64 * (split + 1) / p.split - per0;  // groups of four columns a row
+    const int64_t row0 = static_cast<int64_t>(tp) * 256 + rank * 128, col0 = static_cast<int64_t>(tq) * 256 + per0 * 4;
+    auto sum = [&](auto splits) {
+      constexpr int S = decltype(splits)::value, kThreads = (2 + kPairEpilogueWarps) * 32;
+      constexpr int kGroups = 16 / S;  // a thread's sixteen loads in flight: other CTAs' memory is far away
+      for (int g0 = static_cast<int>(threadIdx.x); g0 < 128 * per; g0 += kGroups * kThreads) {
+        float4 x[kGroups][S];
+#pragma unroll
+        for (int u = 0; u < kGroups; ++u) {
+          const int g = g0 + u * kThreads, i = g / per;
+          const uint32_t off = ring + static_cast<uint32_t>(i * kPartRow + (per0 + g - i * per) * 4) * 4u;
+          if (g < 128 * per) {
+#pragma unroll
+            for (int k = 0; k < S; ++k) x[u][k] = ld_cluster_v4(map_to_rank(off, 2 * k + rank));
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kGroups; ++u) {
+          const int g = g0 + u * kThreads, i = g / per, j = (g - i * per) * 4;
+          if (g >= 128 * per || row0 + i >= p.rows_p || col0 + j >= p.rows_q) continue;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < S; ++k) {
+            v.x += x[u][k].x;
+            v.y += x[u][k].y;
+            v.z += x[u][k].z;
+            v.w += x[u][k].w;
+          }
+          uint16_t* o = static_cast<uint16_t*>(p.out) + (row0 + i) * p.ldc + col0 + j;
+          const uint2 w = make_uint2(cvt2(v.x * alpha, v.y * alpha, p.out_bf16), cvt2(v.z * alpha, v.w * alpha, p.out_bf16));
+          store_four(o, w, p.vec, static_cast<int>(min(static_cast<int64_t>(4), p.rows_q - col0 - j)));
+        }
+      }
+    };
+    if (p.split == 2) sum(std::integral_constant<int, 2>{});
+    else sum(std::integral_constant<int, 3>{});
+    __syncwarp();
+    cluster_sync();
+  }
   if (warp == 1) tmem_dealloc_pair(tmem, p.tmem_cols);
 }
 
@@ -646,12 +707,22 @@ int splits(int64_t tiles, int num_kb) {
 }
 
 // Pairs, unless a side fits one 128-row tile, or there are so few 128 x 128 tiles that single CTAs split K over the GPU
-// and K is long enough to gain by it. Measured, pairs against single CTAs (us): nvfp4 512x4096x4096 (no split) 11.0, 13.6;
-// 256x28672x4096 22.1, 30.3; 256x4096x4096 (two splits of 16 stages) 10.6, 9.9; 256x4096x14336 23.9, 15.7; 1024^3 (two
+// and K is long enough to gain by it. Measured, pairs against single CTAs (us): nvfp4 512x4096x4096 (no split) 10.9, 13.6;
+// 256x28672x4096 22.1, 30.3; 256x4096x4096 (two splits of 16 stages) 10.6, 9.0; 256x4096x14336 17.3, 14.2; 1024^3 (two
 // splits of 4 stages) 6.2, 7.6; mxfp8 512x2048x2048 (of 16) 9.9, 9.2; 1024^3 (of 8) 7.2, 8.0.
 bool use_pairs(int64_t M, int64_t N, int num_kb) {
   if (M <= 128 || N <= 128) return false;
   return num_kb <= 8 || splits(ceil_div(M, 128) * ceil_div(N, 128), num_kb) == 1;
+}
+
+// K splits of a product of `tiles` pairs' tiles: the pairs of one cluster, while every cluster is resident at once. Adding
+// the parts through distributed shared memory takes 4-5 us, the time of some 18 stages, so that many have to be saved (four splits never do: so few tiles have single CTAs split K):
+// 512x4096x14336 (two splits) nvfp4 23.9 -> 20.0 us, mxfp8 40.0 -> 29.7; at K = 4096 nvfp4 10.9 -> 12.9.
+int pair_splits(int64_t tiles, int num_kb) {
+  int split = 1;
+  for (int s = 2; s <= 3; ++s)
+    if (tiles <= kClusters[2 * s] && num_kb * (s - 1) >= 18 * s) split = s;
+  return split;
 }
 
 struct Plan {
@@ -683,6 +754,8 @@ int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b
   pl.N = b->rows;
   pl.kind = a->format;
   pl.empty = pl.M == 0 || pl.N == 0;
+  if (pl.M > INT32_MAX - 512 || pl.N > INT32_MAX - 512)
+    return record_error(B2G_ERR_UNSUPPORTED, "dimension_too_large: a product needs M and N < 2^31 - 512");
   pl.zero = a->cols == 0;
   if (pl.empty) return B2G_OK;
   if (!C || ldc < pl.N) return record_error(B2G_ERR_INVALID_ARG, "null C or ldc below N");
@@ -718,8 +791,8 @@ int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b
     if (tiles > kMaxGrid / 2) return too_large("product");
     p.units = static_cast<int32_t>(tiles);
     p.group = 16;
-    p.split = 1;
-    pl.grid = 2 * (tiles < kPairs ? static_cast<int>(tiles) : kPairs);
+    p.split = pair_splits(tiles, p.num_kb);
+    pl.grid = 2 * p.split * (tiles < kPairs ? static_cast<int>(tiles) : kPairs);
     p.q_bytes = 128u * 128u;
     const uint32_t cta_bytes = 2u * 128u * 128u + 512u * T * 3;
     p.tx_bytes = 2u * cta_bytes;
@@ -802,7 +875,7 @@ int32_t plan_launch(const Plan& pl, cudaStream_t st) {
   lc.gridDim = dim3(static_cast<unsigned>(pl.grid), 1, 1);
   lc.blockDim = dim3(pl.pair ? (2 + kPairEpilogueWarps) * 32 : 192, 1, 1);
   lc.dynamicSmemBytes = pl.smem;
-  const int cluster = pl.pair ? 2 : pl.p.split;
+  const int cluster = pl.pair ? 2 * pl.p.split : pl.p.split;
   if (cluster > 1) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);

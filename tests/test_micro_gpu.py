@@ -158,7 +158,8 @@ def check_product(c: torch.Tensor, a: np.ndarray, b: np.ndarray):
 
 PRODUCTS = [(1, 1, 1), (1, 128, 256), (1, 1000, 4096), (7, 130, 96), (16, 4096, 33), (17, 257, 500), (33, 96, 1031),
             (64, 512, 2048), (65, 127, 64), (128, 384, 640), (129, 129, 129), (200, 1024, 300), (300, 264, 1500),
-            (5, 8, 14336), (512, 640, 256), (1024, 768, 320), (1000, 1111, 777)]
+            (5, 8, 14336), (512, 640, 256), (1024, 768, 320), (1000, 1111, 777),
+            (513, 2050, 9300), (510, 2431, 7001)]  # the last two: K split over two and three CTA pairs of a cluster
 
 
 @pytest.mark.parametrize("dtype", HALF)
