@@ -7,12 +7,14 @@ For every shape of a suite, on one GPU, with one timing protocol (cold L2, CUDA 
   * `lt`    cuBLASLt's heuristic top-`lt_n`, each validated and timed: `lt0` = rank 0 (B2), `lt_best` = best (B3);
             with `--lt-deep-s S`, also the fastest configs of a budgeted search of cuBLASLt's configuration space
             (`cublaslt_deep`, S seconds per shape in a child process): `lt_best` is then B3+;
-  * `torch` torch.matmul (B1).
+  * `torch` torch.matmul (B1);
+  * with `--micro mxfp8,nvfp4`: the same layer in microscaled formats (`cs464_b200.micro`), `<format>_us` the product of
+            operands that are quantised already and `<format>_quantize_us` quantising A, in the same protocol.
 The row's `gap_sel_vs_lt` = sel / lt_best - 1 and `gap_sel_vs_best` = sel / best - 1 (the reference's regret,
 results/README.md:79); the summary gives their median and p95.
 
     python -m cs464_b200.compare --suite config3 [--limit N] [--k 3] [--space 0] [--lt-n 16] [--lt-deep-s 5]
-                                 [--out rows.jsonl]
+                                 [--micro FORMAT,...] [--out rows.jsonl]
 """
 from __future__ import annotations
 
@@ -39,8 +41,16 @@ def _time(backend, a, b) -> float:
     return measure_us(backend.make_runner(a, b), FULL, keep_samples=False).trimmed_us
 
 
+def _time_micro(fmt: str, a, b) -> dict:
+    """The product of a and b in a microscaled format, and what quantising a costs each call (b is a layer's weights)."""
+    from cs464_b200 import micro
+    qa, qb = micro.quantize(a, fmt), micro.quantize(b.t(), fmt)
+    return {f"{fmt}_us": _time(micro.MicroMatmul(a.dtype), qa, qb),
+            f"{fmt}_quantize_us": measure_us(lambda: micro.quantize(a, fmt), FULL, keep_samples=False).trimmed_us}
+
+
 def compare_shape(shape: dict, *, k: int = 3, space: int = 0, lt_n: int = 16, ranker=None, lt_deep_s: float = 0.0,
-                  deep_cache: str = "lt_deep_cache") -> dict:
+                  deep_cache: str = "lt_deep_cache", micro: tuple = ()) -> dict:
     M, N, K = shape["M"], shape["N"], shape["K"]
     dtype = torch.float16
     a, b = make_inputs(M, N, K, dtype, scale_b=shape.get("weight_std", 1.0))
@@ -85,6 +95,9 @@ def compare_shape(shape: dict, *, k: int = 3, space: int = 0, lt_n: int = 16, ra
         row["lt_best_us"] = min(t for _, t in lts)
         row["lt_n_valid"] = len(lts)
     row["torch_us"] = _time(TorchMatmul(), a, b)
+    for fmt in micro:
+        row.update(_time_micro(fmt, a, b))
+        row[f"{fmt}_tflops"] = flops / row[f"{fmt}_us"] / 1e6
     for name in ("sel", "best", "lt_best", "torch"):
         t = row.get(f"{name}_us")
         if t:
@@ -122,6 +135,7 @@ def main(argv=None) -> dict:
     ap.add_argument("--lt-n", type=int, default=16)
     ap.add_argument("--lt-deep-s", type=float, default=0.0, help="cuBLASLt configuration search budget per shape")
     ap.add_argument("--deep-cache", default="lt_deep_cache")
+    ap.add_argument("--micro", default="", help="microscaled formats to time too: mxfp8, mxfp4, nvfp4, comma-separated")
     ap.add_argument("--out", default=None)
     a = ap.parse_args(argv)
     shapes = suites.load(a.suite)[: a.limit]
@@ -131,7 +145,8 @@ def main(argv=None) -> dict:
                                             budget_s=a.lt_deep_s)
     rows = []
     for s in shapes:
-        r = compare_shape(s, k=a.k, space=a.space, lt_n=a.lt_n, lt_deep_s=a.lt_deep_s, deep_cache=a.deep_cache)
+        r = compare_shape(s, k=a.k, space=a.space, lt_n=a.lt_n, lt_deep_s=a.lt_deep_s, deep_cache=a.deep_cache,
+                          micro=tuple(f for f in a.micro.split(",") if f))
         rows.append(r)
         print(json.dumps(r), flush=True)
         if a.out:

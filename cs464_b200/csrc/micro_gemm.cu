@@ -291,21 +291,33 @@ __global__ void __launch_bounds__(192, 1)
     const int g1 = groups * (split + 1) / p.split;
     uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(tq) * p.tile_q * p.ldc + static_cast<int64_t>(tp) * 128;
     const int rows = p.rows_p - tp * 128;  // the tile's rows inside C^T
-    for (int g = groups * split / p.split + static_cast<int>(threadIdx.x); g < g1; g += 192) {
-      const int j = g >> 5, i = (g & 31) * 4;
-      if (i >= rows) continue;
-      const uint32_t off = ring + (j * 132 + i) * 4u;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int g0 = groups * split / p.split + static_cast<int>(threadIdx.x); g0 < g1; g0 += 2 * 192) {  // two at a time
+      float4 v[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int s = 0; s < p.split; ++s) {
-        const float4 x = ld_cluster_v4(p.split > 1 ? map_to_rank(off, s) : off);
-        v.x += x.x;
-        v.y += x.y;
-        v.z += x.z;
-        v.w += x.w;
+        float4 x[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int g = min(g0 + u * 192, g1 - 1);
+          const uint32_t off = ring + ((g >> 5) * 132 + (g & 31) * 4) * 4u;
+          x[u] = ld_cluster_v4(p.split > 1 ? map_to_rank(off, s) : off);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          v[u].x += x[u].x;
+          v[u].y += x[u].y;
+          v[u].z += x[u].z;
+          v[u].w += x[u].w;
+        }
       }
-      uint16_t* o = out + j * p.ldc + i;
-      const uint2 w = make_uint2(cvt2(v.x * alpha, v.y * alpha, p.out_bf16), cvt2(v.z * alpha, v.w * alpha, p.out_bf16));
-      store_four(o, w, p.vec, rows - i);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int g = g0 + u * 192, j = g >> 5, i = (g & 31) * 4;
+        if (g >= g1 || i >= rows) continue;
+        const uint2 w = make_uint2(cvt2(v[u].x * alpha, v[u].y * alpha, p.out_bf16), cvt2(v[u].z * alpha, v[u].w * alpha, p.out_bf16));
+        store_four(out + j * p.ldc + i, w, p.vec, rows - i);
+      }
     }
   }
   __syncwarp();
@@ -708,7 +720,7 @@ int splits(int64_t tiles, int num_kb) {
 
 // Pairs, unless a side fits one 128-row tile, or there are so few 128 x 128 tiles that single CTAs split K over the GPU
 // and K is long enough to gain by it. Measured, pairs against single CTAs (us): nvfp4 512x4096x4096 (no split) 10.9, 13.6;
-// 256x28672x4096 22.1, 30.3; 256x4096x4096 (two splits of 16 stages) 10.6, 9.0; 256x4096x14336 17.3, 14.2; 1024^3 (two
+// 256x28672x4096 22.1, 30.3; 256x4096x4096 (two splits of 16 stages) 10.6, 9.5; 256x4096x14336 17.3, 15.4; 1024^3 (two
 // splits of 4 stages) 6.2, 7.6; mxfp8 512x2048x2048 (of 16) 9.9, 9.2; 1024^3 (of 8) 7.2, 8.0.
 bool use_pairs(int64_t M, int64_t N, int num_kb) {
   if (M <= 128 || N <= 128) return false;

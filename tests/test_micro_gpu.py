@@ -676,6 +676,30 @@ def test_two_products_at_once():
     micro.check_status()
 
 
+def test_compare_times_the_formats():
+    """compare.py's --micro: the product and the quantisation of a row-major problem in the callers' timing protocol."""
+    from cs464_b200.compare import _time_micro
+    from cs464_b200.gate import make_inputs
+    a, b = make_inputs(64, 384, 512)
+    for fmt in FORMATS:
+        row = _time_micro(fmt, a, b)
+        assert set(row) == {f"{fmt}_us", f"{fmt}_quantize_us"} and all(0 < v < 1e4 for v in row.values())
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second GPU")
+def test_tensors_of_another_device_than_the_current_one():
+    x = normal(40, 256).to("cuda:1")
+    w = normal(96, 256, seed=1).to("cuda:1")
+    with torch.cuda.device(0):
+        c = micro.micro_matmul(micro.quantize(x, "nvfp4"), micro.quantize(w, "nvfp4"))
+        y, _ = micro.rms_norm(x, w[0])
+    with torch.cuda.device(1):
+        assert torch.equal(c, micro.micro_matmul(micro.quantize(x, "nvfp4"), micro.quantize(w, "nvfp4")))
+        assert torch.equal(y, micro.rms_norm(x, w[0])[0])
+    with pytest.raises(ValueError, match="is on cuda:0"):
+        micro.rms_norm(x, normal(256))
+
+
 def test_offsets_past_32_bits():
     """Rows that lie more than 2^31 values into their buffers (6 GB at most here): first and last rows against the same
     rows quantised alone."""
