@@ -169,6 +169,16 @@ __global__ void __launch_bounds__(192, 1)
   const int kb0 = static_cast<int>(static_cast<int64_t>(split) * p.num_kb / p.split);
   const int kb1 = static_cast<int>(static_cast<int64_t>(split + 1) * p.num_kb / p.split);
 
+  // Stage `s` of the ring from K block `kb`, by one thread.
+  auto load_stage = [&](int s, int kb) {
+    const uint32_t full = ctl + O_FULL + 8 * s, base = ring + s * p.stage_bytes;
+    mbar_arrive_expect_tx(full, p.tx_bytes);
+    tma_load_2d(base, &map_p, full, kb * 128, tp * 128);
+    tma_load_2d(base + kPBytes, &map_q, full, kb * 128, tq * p.tile_q);
+    tma_load_3d(base + kPBytes + p.q_bytes, &map_sp, full, 0, kb * tiles_of(KIND), tp);
+    tma_load_3d(base + kPBytes + p.q_bytes + kTileBytes, &map_sq, full, 0, kb * tiles_of(KIND), tq * p.tile_q / 128);
+  };
+
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&map_p);
     tma_prefetch_desc(&map_q);
@@ -182,6 +192,9 @@ __global__ void __launch_bounds__(192, 1)
     mbar_init(ctl + O_DRAIN, 1);
     *abort_flag = 0u;
     fence_mbar_init();
+    // The first stage goes out while warp 1 allocates tensor memory (one stage: more would hold up the block's barrier).
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    load_stage(0, kb0);  // every split has a K block
   }
   if (warp == 1) {
     tmem_alloc(ctl + O_TMEM, p.tmem_cols);
@@ -195,22 +208,17 @@ __global__ void __launch_bounds__(192, 1)
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + O_TMEM);
 
   if (warp == 0) {
-    if (lane == 0) {  // TMA producer
-      int s = 0, issued = 0;
+    if (lane == 0) {  // TMA producer; the first stage is under way
+      int s = 1, issued = 1;
       uint32_t ph = 0;
       bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const uint32_t empty = ctl + O_EMPTY + 8 * s, full = ctl + O_FULL + 8 * s;
+      for (int kb = kb0 + 1; kb < kb1; ++kb) {
+        const uint32_t empty = ctl + O_EMPTY + 8 * s;
         if (!mbar_try_wait(empty, ph ^ 1u) && !wait_phase(empty, ph ^ 1u, abort_flag, p.status, kProducerTimeout)) {
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(full, p.tx_bytes);
-        const uint32_t base = ring + s * p.stage_bytes;
-        tma_load_2d(base, &map_p, full, kb * 128, tp * 128);
-        tma_load_2d(base + kPBytes, &map_q, full, kb * 128, tq * p.tile_q);
-        tma_load_3d(base + kPBytes + p.q_bytes, &map_sp, full, 0, kb * tiles_of(KIND), tp);
-        tma_load_3d(base + kPBytes + p.q_bytes + kTileBytes, &map_sq, full, 0, kb * tiles_of(KIND), tq * p.tile_q / 128);
+        load_stage(s, kb);
         ++issued;
         if (++s == p.stages) {
           s = 0;
@@ -253,29 +261,26 @@ __global__ void __launch_bounds__(192, 1)
         ph ^= 1u;
       }
     }
-    if (ok && kb1 > kb0) umma_commit_w(ctl + O_TFULL);
+    if (ok) umma_commit_w(ctl + O_TFULL);
     umma_commit_w(ctl + O_DRAIN);
     drain_phase(ctl + O_DRAIN, 0, ok ? kWaitNs : kDrainNs);
   } else {
     // Epilogue, part one: this split's fp32 tile into shared memory as [column j][row i] (128 + 4 floats a column: 32
     // lanes store 32 consecutive words). The ring is free: every MMA has completed.
     const int q = warp & 3;
-    const bool some = kb1 > kb0;
-    if (!some || wait_phase(ctl + O_TFULL, 0u, abort_flag, p.status, kEpilogueTimeout)) {
+    if (wait_phase(ctl + O_TFULL, 0u, abort_flag, p.status, kEpilogueTimeout)) {
       tc_fence_after();
       const int i = q * 32 + lane;
       for (int c = 0; c < p.tile_q; c += 32) {
         const int n = min(32, p.tile_q - c);
         uint32_t v[32];
-        if (some) {
-          const uint32_t at = tmem + c + (static_cast<uint32_t>(q * 32) << 16);
-          if (n == 32) tmem_ld_32cols(at, v);
-          else tmem_ld_16cols(at, v);
-          tmem_ld_wait();
-        }
+        const uint32_t at = tmem + c + (static_cast<uint32_t>(q * 32) << 16);
+        if (n == 32) tmem_ld_32cols(at, v);
+        else tmem_ld_16cols(at, v);
+        tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (j < n) st_shared_u32(ring + ((c + j) * 132 + i) * 4u, some ? v[j] : 0u);
+          if (j < n) st_shared_u32(ring + ((c + j) * 132 + i) * 4u, v[j]);
       }
     }
   }
