@@ -228,14 +228,14 @@ __device__ __forceinline__ Raw8<float> pack8<float>(const float (&v)[8]) {
 }
 
 // How a row's values lie. kVec: unit column stride, 16-byte aligned rows and a multiple of 8 columns, so that eight
-// columns exist or do not and are one or two 16-byte accesses. kUnit: unit column stride, any alignment and width: a warp
-// moves 32 consecutive values an instruction and shared memory turns them to eight a lane (through strided scalars an odd
-// width ran at a fifth of an even one's rate). kAny: any strides, a value at a time.
+// columns exist or do not and are one or two 16-byte accesses. kUnit: unit column stride, any alignment and width: a
+// warp moves 32 consecutive values an instruction and shared memory turns them to eight a lane (through strided
+// scalars an odd width ran at a fifth of an even one's rate). kAny: any strides, a value at a time.
 enum Mode : int { kVec = 0, kUnit = 1, kAny = 2 };
 
 // A lane's eight columns c .. c+7 on their way from a row, columns at or past `cols` zero: `fetch` issues the loads,
-// `settle` gives the values. In kUnit both are called by a converged warp whose lanes hold 256 consecutive columns, with a
-// scratch of 256 values of the warp's own.
+// `settle` gives the values. In kUnit both are called by a converged warp whose lanes hold 256 consecutive columns,
+// with a scratch of 256 values of the warp's own.
 template <typename T, int MODE>
 struct Frag {
   Raw8<T> r;
@@ -348,10 +348,10 @@ __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7fffffffu) : byte ? __uint_as_float(byte << 23) : __uint_as_float(0x00400000u);
 }
 
-// Bits of the largest magnitude among eight values, as an fp32's; at least 0x7f800000 where an infinity or a NaN is among
-// them. The integer pipe is what bounds the quantising kernels, so 16-bit values are compared as they lie, two at a time
-// (magnitudes order as their bits do), and fp32 values by a maximum that takes the magnitude on the way, with a product
-// by zero on the otherwise idle multiply-add pipe to catch what is not finite.
+// Bits of the largest magnitude among eight values, as an fp32's; at least 0x7f800000 where an infinity or a NaN is
+// among them. The integer pipe is what bounds the quantising kernels, so 16-bit values are compared as they lie, two
+// at a time (magnitudes order as their bits do), and fp32 values by a maximum that takes the magnitude on the way,
+// with a product by zero on the otherwise idle multiply-add pipe to catch what is not finite.
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   uint32_t m;
   asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
@@ -391,9 +391,9 @@ __device__ __forceinline__ uint32_t amax8(const Raw8<float>& r) {
 //   estimate corrected by its residual (Markstein, "Computation of elementary functions on the IBM RISC System/6000
 //   processor", 1990). The residual is taken negated, so that zeros keep the value's sign. A block whose scale rounds to
 //   zero is zero.
-// The codes of a NaN block are cleared by `keep`.
-// NVFP4's tensor scale g as a thread uses it: 6 g and its reciprocal, once, so that a block's scale amax / (6 g) is three
-// operations of the same kind. (Below 2^-60 the residual would leave fp32's range: the division is done as such.)
+// The codes of a NaN block are cleared by `keep`. NVFP4's tensor scale g as a thread uses it: 6 g and its reciprocal,
+// once, so that a block's scale amax / (6 g) is three operations of the same kind. (Below 2^-60 the residual would
+// leave fp32's range: the division is done as such.)
 struct TensorScale {
   float g, six, inv;
   __device__ __forceinline__ explicit TensorScale(float scale) : g(scale), six(6.f * scale), inv(1.f / (6.f * scale)) {}
@@ -449,7 +449,8 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return r;
 }
 
-// Eight e2m1 codes, the lowest value in the lowest bits: four conversions of two values to a byte and one packing move.
+// Eight e2m1 codes, the lowest value in the lowest bits: four conversions of two values to a byte and one packing
+// move.
 __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
   uint32_t r;
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
@@ -474,8 +475,8 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], const BlockQuant<FM
   else return make_uint2(e2m1x8(s) & b.keep, 0u);
 }
 
-// Where a lane's eight columns of a row go: eight consecutive columns per lane, the warp's 32 lanes holding 256 of one row
-// (lane 0's first, a multiple of 256 past the row's start).
+// Where a lane's eight columns of a row go: eight consecutive columns per lane, the warp's 32 lanes holding 256 of one
+// row (lane 0's first, a multiple of 256 past the row's start).
 template <int FMT>
 struct CodePlace {
   uint8_t* codes;   // the lane's codes in the row
@@ -492,8 +493,9 @@ struct CodePlace {
   }
 };
 
-// Quantise them. `m`: the eight values' amax8. A block's lanes (4 for blocks of 32, 2 for 16) share their largest magnitude
-// by shuffles; the four scale bytes of one tile row are gathered into one 4-byte store. Called by a converged warp.
+// Quantise them. `m`: the eight values' amax8. A block's lanes (4 for blocks of 32, 2 for 16) share their largest
+// magnitude by shuffles; the four scale bytes of one tile row are gathered into one 4-byte store. Called by a
+// converged warp.
 template <int FMT>
 __device__ __forceinline__ void quantize_store(const float (&v)[8], uint32_t m, int lane, const CodePlace<FMT>& to,
                                                const TensorScale& ts) {

@@ -1,14 +1,19 @@
-// micro_gemm.cu — products of two microscaled tensors on the block-scaled tensor-core kinds: C[M,N] = A[M,K] * B[N,K]^T.
+// micro_gemm.cu — products of two microscaled tensors on the block-scaled tensor-core kinds: C[M,N] = A[M,K] *
+// B[N,K]^T.
 //
 // Both operands lie as codes with K contiguous and scales in the order the tensor core reads them, so nothing is
 // converted on the way: TMA brings 128 bytes of codes a row (256 columns of 4 bits, 128 of 8) and the scale tiles that
-// belong to them into a ring of shared-memory stages, tcgen05.cp moves the scales on into tensor memory (a region of its
-// own for every stage, free once the stage's MMAs have completed), and four block-scaled MMAs of 32 bytes of K multiply
-// the stage into fp32 accumulators. Two kernels:
+// belong to them into a ring of shared-memory stages, tcgen05.cp moves the scales on into tensor memory (a region of
+// its own for every stage, free once the stage's MMAs have completed), and four block-scaled MMAs of 32 bytes of K
+// multiply the stage into fp32 accumulators. Two kernels:
 //   product_kernel       one CTA per 128 x tile_q tile and K split; the MMA's 128 rows run over B's rows (a layer's
 //                        weights), its narrow side over A's (the tokens), so a few tokens cost a narrow tile. The K
 //                        splits of a tile are one thread-block cluster and are summed through distributed shared memory.
 //   product_pair_kernel  CTA pairs (cta_group::2) of 256 x 256 tiles for products with many of them.
+// Measured: nvfp4 1x28672x4096 13.8 us (4.8 TB/s: the weights' bytes and 3 us of launch, first loads and epilogue bound
+// it), 128x4096x14336 12.2 us; 8192x28672x4096 nvfp4 390 us (4.9 PFLOP/s), mxfp4 366 us (5.3), mxfp8 690 us (2.8).
+// With its loads, scales or stores left out the last shape's nvfp4 time falls by some 100, 55 and 45 us: the MMAs alone take
+// 244 us, and shared memory's bandwidth, which they share with the copies in and out, is what is between.
 // Every wait is bounded as in b2g_gemm.cu: on expiry the status word gets a code and the CTA drains and returns.
 
 #include <cuda.h>
@@ -76,7 +81,8 @@ __device__ __noinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile 
 
 // The same for a converged warp, which goes on with one answer: the votes make it, and with it every loop counter and
 // descriptor of the warp's loop, uniform in the compiler's eyes. Operands of tcgen05 instructions come from uniform
-// registers; from per-thread ones each costs a move of tens of cycles, and the issue, not the tensor core, sets the pace.
+// registers; from per-thread ones each costs a move of tens of cycles, and the issue, not the tensor core, sets the
+// pace.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int* status, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   const uint64_t t0 = global_timer_ns();
@@ -126,9 +132,9 @@ __device__ __forceinline__ void store_four(uint16_t* o, uint2 w, bool vec, int n
   }
 }
 
-// Issue one stage: its scales into tensor memory, then up to four MMAs (fewer where K ends inside the stage: codes past
-// K are zero but the scales there may be any bytes). `sp`, `sq`, `cp`, `cq`: shared addresses of P's and Q's codes and of
-// their scales.
+// Issue one stage: its scales into tensor memory, then up to four MMAs (fewer where K ends inside the stage: codes
+// past K are zero but the scales there may be any bytes). `sp`, `sq`, `cp`, `cq`: shared addresses of P's and Q's
+// codes and of their scales.
 template <int KIND, int PAIR>
 __device__ __forceinline__ void issue_stage(uint32_t d, uint64_t p_desc, uint64_t q_desc, uint32_t cp, uint32_t cq,
                                             uint32_t tmem_scales, int q_tiles, const uint32_t (&idesc)[kStepsPerStage],
@@ -192,7 +198,8 @@ __global__ void __launch_bounds__(192, 1)
     mbar_init(ctl + O_DRAIN, 1);
     *abort_flag = 0u;
     fence_mbar_init();
-    // The first stage goes out while warp 1 allocates tensor memory (one stage: more would hold up the block's barrier).
+    // The first stage goes out while warp 1 allocates tensor memory (one stage: more would hold up the block's
+    // barrier).
     asm volatile("griddepcontrol.wait;" ::: "memory");
     load_stage(0, kb0);  // every split has a K block
   }
@@ -285,7 +292,8 @@ __global__ void __launch_bounds__(192, 1)
     }
   }
   // Part two: CTA r of the cluster adds its share of the tile over the cluster's CTAs in split order, scales, converts
-  // and stores, a lane four consecutive values (a warp's loads of other CTAs' memory are whole lines that way). Every thread of every CTA reaches both barriers.
+  // and stores, a lane four consecutive values (a warp's loads of other CTAs' memory are whole lines that way). Every
+  // thread of every CTA reaches both barriers.
   __syncwarp();
   if (p.split > 1) cluster_sync();
   else __syncthreads();
@@ -336,8 +344,8 @@ constexpr int kPairEpilogueWarps = 8;
 constexpr uint32_t kPairStaging = kPairEpilogueWarps * 4096u;
 constexpr int kPartRow = 256 + 4;  // floats a row of a split's part in shared memory
 
-// Tile `t` of the pairs' walk: bands of `group` tile rows, inside a band down the rows first, so that the tiles that run
-// at one time share operands in L2.
+// Tile `t` of the pairs' walk: bands of `group` tile rows, inside a band down the rows first, so that the tiles that
+// run at one time share operands in L2.
 __device__ __forceinline__ void pair_tile(const Params& p, int t, int& tp, int& tq) {
   const int band = p.group * p.tiles_q;
   const int g = t / band, r = t - g * band;
@@ -346,11 +354,12 @@ __device__ __forceinline__ void pair_tile(const Params& p, int t, int& tp, int& 
   tp = g * p.group + (r - tq * h);
 }
 
-// 256 x 256 tiles, a persistent CTA pair on each (or, with K split, the pairs of a cluster on one tile, a K range each): every CTA loads its 128 rows of P, half of Q's 256 and the scales of
-// its P rows and of all of Q (both tensor memories hold Q's scales), the leader issues MMAs of M = 256, and each CTA ends
-// with a 128 x 256 accumulator. 256 accumulator columns and the stages' scales fill tensor memory, so there is one
-// accumulator: the epilogue's eight warps read it into registers and free it before they convert the second half and
-// store, while the next tile's MMAs run.
+// 256 x 256 tiles, a persistent CTA pair on each (or, with K split, the pairs of a cluster on one tile, a K range
+// each): every CTA loads its 128 rows of P, half of Q's 256 and the scales of its P rows and of all of Q (both tensor
+// memories hold Q's scales), the leader issues MMAs of M = 256, and each CTA ends with a 128 x 256 accumulator. 256
+// accumulator columns and the stages' scales fill tensor memory, so there is one accumulator: the epilogue's eight
+// warps read it into registers and free it before they convert the second half and store, while the next tile's MMAs
+// run.
 template <int KIND>
 __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
     product_pair_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap map_p,
@@ -530,8 +539,8 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
       const int64_t row0 = static_cast<int64_t>(tp) * 256 + rank * 128 + q * 32;
       const int64_t col0 = static_cast<int64_t>(tq) * 256 + half * 128;
       if (p.vec) {
-        // 32 rows x 64 columns at a time through the warp's 4 KB of shared memory (16-byte pieces XOR-ed by the row, the
-        // 128-byte swizzle) and out by TMA, which writes whole lines and drops what lies outside C
+        // 32 rows x 64 columns at a time through the warp's 4 KB of shared memory (16-byte pieces XOR-ed by the row,
+        // the 128-byte swizzle) and out by TMA, which writes whole lines and drops what lies outside C
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (lane == 0) tma_store_wait_read();  // the last store has read the buffer
@@ -570,8 +579,8 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
   __syncwarp();
   cluster_sync();  // the pair's MMAs and signals are done in both CTAs; the splits' parts lie in shared memory
   if (p.split > 1) {
-    // Each CTA adds its share of the columns of its 128 rows over the splits, in split order, from the CTAs of its rank in
-    // every pair; the rows were stored 4 floats apart in banks. Then the cluster's shared memory may go.
+    // Each CTA adds its share of the columns of its 128 rows over the splits, in split order, from the CTAs of its
+    // rank in every pair; the rows were stored 4 floats apart in banks. Then the cluster's shared memory may go.
     int tp, tq;
     pair_tile(p, first, tp, tq);
     const float alpha = p.scale_a ? *p.scale_a * *p.scale_b : 1.f;
@@ -637,8 +646,8 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-// Codes as rows of bytes: boxes of 128 bytes x `box_rows` rows, 128-byte swizzle. What lies past a row's last code byte
-// reads as zero.
+// Codes as rows of bytes: boxes of 128 bytes x `box_rows` rows, 128-byte swizzle. What lies past a row's last code
+// byte reads as zero.
 int32_t encode_codes(CUtensorMap* map, const b2g_micro_tensor* t, int box_rows) {
   const EncodeFn fn = encode_fn();
   if (!fn) return record_error(B2G_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
@@ -714,8 +723,8 @@ constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
 
 constexpr int kPairs = 74;  // CTA pairs resident at once
 
-// K splits of a single-CTA product of `tiles` tiles: one cluster a tile, as many splits as keep every cluster resident at
-// once and leave each split two stages.
+// K splits of a single-CTA product of `tiles` tiles: one cluster a tile, as many splits as keep every cluster resident
+// at once and leave each split two stages.
 int splits(int64_t tiles, int num_kb) {
   int split = 1;
   for (int s = 2; s <= 8; ++s)
@@ -723,18 +732,19 @@ int splits(int64_t tiles, int num_kb) {
   return split;
 }
 
-// Pairs, unless a side fits one 128-row tile, or there are so few 128 x 128 tiles that single CTAs split K over the GPU
-// and K is long enough to gain by it. Measured, pairs against single CTAs (us): nvfp4 512x4096x4096 (no split) 10.9, 13.6;
-// 256x28672x4096 22.1, 30.3; 256x4096x4096 (two splits of 16 stages) 10.6, 9.5; 256x4096x14336 17.3, 15.4; 1024^3 (two
-// splits of 4 stages) 6.2, 7.6; mxfp8 512x2048x2048 (of 16) 9.9, 9.2; 1024^3 (of 8) 7.2, 8.0.
+// Pairs, unless a side fits one 128-row tile, or there are so few 128 x 128 tiles that single CTAs split K over the
+// GPU and K is long enough to gain by it. Measured, pairs against single CTAs (us): nvfp4 512x4096x4096 (no split)
+// 10.9, 13.6; 256x28672x4096 22.1, 30.3; 256x4096x4096 (two splits of 16 stages) 10.6, 9.5; 256x4096x14336 17.3, 15.4;
+// 1024^3 (two splits of 4 stages) 6.2, 7.6; mxfp8 512x2048x2048 (of 16) 9.9, 9.2; 1024^3 (of 8) 7.2, 8.0.
 bool use_pairs(int64_t M, int64_t N, int num_kb) {
   if (M <= 128 || N <= 128) return false;
   return num_kb <= 8 || splits(ceil_div(M, 128) * ceil_div(N, 128), num_kb) == 1;
 }
 
-// K splits of a product of `tiles` pairs' tiles: the pairs of one cluster, while every cluster is resident at once. Adding
-// the parts through distributed shared memory takes 4-5 us, the time of some 18 stages, so that many have to be saved (four splits never do: so few tiles have single CTAs split K):
-// 512x4096x14336 (two splits) nvfp4 23.9 -> 20.0 us, mxfp8 40.0 -> 29.7; at K = 4096 nvfp4 10.9 -> 12.9.
+// K splits of a product of `tiles` pairs' tiles: the pairs of one cluster, while every cluster is resident at once.
+// Adding the parts through distributed shared memory takes 4-5 us, the time of some 18 stages, so that many have to be
+// saved (four splits never do: so few tiles have single CTAs split K): 512x4096x14336 (two splits) nvfp4 23.9 -> 20.0
+// us, mxfp8 40.0 -> 29.7; at K = 4096 nvfp4 10.9 -> 12.9.
 int pair_splits(int64_t tiles, int num_kb) {
   int split = 1;
   for (int s = 2; s <= 3; ++s)
@@ -845,9 +855,9 @@ int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b
   p.tx_bytes = 128u * 128u + p.q_bytes + 512u * T * (1 + p.q_tiles);
   p.stage_bytes = (p.tx_bytes + 1023u) & ~1023u;
   p.acc_cols = pow2_cols(p.tile_q);
-  // Shared memory: clusters take a whole SM's each, so that no CTA of another launch can hold tensor memory there while
-  // this cluster's CTAs wait for one another; single CTAs take at most half, two to an SM, and at most half of the
-  // tensor memory.
+  // Shared memory: clusters take a whole SM's each, so that no CTA of another launch can hold tensor memory there
+  // while this cluster's CTAs wait for one another; single CTAs take at most half, two to an SM, and at most half of
+  // the tensor memory.
   const uint32_t room = p.split > 1 ? kMaxSmem : 113u * 1024u;
   const uint32_t cols = tiles_of(pl.kind) * 4u * (1u + p.q_tiles);
   uint32_t stages = (room - 2048u) / p.stage_bytes;

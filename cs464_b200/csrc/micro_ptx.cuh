@@ -6,11 +6,11 @@
 
 namespace b2g {
 
-// D[tmem] (+)= (A * scale A) * (B * scale B), A and B from shared memory, scales from tensor memory, fp32 accumulators.
-// KIND 1: 8-bit floats, K = 32, one power-of-two scale per row (kind::mxf8f6f4); 2: e2m1, K = 64, two power-of-two
-// scales per row (kind::mxf4); 3: e2m1, K = 64, four e4m3 scales per row (kind::mxf4nvf4). Issued by lane 0 of a
-// converged warp. `a`, `b`: the descriptors' low words; `hi`: the high word both share (what varies between stages and K
-// steps is the start address, so only one word is computed).
+// D[tmem] (+)= (A * scale A) * (B * scale B), A and B from shared memory, scales from tensor memory, fp32
+// accumulators. KIND 1: 8-bit floats, K = 32, one power-of-two scale per row (kind::mxf8f6f4); 2: e2m1, K = 64, two
+// power-of-two scales per row (kind::mxf4); 3: e2m1, K = 64, four e4m3 scales per row (kind::mxf4nvf4). Issued by lane
+// 0 of a converged warp. `a`, `b`: the descriptors' low words; `hi`: the high word both share (what varies between
+// stages and K steps is the start address, so only one word is computed).
 template <int KIND, int PAIR>
 __device__ __forceinline__ void umma_scaled_w(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t sa,
                                               uint32_t sb, uint32_t accumulate) {
@@ -38,8 +38,8 @@ __device__ __forceinline__ void umma_scaled_w(uint32_t d, uint32_t a, uint32_t b
 #undef B2G_UMMA_SCALED
 }
 
-// A 512-byte scale tile (32 rows of 16 bytes) at shared address `from` into four tensor-memory columns, repeated in each
-// quarter of the lanes. The descriptor has no swizzle: 8-row groups of 16 bytes a row, 128 bytes apart.
+// A 512-byte scale tile (32 rows of 16 bytes) at shared address `from` into four tensor-memory columns, repeated in
+// each quarter of the lanes. The descriptor has no swizzle: 8-row groups of 16 bytes a row, 128 bytes apart.
 template <int PAIR>
 __device__ __forceinline__ void scales_to_tmem_w(uint32_t tmem, uint32_t from) {
 #define B2G_SCALE_COPY(GROUP)                                                           \
