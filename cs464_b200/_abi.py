@@ -37,7 +37,8 @@ EXPORTS = (
 # every symbol include/b2g_micro.h declares
 MICRO_EXPORTS = (
     "b2g_micro_layout", "b2g_micro_tensor_scale", "b2g_micro_quantize", "b2g_micro_dequantize", "b2g_micro_plan_create",
-    "b2g_micro_plan_launch", "b2g_micro_plan_destroy", "b2g_micro_matmul", "b2g_micro_rms_norm",
+    "b2g_micro_plan_launch", "b2g_micro_plan_destroy", "b2g_micro_matmul", "b2g_micro_matmul_values_workspace",
+    "b2g_micro_matmul_values", "b2g_micro_rms_norm",
     "b2g_micro_rms_norm_workspace", "b2g_micro_rms_norm_backward", "b2g_micro_silu_mul", "b2g_micro_silu_mul_backward",
 )
 
@@ -134,6 +135,9 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b2g_micro_plan_launch": (c_int32, [c_void_p, c_void_p]),
         "b2g_micro_plan_destroy": (c_int32, [c_void_p]),
         "b2g_micro_matmul": (c_int32, [mt, mt, c_void_p, i64, c_int32, c_void_p, c_void_p]),
+        "b2g_micro_matmul_values_workspace": (c_int32, [c_int32, i64, i64, i64, P(c_size_t)]),
+        "b2g_micro_matmul_values": (c_int32, [mm, mm, i64, i64, i64, c_int32, c_int32, c_void_p, i64, c_int32, c_void_p,
+                                              c_size_t, c_void_p, c_void_p]),
         "b2g_micro_rms_norm": (c_int32, [mm, mm, c_void_p, mm, mm, mt, i64, i64, ctypes.c_float, c_int32, c_void_p]),
         "b2g_micro_rms_norm_workspace": (c_int32, [i64, i64, P(c_size_t)]),
         "b2g_micro_rms_norm_backward": (c_int32, [mm, mm, c_void_p, mm, mm, c_void_p, c_void_p, c_size_t, i64, i64,

@@ -786,7 +786,9 @@ int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b
   pl.zero = a->cols == 0;
   if (pl.empty) return B2G_OK;
   if (!C || ldc < pl.N) return record_error(B2G_ERR_INVALID_ARG, "null C or ldc below N");
-  if (cudaGetDevice(&pl.device) != cudaSuccess) {
+  // Encoding tensor maps needs the device's context bound to this thread, which a thread that has not used the runtime
+  // yet (autograd's own, for one) does not have; naming its current device binds it.
+  if (cudaGetDevice(&pl.device) != cudaSuccess || cudaSetDevice(pl.device) != cudaSuccess) {
     cudaGetLastError();
     return record_error(B2G_ERR_CUDA, "no CUDA device");
   }
@@ -922,6 +924,35 @@ int32_t plan_launch(const Plan& pl, cudaStream_t st) {
   return record_error(B2G_ERR_CUDA, std::string("product launch: ") + cudaGetErrorString(e));
 }
 
+// Where the quantised operands of a product of values lie in its workspace: A's tensor scale, B's, then codes and scales
+// of each. Every part is a multiple of 16 bytes.
+struct ValuesLayout {
+  b2g_micro_tensor a, b;
+  size_t bytes;
+};
+
+ValuesLayout values_layout(int fmt, int64_t M, int64_t N, int64_t K, uint8_t* base) {
+  ValuesLayout l;
+  size_t at = 32;
+  const auto place = [&](int64_t rows, size_t scale_at) {
+    b2g_micro_tensor t = {};
+    t.format = fmt;
+    t.rows = rows;
+    t.cols = K;
+    t.pitch = min_pitch(fmt, K);
+    t.codes = base + at;
+    at += static_cast<size_t>(rows * t.pitch);
+    t.scales = base + at;
+    at += static_cast<size_t>(ceil_div(rows, 128) * ceil_div(K, 4 * block_of(fmt)) * 512);
+    t.scale = fmt == FMT_NVFP4 ? reinterpret_cast<const float*>(base + scale_at) : nullptr;
+    return t;
+  };
+  l.a = place(M, 0);
+  l.b = place(N, 16);
+  l.bytes = at;
+  return l;
+}
+
 }  // namespace micro
 }  // namespace b2g
 
@@ -968,6 +999,41 @@ int32_t b2g_micro_matmul(const b2g_micro_tensor* a, const b2g_micro_tensor* b, v
   return guarded([&]() -> int32_t {
     Plan pl;
     if (const int32_t rc = plan_init(pl, a, b, C, ldc, dtype, status)) return rc;
+    return plan_launch(pl, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int32_t b2g_micro_matmul_values_workspace(int32_t format, int64_t M, int64_t N, int64_t K, size_t* bytes) {
+  return guarded([&]() -> int32_t {
+    if (format < FMT_MXFP8 || format > FMT_NVFP4 || M < 0 || N < 0 || K < 0 || !bytes)
+      return record_error(B2G_ERR_INVALID_ARG, "matmul_values_workspace: bad format, dimension or output pointer");
+    *bytes = values_layout(format, M, N, K, nullptr).bytes;
+    return B2G_OK;
+  });
+}
+
+int32_t b2g_micro_matmul_values(const b2g_micro_matrix* A, const b2g_micro_matrix* B, int64_t M, int64_t N, int64_t K,
+                                int32_t value_dtype, int32_t format, void* C, int64_t ldc, int32_t dtype,
+                                void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  return guarded([&]() -> int32_t {
+    if (format < FMT_MXFP8 || format > FMT_NVFP4 || M < 0 || N < 0 || K < 0)
+      return record_error(B2G_ERR_INVALID_ARG, "matmul_values: bad format or dimension");
+    const ValuesLayout l = values_layout(format, M, N, K, static_cast<uint8_t*>(workspace));
+    if (!workspace || !aligned16(workspace) || workspace_bytes < l.bytes)
+      return record_error(B2G_ERR_WORKSPACE, "matmul_values: workspace missing, misaligned or too small");
+    Plan pl;  // checks everything before the first launch
+    if (const int32_t rc = plan_init(pl, &l.a, &l.b, C, ldc, dtype, status)) return rc;
+    if (!pl.empty && !pl.zero) {
+      const b2g_micro_matrix* values[] = {A, B};
+      const b2g_micro_tensor* to[] = {&l.a, &l.b};
+      for (int i = 0; i < 2; ++i) {
+        if (format == FMT_NVFP4)
+          if (const int32_t rc = b2g_micro_tensor_scale(values[i], to[i]->rows, K, value_dtype,
+                                                        const_cast<float*>(to[i]->scale), stream))
+            return rc;
+        if (const int32_t rc = b2g_micro_quantize(values[i], value_dtype, to[i], stream)) return rc;
+      }
+    }
     return plan_launch(pl, static_cast<cudaStream_t>(stream));
   });
 }

@@ -60,6 +60,7 @@ class _Entry:
     """The entry points that enqueue work, bound with plain pointers for the structures, on first use."""
 
     _ARGS = {"tensor_scale": "pqqipp", "quantize": "pipp", "dequantize": "ppip", "matmul": "pppqipp", "plan_launch": "pp",
+             "matmul_values": "ppqqqiipqipzpp",
              "rms_norm": "ppppppqqfip", "rms_norm_backward": "pppppppzqqfip", "silu_mul": "pppqqip",
              "silu_mul_backward": "pppqqip"}
     _KIND = {"p": ctypes.c_void_p, "q": ctypes.c_int64, "i": ctypes.c_int32, "f": ctypes.c_float, "z": ctypes.c_size_t}
@@ -380,12 +381,25 @@ class MicroMatmul:
         return _MicroRunner(plan, c, status, (a, b))
 
 
+def _values_product(a: torch.Tensor, b: torch.Tensor, fmt: int) -> torch.Tensor:
+    """q(a) @ q(b).T of matrices of values, in their type: quantize and micro_matmul in one call."""
+    M, K = a.shape
+    N = b.shape[0]
+    c = a.new_empty((M, N))
+    pitch, a_scales = _layout(fmt, M, K)
+    n = 32 + (M + N) * pitch + a_scales + _layout(fmt, N, K)[1]  # b2g_micro_matmul_values_workspace
+    ws, index, kind = _new_bytes(n, a), a.get_device(), _HALF[a.dtype]
+    _call(index, _entry.matmul_values, _matrix(a), _matrix(b), M, N, K, kind, fmt, c.data_ptr(), max(N, 1), kind,
+          ws.data_ptr(), n, _status(index))
+    return c
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, fmt):
         ctx.save_for_backward(x, w)
         ctx.fmt = fmt
-        return micro_matmul(quantize(x, fmt), quantize(w, fmt), dtype=x.dtype)
+        return _values_product(x, w, fmt)
 
     @staticmethod
     @once_differentiable
@@ -393,9 +407,9 @@ class _Linear(torch.autograd.Function):
         x, w = ctx.saved_tensors
         fmt, dx, dw = ctx.fmt, None, None
         if ctx.needs_input_grad[0]:
-            dx = micro_matmul(quantize(dy, fmt), quantize(w.t(), fmt), dtype=x.dtype)
+            dx = _values_product(dy, w.t(), fmt)
         if ctx.needs_input_grad[1]:
-            dw = micro_matmul(quantize(dy.t(), fmt), quantize(x.t(), fmt), dtype=w.dtype)
+            dw = _values_product(dy.t(), x.t(), fmt)
         return dx, dw, None
 
 
@@ -403,12 +417,12 @@ def micro_linear(x: torch.Tensor, w: torch.Tensor, format: str = "mxfp8") -> tor
     """x [..., K] @ w [N, K].T (fp16 or bf16, one type), differentiable, in a format: y = q(x) q(w)^T, and with the
     gradient passed through the quantisations dx = q(dy) q(w^T)^T and dw = q(dy^T) q(x^T)^T. Each product's operands are
     quantised along the dimension it sums over, so the backward pass quantises x, w and dy anew from their values."""
-    _format(format)
+    fmt = _format(format)
     _check(x, "x", _HALF)
     _check(w, "w", (x.dtype,), x)
     if w.ndim != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"x must be [..., K] and w [N, K], not {tuple(x.shape)} and {tuple(w.shape)}")
-    y = _Linear.apply(_rows(x), w, format)
+    y = _Linear.apply(_rows(x), w, fmt)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.shape[0])
 
 

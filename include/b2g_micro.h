@@ -82,6 +82,15 @@ int32_t b2g_micro_plan_destroy(b2g_micro_plan* plan);
 int32_t b2g_micro_matmul(const b2g_micro_tensor* a, const b2g_micro_tensor* b, void* C, int64_t ldc, int32_t dtype,
                          int32_t* status, void* stream);
 
+/* Product of two matrices of values, quantised on the way: C[M, N] = q(A)[M, K] * q(B)[N, K]^T, A and B of any strides and
+   one type, NVFP4 with the scales of b2g_micro_tensor_scale. What quantize and matmul give one after the other, in one
+   call; the quantised operands lie in `workspace`, b2g_micro_matmul_values_workspace() bytes of device memory, 16-byte
+   aligned, any contents. */
+int32_t b2g_micro_matmul_values_workspace(int32_t format, int64_t M, int64_t N, int64_t K, size_t* bytes);
+int32_t b2g_micro_matmul_values(const b2g_micro_matrix* A, const b2g_micro_matrix* B, int64_t M, int64_t N, int64_t K,
+                                int32_t value_dtype, int32_t format, void* C, int64_t ldc, int32_t dtype,
+                                void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
 /* h = x + residual (x alone where residual is NULL); y = h * weight / sqrt(mean(h^2) + eps) by rows of `cols`. The norm
    is taken of the fp32 sum, before h is rounded. Outputs: h (NULL: not wanted), and either y (values) or q (a
    microscaled tensor). x, residual, weight, h and y share `dtype` (F16 or BF16); weight is contiguous. */

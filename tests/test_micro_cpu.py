@@ -93,6 +93,12 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.b2g_micro_silu_mul_backward(mat, None, mat, 4, 64, 1, None) == inv
     assert lib.b2g_micro_tensor_scale(mat, 4, 64, 1, None, None) == inv
     n = ctypes.c_size_t()
+    assert lib.b2g_micro_matmul_values_workspace(3, 130, 5, 70, ctypes.byref(n)) == 0
+    assert n.value == 32 + 135 * micro._layout(3, 1, 70)[0] + micro._layout(3, 130, 70)[1] + micro._layout(3, 5, 70)[1]
+    assert lib.b2g_micro_matmul_values_workspace(0, 4, 4, 4, ctypes.byref(n)) == inv
+    assert lib.b2g_micro_matmul_values(mat, mat, 4, 4, 4, 1, 1, 4096, 4, 1, None, 0, None, None) == _abi.B2G_ERR_WORKSPACE
+    assert lib.b2g_micro_matmul_values(mat, mat, 4, 4, 4, 1, 1, 4096, 3, 1, 4096, 1 << 20, None, None) == inv
+    assert lib.b2g_micro_matmul_values(mat, mat, 4, 4, 4, 1, 7, 4096, 4, 1, 4096, 1 << 20, None, None) == inv
     assert lib.b2g_micro_rms_norm_workspace(4, 64, ctypes.byref(n)) == 0 and n.value >= 64 * 4  # an fp32 row at least
     assert lib.b2g_micro_rms_norm_workspace(-1, 64, ctypes.byref(n)) == inv
 

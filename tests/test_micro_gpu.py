@@ -658,6 +658,27 @@ def test_capture_replay_and_streams():
     micro.check_status()
 
 
+def test_product_as_a_threads_first_call():
+    """Threads that have not used CUDA yet (autograd's, a server's workers) build tensor maps too."""
+    import threading
+    (qa, a), (qb, b) = random_operand(40, 300, "nvfp4", 1), random_operand(70, 300, "nvfp4", 2)
+    micro.micro_matmul(qa, qb)
+    got = []
+
+    def work():
+        got.append(micro.micro_matmul(qa, qb))
+        got.append(micro.MicroMatmul().make_runner(qa, qb)())
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 6
+    for c in got:
+        check_product(c, a, b)
+
+
 def test_two_products_at_once():
     """Products on two streams at the same time, K split over clusters in both."""
     ops = [(random_operand(m, 4096, fmt, i), random_operand(1000, 4096, fmt, i + 9)) for i, (m, fmt) in
