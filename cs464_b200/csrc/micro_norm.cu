@@ -14,6 +14,7 @@ namespace micro {
 
 constexpr int kMostRounds = 4;
 constexpr int kMaxThreads = 512;  // per row, and per block where that is more than 128
+constexpr int64_t kMostCols = (int64_t(1) << 31) - 8192;
 
 // Blocks of kMaxThreads an SM holds at once, by rounds held in registers.
 constexpr int blocks_per_sm(int rounds) { return rounds <= 2 ? 2 : 1; }
@@ -42,7 +43,7 @@ __device__ __forceinline__ float2 row_sum(float2 v, int tpr, float2 (*part)[32],
 }
 
 // FMT_NONE writes values (y), the formats write q; rows from `rows` to the end of their 128-row scale tile get zero
-// scales. RES: h = x + residual, else h = x. Columns fit 31 bits.
+// scales. RES: h = x + residual, else h = x. Columns, counted on to the end of a round, fit 31 bits (kMostCols).
 template <typename T, int FMT, bool RES, int MODE, int ROUNDS>
 __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
     norm_kernel(Mat x, Mat res, const T* w, T* h, int64_t shr, int64_t shc, T* y, int64_t syr, int64_t syc, Quant q,
@@ -395,6 +396,7 @@ int32_t b2g_micro_rms_norm(const b2g_micro_matrix* x, const b2g_micro_matrix* re
       if (const int32_t rc = check_tensor(q, "q")) return rc;
       if (q->rows != rows || q->cols != cols) return record_error(B2G_ERR_INVALID_ARG, "rms_norm: q is not [rows, cols]");
     }
+    if (cols > kMostCols) return too_large("rms_norm");
     if (rows == 0 || cols == 0) return B2G_OK;
     if (const int32_t rc = check_matrix(x, "x")) return rc;
     if (residual)
@@ -455,6 +457,7 @@ int32_t b2g_micro_rms_norm_backward(const b2g_micro_matrix* dy, const b2g_micro_
   return guarded([&]() -> int32_t {
     if (rows < 0 || cols < 0 || (dtype != B2G_VALUE_F16 && dtype != B2G_VALUE_BF16))
       return record_error(B2G_ERR_INVALID_ARG, "rms_norm_backward: bad dimension or dtype");
+    if (cols > kMostCols) return too_large("rms_norm_backward");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (cols == 0) return B2G_OK;
     if (!dweight || !weight) return record_error(B2G_ERR_INVALID_ARG, "null weight or dweight");

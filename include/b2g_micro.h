@@ -93,7 +93,8 @@ int32_t b2g_micro_matmul_values(const b2g_micro_matrix* A, const b2g_micro_matri
 
 /* h = x + residual (x alone where residual is NULL); y = h * weight / sqrt(mean(h^2) + eps) by rows of `cols`. The norm
    is taken of the fp32 sum, before h is rounded. Outputs: h (NULL: not wanted), and either y (values) or q (a
-   microscaled tensor). x, residual, weight, h and y share `dtype` (F16 or BF16); weight is contiguous. */
+   microscaled tensor). x, residual, weight, h and y share `dtype` (F16 or BF16); weight is contiguous; cols is at most
+   2^31 - 8192. */
 int32_t b2g_micro_rms_norm(const b2g_micro_matrix* x, const b2g_micro_matrix* residual, const void* weight,
                            const b2g_micro_matrix* h, const b2g_micro_matrix* y, const b2g_micro_tensor* q, int64_t rows,
                            int64_t cols, float eps, int32_t dtype, void* stream);

@@ -103,6 +103,17 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.b2g_micro_rms_norm_workspace(-1, 64, ctypes.byref(n)) == inv
 
 
+def test_norm_refuses_columns_past_its_counters():
+    """A row's columns are counted in 31 bits, a round of up to 4096 past its end included."""
+    lib = _abi.load()
+    for cols in (2 ** 31 - 8191, 2 ** 31 - 200, 2 ** 31, 2 ** 32 + 64):
+        mat = _abi.MicroMatrix(4096, cols, 1)
+        assert lib.b2g_micro_rms_norm(mat, mat, 4096, mat, mat, None, 1, cols, 1e-5, 1, None) == _abi.B2G_ERR_UNSUPPORTED
+        assert _abi.last_error().startswith("dimension_too_large")
+        assert lib.b2g_micro_rms_norm_backward(mat, mat, 4096, None, mat, 4096, 4096, 1 << 50, 1, cols, 1e-5, 1,
+                                               None) == _abi.B2G_ERR_UNSUPPORTED
+
+
 def test_empty_calls_do_nothing():
     lib = _abi.load()
     e = _tensor(rows=0, codes=None, scales=None)
