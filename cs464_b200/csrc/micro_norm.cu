@@ -392,6 +392,7 @@ int32_t b2g_micro_rms_norm(const b2g_micro_matrix* x, const b2g_micro_matrix* re
   return guarded([&]() -> int32_t {
     if (rows < 0 || cols < 0 || (dtype != B2G_VALUE_F16 && dtype != B2G_VALUE_BF16) || (!y && !q) || (y && q))
       return record_error(B2G_ERR_INVALID_ARG, "rms_norm: bad dimension or dtype, or not one output");
+    if (h && !residual) return record_error(B2G_ERR_INVALID_ARG, "rms_norm: without a residual h is x itself, pass NULL");
     if (q) {
       if (const int32_t rc = check_tensor(q, "q")) return rc;
       if (q->rows != rows || q->cols != cols) return record_error(B2G_ERR_INVALID_ARG, "rms_norm: q is not [rows, cols]");

@@ -5,7 +5,7 @@
  * Conventions, return codes and error texts are those of b2g.h: device pointers are raw CUDA addresses on the current
  * device, `stream` is a cudaStream_t, every function returns B2G_OK or a negative B2G_ERR_* code with
  * b2g_last_error() text, and nothing here allocates device memory or synchronises, so every call can be captured into
- * a CUDA graph. No state is kept between calls.
+ * a CUDA graph. No state is kept between calls. An output overlaps no input and no other output.
  *
  * A microscaled tensor [rows, cols] is quantised in blocks of consecutive columns (the dimension a product sums over):
  *   MXFP8  e4m3 codes, one power-of-two scale (a biased exponent byte, 255 = NaN) per 32 columns
@@ -92,7 +92,8 @@ int32_t b2g_micro_matmul_values(const b2g_micro_matrix* A, const b2g_micro_matri
                                 void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /* h = x + residual (x alone where residual is NULL); y = h * weight / sqrt(mean(h^2) + eps) by rows of `cols`. The norm
-   is taken of the fp32 sum, before h is rounded. Outputs: h (NULL: not wanted), and either y (values) or q (a
+   is taken of the fp32 sum, before h is rounded. Outputs: h (NULL: not wanted; without a residual it is x itself and has
+   to be NULL), and either y (values) or q (a
    microscaled tensor). x, residual, weight, h and y share `dtype` (F16 or BF16); weight is contiguous; cols is at most
    2^31 - 8192. */
 int32_t b2g_micro_rms_norm(const b2g_micro_matrix* x, const b2g_micro_matrix* residual, const void* weight,

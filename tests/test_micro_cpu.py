@@ -85,6 +85,7 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.b2g_micro_plan_launch(None, None) == inv and lib.b2g_micro_plan_destroy(None) == 0
     assert lib.b2g_micro_rms_norm(mat, None, 4096, None, mat, a, 4, 64, 1e-5, 1, None) == inv   # two outputs
     assert lib.b2g_micro_rms_norm(mat, None, 4096, None, None, None, 4, 64, 1e-5, 1, None) == inv
+    assert lib.b2g_micro_rms_norm(mat, None, 4096, mat, mat, None, 4, 64, 1e-5, 1, None) == inv  # h without a residual
     assert lib.b2g_micro_rms_norm(mat, None, 4096, None, None, a, 5, 64, 1e-5, 1, None) == inv  # q of other rows
     assert lib.b2g_micro_rms_norm(mat, None, 4096, None, mat, None, 4, 64, 1e-5, 2, None) == inv
     assert lib.b2g_micro_rms_norm_backward(mat, mat, 4096, None, mat, 4096, 4096, 0, 4, 64, 1e-5, 1,
