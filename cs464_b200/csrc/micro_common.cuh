@@ -398,9 +398,10 @@ struct TensorScale {
   float g, six, inv;
   __device__ __forceinline__ explicit TensorScale(float scale) : g(scale), six(6.f * scale), inv(1.f / (6.f * scale)) {}
   __device__ __forceinline__ float block(float amax) const {
-    if (g < 8.67361738e-19f) return amax / six;
-    const float q = amax * inv;
-    return fmaf(-fmaf(q, six, -amax), inv, q);
+    const float a = fminf(amax, 448.f * six);  // past it the scale saturates, and the quotient may leave fp32's range
+    if (g < 8.67361738e-19f) return a / six;
+    const float q = a * inv;
+    return fmaf(-fmaf(q, six, -a), inv, q);
   }
 };
 
@@ -469,7 +470,16 @@ template <int FMT>
 __device__ __forceinline__ uint2 codes8(const float (&v)[8], const BlockQuant<FMT>& b) {
   float s[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = b.scaled(v[i]);
+  for (int i = 0; i < 8; ++i) s[i] = v[i];
+  if constexpr (FMT == FMT_NVFP4) {
+    if (b.byte == 0x7eu) {  // the largest scale: values past 6 u saturate, and their quotients may leave fp32's range
+      const float top = 8.f * b.unit;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = fminf(fmaxf(s[i], -top), top);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = b.scaled(s[i]);
   if constexpr (FMT == FMT_MXFP8)
     return make_uint2(e4m3x4(s[0], s[1], s[2], s[3]) & b.keep, e4m3x4(s[4], s[5], s[6], s[7]) & b.keep);
   else return make_uint2(e2m1x8(s) & b.keep, 0u);

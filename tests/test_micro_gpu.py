@@ -139,6 +139,22 @@ def test_dequantize(fmt, dtype):
 
 
 # ---------------------------------------------------------------- products
+@pytest.mark.parametrize("dtype", ALL)
+def test_nvfp4_saturates_whatever_the_quotient(dtype):
+    """Values whose quotient by the given scale leaves fp32's range (a mask's lowest value, say) saturate like others past
+    2688 times it; the rest of their block is what the definition gives. Powers of two, so that nothing rounds but the
+    codes."""
+    info = torch.finfo(dtype)
+    for g in (2.0 ** -100, 2.0 ** -58, 2.0 ** -20, 2.0 ** -3, 1.0):
+        x = normal(70, 200, dtype=dtype, seed=5, std=min(700.0 * g, 100.0))
+        x[:, 3] = info.min
+        x[1::2, 77] = info.max
+        x[2, 100:120] = info.min
+        for t in (x, x.t().contiguous().t(), x[:, :199]):
+            q = micro.quantize(t, "nvfp4", scale=torch.full((1,), g, device="cuda"))
+            check_quantized(q, f64(t))
+
+
 def random_operand(rows, cols, fmt, seed, std=1.0):
     q = micro.quantize(normal(rows, cols, dtype=torch.float32, seed=seed, std=std), fmt)
     g = None if q.scale is None else float(q.scale)
