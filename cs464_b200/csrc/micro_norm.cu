@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kMaxThreads, backward_blocks_per_sm(ROUNDS))
     s = row_sum(s, tpr, part, buf);
     buf ^= 1;
     const float r = rsqrtf(s.x / n + eps);
-    const float rm = r * r * r * (s.y / n);  // dx = r * dy * w - h * rm
+    const float rm = s.y / n * r * r * r;  // dx = r * dy * w - h * rm; r^3 alone may leave fp32's range where rm does not
 #pragma unroll
     for (int k = 0; k < ROUNDS; ++k) {
       const int c = k * width + t * 8;

@@ -426,6 +426,21 @@ def test_norm_backward(dtype):
             assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
 
 
+@pytest.mark.parametrize("size", [1e-9, 1e9, 1e13, 1e15, 1e16])
+def test_norm_backward_of_large_and_small_rows(size):
+    """Rows whose 1 / norm cubed leaves fp32's range; the squares' sum does not (64 columns of up to 5e16: below 2e35).
+    Bounds as in test_norm_backward. dweight's terms are of the size of dy."""
+    dy, w = normal(33, 64, seed=1), normal(64, seed=2)
+    h = (normal(33, 64, dtype=torch.float32, seed=3) * size).bfloat16()
+    dx, dw = micro.rms_norm_backward(dy, h, w, 1e-5)
+    a, b, c = f64(dy), f64(h), f64(w)
+    rx, rw, r = norm_grad64(a, b, c, 1e-5)
+    mag = np.abs(a * c) * r + np.abs(b) * r ** 3 * np.abs(a * b * c).mean(1, keepdims=True)
+    assert (np.abs(f64(dx) - rx) <= half_step(torch.bfloat16) * np.abs(rx) + 2.0 ** -18 * (mag + np.abs(rx))).all()
+    tol = half_step(torch.bfloat16) * np.abs(rw) + (2.0 ** -18 + 33 * 2.0 ** -24) * np.abs(a * b * r).sum(0)
+    assert (np.abs(f64(dw) - rw) <= tol).all()
+
+
 def test_norm_gradient_formula_against_differences():
     """The formula the gradients are tested against, by central differences of the 64-bit forward pass."""
     rng = np.random.default_rng(0)
