@@ -111,8 +111,18 @@ __device__ __forceinline__ uint32_t cvt2(float a, float b, int bf16) {
   return bf16 ? pack_pair(a, b, static_cast<__nv_bfloat16*>(nullptr)) : pack_pair(a, b, static_cast<__half*>(nullptr));
 }
 
-__device__ __forceinline__ uint16_t cvt1(float a, int bf16) {
-  return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(a)) : __half_as_ushort(__float2half_rn(a));
+// Both tensor scales as two factors for the accumulators. One large and one small scale are multiplied beforehand; two
+// of one kind are applied one after the other, since their product may leave fp32's range where a result does not (and
+// a zero times an infinity is none).
+__device__ __forceinline__ float2 output_scale(const Params& p) {
+  if (!p.scale_a) return make_float2(1.f, 1.f);
+  const float a = *p.scale_a, b = *p.scale_b;
+  return (a < 1.f) == (b < 1.f) ? make_float2(a, b) : make_float2(a * b, 1.f);
+}
+
+// Two accumulators as two values of C.
+__device__ __forceinline__ uint32_t result2(float a, float b, float2 scale, int bf16) {
+  return cvt2(a * scale.x * scale.y, b * scale.x * scale.y, bf16);
 }
 
 // Scales of stage columns in tensor memory: P's tiles first (4 columns each), then Q's, K tile by K tile.
@@ -298,7 +308,7 @@ __global__ void __launch_bounds__(192, 1)
   if (p.split > 1) cluster_sync();
   else __syncthreads();
   {
-    const float alpha = p.scale_a ? *p.scale_a * *p.scale_b : 1.f;
+    const float2 alpha = output_scale(p);
     const int cols = min(p.tile_q, p.rows_q - tq * p.tile_q);  // columns of the tile inside C^T
     const int groups = cols * 32;  // of four values
     const int g1 = groups * (split + 1) / p.split;
@@ -328,7 +338,7 @@ __global__ void __launch_bounds__(192, 1)
       for (int u = 0; u < 2; ++u) {
         const int g = g0 + u * 192, j = g >> 5, i = (g & 31) * 4;
         if (g >= g1 || i >= rows) continue;
-        const uint2 w = make_uint2(cvt2(v[u].x * alpha, v[u].y * alpha, p.out_bf16), cvt2(v[u].z * alpha, v[u].w * alpha, p.out_bf16));
+        const uint2 w = make_uint2(result2(v[u].x, v[u].y, alpha, p.out_bf16), result2(v[u].z, v[u].w, alpha, p.out_bf16));
         store_four(out + j * p.ldc + i, w, p.vec, rows - i);
       }
     }
@@ -494,7 +504,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
     const int e = warp - 2, q = warp & 3, half = e >> 2;  // tensor-memory lane quarter, half of the columns
     const uint32_t tempty = map_to_rank(ctl + O_TEMPTY, lead);
     const uint32_t stg = ring + p.stages * p.stage_bytes + static_cast<uint32_t>(e) * 4096u;
-    const float alpha = p.scale_a ? *p.scale_a * *p.scale_b : 1.f;
+    const float2 alpha = output_scale(p);
     uint16_t* out = static_cast<uint16_t*>(p.out);
     uint32_t ph = 0;
     for (int t = first; t < p.units; t += step) {
@@ -534,7 +544,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             w[h * 32 + c * 16 + j] =
-                cvt2(__uint_as_float(v[c][2 * j]) * alpha, __uint_as_float(v[c][2 * j + 1]) * alpha, p.out_bf16);
+                result2(__uint_as_float(v[c][2 * j]), __uint_as_float(v[c][2 * j + 1]), alpha, p.out_bf16);
       }
       const int64_t row0 = static_cast<int64_t>(tp) * 256 + rank * 128 + q * 32;
       const int64_t col0 = static_cast<int64_t>(tq) * 256 + half * 128;
@@ -583,7 +593,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
     // rank in every pair; the rows were stored 4 floats apart in banks. Then the cluster's shared memory may go.
     int tp, tq;
     pair_tile(p, first, tp, tq);
-    const float alpha = p.scale_a ? *p.scale_a * *p.scale_b : 1.f;
+    const float2 alpha = output_scale(p);
     const int per0 = 64 * split / p.split, per = 64 * (split + 1) / p.split - per0;  // groups of four columns a row
     const int64_t row0 = static_cast<int64_t>(tp) * 256 + rank * 128, col0 = static_cast<int64_t>(tq) * 256 + per0 * 4;
     auto sum = [&](auto splits) {
@@ -613,7 +623,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
             v.w += x[u][k].w;
           }
           uint16_t* o = static_cast<uint16_t*>(p.out) + (row0 + i) * p.ldc + col0 + j;
-          const uint2 w = make_uint2(cvt2(v.x * alpha, v.y * alpha, p.out_bf16), cvt2(v.z * alpha, v.w * alpha, p.out_bf16));
+          const uint2 w = make_uint2(result2(v.x, v.y, alpha, p.out_bf16), result2(v.z, v.w, alpha, p.out_bf16));
           store_four(o, w, p.vec, static_cast<int>(min(static_cast<int64_t>(4), p.rows_q - col0 - j)));
         }
       }

@@ -216,6 +216,25 @@ def test_product_llama_layers(layer):
     micro.check_status()
 
 
+@pytest.mark.parametrize("shape", [(5, 130, 96), (130, 130, 96), (300, 264, 1500), (513, 2050, 9300)])
+def test_product_of_large_and_small_tensor_scales(shape):
+    """Tensor scales whose product leaves fp32's range while results do not: tiny operands, and huge ones with zero rows
+    and columns (0, where 0 times an infinity would be NaN)."""
+    M, N, K = shape
+    a, b = normal(M, K, dtype=torch.float32, seed=1), normal(N, K, dtype=torch.float32, seed=2)
+    for sa, sb in ((2.0 ** -70, 2.0 ** -60), (2.0 ** 90, 2.0 ** -90), (2.0 ** -20, 2.0 ** 110)):
+        qa, qb = micro.quantize(a * sa, "nvfp4"), micro.quantize(b * sb, "nvfp4")
+        va, vb = (om.values(*stored(q), "nvfp4", float(q.scale)) for q in (qa, qb))
+        c = micro.micro_matmul(qa, qb)
+        ref, size = va @ vb.T, np.abs(va) @ np.abs(vb).T
+        # as check_product, one scaling more; bf16's smallest subnormal is 2^-133
+        bound = half_step(c.dtype) * np.abs(ref) + (-(-K // 32) + 10) * 2.0 ** -22 * size + 2.0 ** -134
+        assert (np.abs(f64(c) - ref) <= bound).all(), (sa, sb)
+    a[M // 2:], b[N // 2:] = 0, 0
+    c = f64(micro.micro_matmul(micro.quantize(a * 2.0 ** 90, "nvfp4"), micro.quantize(b * 2.0 ** 90, "nvfp4")))
+    assert (c[M // 2:] == 0).all() and (c[:, N // 2:] == 0).all() and np.isinf(c[:M // 2, :N // 2]).any()
+
+
 def test_product_of_nan_blocks_stays_in_its_rows():
     """A NaN scale makes its own row (or column) of the product NaN and nothing else, in every format."""
     for fmt in FORMATS:
