@@ -100,10 +100,13 @@ struct ValueSource {
   }
 };
 
-// 1 / (1 + exp(-x)), the exponential and the division in their fast forms: their errors (2 + 1.173 |x| and 2 ulps) are
-// far below the rounding of any output type where the result is not itself negligible. Where exp(-x) passes 2^126 the
-// result is 0.
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// 1 / (1 + exp(-x)) and 1 / (1 + exp(x)) from e = exp(-|x|), which is at most one: nothing overflows, and both keep their
+// digits however small they are. Exponential and division are the fast forms: their errors (2 + 1.173 |x| and 2 ulps)
+// are below the rounding of any output type.
+__device__ __forceinline__ float2 sigmoids(float x) {
+  const float e = __expf(-fabsf(x)), inv = __fdividef(1.f, 1.f + e);
+  return x >= 0.f ? make_float2(inv, e * inv) : make_float2(e * inv, inv);
+}
 
 template <typename T>
 struct GateSource {
@@ -113,7 +116,7 @@ struct GateSource {
     unpack8(r[0], g);
     unpack8(r[1], u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = g[i] * sigmoid(g[i]) * u[i];
+    for (int i = 0; i < 8; ++i) v[i] = g[i] * sigmoids(g[i]).x * u[i];
     return amax8(v);
   }
 };
@@ -380,10 +383,9 @@ __global__ void __launch_bounds__(256)
   unpack8(rd, d);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float e = __expf(-fabsf(g[i])), inv = __fdividef(1.f, 1.f + e);  // e <= 1: nothing overflows
-    const float s = g[i] >= 0.f ? inv : e * inv, t = g[i] >= 0.f ? e * inv : inv;  // sigmoid(g), sigmoid(-g)
-    dg[i] = d[i] * u[i] * s * (1.f + g[i] * t);
-    du[i] = d[i] * g[i] * s;
+    const float2 s = sigmoids(g[i]);
+    dg[i] = d[i] * u[i] * s.x * (1.f + g[i] * s.y);
+    du[i] = d[i] * g[i] * s.x;
   }
   T* o = dx + row * sxr;
   store8<T, MODE>(o, sxc, c, cols, pack8<T>(dg), scratch);

@@ -594,6 +594,15 @@ def test_gate_extremes():
     assert micro.silu_mul(x[:0]).shape == (0, 12) and micro.silu_mul(x.view(1, 1, 24)).shape == (1, 1, 12)
 
 
+def test_gate_of_very_negative_gates():
+    """Gates down to -88, where the sigmoid (6e-39 and up) is among fp32's subnormals, against large values: the
+    exponential errs by 2 + 1.173 * 88 ulps, of at most 2^-149 / 6e-39 < 2^-21.9 of the value: below 2^-15 in all."""
+    g = torch.linspace(-88.0, -60.0, 113).bfloat16().cuda().expand(3, -1)
+    x = torch.cat([g, torch.full_like(g, 1e30)], 1)
+    ref = gate64(f64(x))
+    assert (np.abs(f64(micro.silu_mul(x)) - ref) <= (half_step(torch.bfloat16) + 2.0 ** -15) * np.abs(ref)).all()
+
+
 def test_gate_gradient_formula_against_differences():
     rng = np.random.default_rng(0)
     x, dy, e = rng.normal(size=(2, 12)) * 2, rng.normal(size=(2, 6)), 1e-6
