@@ -10,8 +10,9 @@
 //                        weights), its narrow side over A's (the tokens), so a few tokens cost a narrow tile. The K
 //                        splits of a tile are one thread-block cluster and are summed through distributed shared memory.
 //   product_pair_kernel  CTA pairs (cta_group::2) of 256 x 256 tiles for products with many of them.
-// Measured: nvfp4 1x28672x4096 13.8 us (4.8 TB/s: the weights' bytes and 3 us of launch, first loads and epilogue bound
-// it), 128x4096x14336 12.2 us; 8192x28672x4096 nvfp4 390 us (4.9 PFLOP/s), mxfp4 366 us (5.3), mxfp8 690 us (2.8).
+// Measured: nvfp4 1x28672x4096 13.6 us (4.85 TB/s: the weights' bytes and 3 us of launch, first loads and epilogue bound
+// it), mxfp4 128x4096x14336 12.7 us; 8192x28672x4096 nvfp4 383-401 us from GPU to GPU (4.8-5.0 PFLOP/s), mxfp4 366-376,
+// mxfp8 690 (2.8).
 // With its loads, scales or stores left out the last shape's nvfp4 time falls by some 100, 55 and 45 us: the MMAs alone take
 // 244 us, and shared memory's bandwidth, which they share with the copies in and out, is what is between.
 // Every wait is bounded as in b2g_gemm.cu: on expiry the status word gets a code and the CTA drains and returns.

@@ -247,10 +247,11 @@ class MicroTensor:
 
 
 def quantize(x: torch.Tensor, format: str = "mxfp8", scale: torch.Tensor | None = None) -> MicroTensor:
-    """x [rows, cols] (fp16, bf16 or fp32, any strides) in a microscaled format, blocks along the columns.
+    """x [rows, cols] (fp16, bf16 or fp32, any strides) in a microscaled format, blocks along the columns. No gradient
+    passes (micro_linear is the differentiable layer).
 
-    nvfp4: `scale` is the tensor's fp32 scale, one positive element on the device; values past 2688 times it saturate.
-    Without it, x is read twice: its scale becomes the smallest power of two at which nothing saturates."""
+    nvfp4: `scale` is the tensor's fp32 scale, one element on the device from 2^-100 to 2^117; values past 2688 times it
+    saturate. Without it, x is read twice: its scale becomes the smallest power of two at which nothing saturates."""
     fmt = FORMATS.get(format)
     if fmt is None or not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _VALUES or x.dim() != 2:
         _format(format)
