@@ -15,8 +15,9 @@ constexpr int64_t kOneBlock = 16384;  // chunks of eight values up to which one 
 // ---------------------------------------------------------------- largest magnitude -> NVFP4 tensor scale
 // The smallest power of two 2^e >= 2^-100 with amax <= 2688 * 2^e (2688 = 6 * 448 = 1.3125 * 2^11). Every block takes
 // the maximum of its own candidate: the order does not matter. Infinities and NaN do not count. Up to kOneBlock chunks
-// one block does it alone, without a launch that clears the scale first (16x4096: 3 us less). 4096x14336 takes 24 us
-// (4.9 TB/s; loads' latency bounds it), as much again where x is then read from memory to be quantised.
+// one block does it alone, without a launch that clears the scale first (16x4096: 3 us less). 4096x14336 takes 24 us,
+// three of them the launch that clears the scale: reading alone takes 21 (5.6 TB/s), and no other launch shape (256 to 1024
+// threads a block, two to eight loads in flight each, 296 to 7104 blocks) was faster.
 __device__ __forceinline__ uint32_t finite_bits(float v) {
   const uint32_t a = __float_as_uint(v) & 0x7fffffffu;
   return a >= 0x7f800000u ? 0u : a;
