@@ -607,6 +607,8 @@ def micro_mlp(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: torch
     [2 * F, hidden] and w_down [hidden, F] are quantised weights of one format; the norm and the gate write their outputs
     in it, so no activation is read or written in between but once. `scales`: for nvfp4, the calibrated tensor scales of
     the norm's and the gate's output."""
+    if not isinstance(w_gate_up, MicroTensor) or not isinstance(w_down, MicroTensor):
+        raise TypeError("w_gate_up and w_down must be MicroTensors (quantize makes them)")
     if w_gate_up.format != w_down.format:
         raise ValueError(f"w_gate_up is {w_gate_up.format}, w_down {w_down.format}: a block needs one format")
     s = scales if scales is not None else (None, None)

@@ -140,6 +140,8 @@ def test_python_refuses_cpu_tensors_and_bad_formats():
             call()
     with pytest.raises(TypeError, match="MicroTensors"):
         micro.micro_matmul(x, x)
+    with pytest.raises(TypeError, match="MicroTensors"):
+        micro.micro_mlp(x, None, x[0], x, x)
     with pytest.raises(TypeError, match="float16 or bfloat16"):
         micro.MicroMatmul(torch.float32)
 
