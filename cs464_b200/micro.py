@@ -33,6 +33,7 @@ import ctypes
 import math
 import struct
 import weakref
+from operator import attrgetter
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -152,9 +153,11 @@ class MicroTensor:
     codes a byte, the lower column in the low bits, what is left of an odd row's last byte zero. `scales`: uint8,
     contiguous, ceil(rows / 128) * ceil(blocks / 4) tiles of 512 bytes in the tensor cores' order (include/b2g_micro.h),
     zero where rows or blocks do not exist. `scale`: nvfp4's fp32 scale of the tensor (one element on the device), which
-    other formats do not have. The constructor checks and takes the tensors as they are."""
+    other formats do not have. The constructor checks and takes the tensors as they are. None of the fields can be
+    assigned: calls read the addresses packed here. Another scale is another tensor, MicroTensor(q.codes, q.scales,
+    q.shape, q.format, scale); what the tensors hold may be changed in place."""
 
-    __slots__ = ("_codes", "_scales", "shape", "format", "scale", "_buf", "_raw", "__weakref__")
+    __slots__ = ("_codes", "_scales", "_shape", "_format", "_scale", "_buf", "_raw", "__weakref__")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, format: str, scale: torch.Tensor | None = None):
         fmt = _format(format)
@@ -183,7 +186,7 @@ class MicroTensor:
         elif scale is not None:
             raise ValueError(f"{format} has no tensor scale")
         self._codes, self._scales, self._buf = codes, scales, codes
-        self.shape, self.format, self.scale = (rows, cols), format, scale
+        self._shape, self._format, self._scale = (rows, cols), format, scale
         self._raw = _pack_tensor(fmt, 0, rows, cols, at, row, sat, scale.data_ptr() if scale is not None else 0)
 
     @classmethod
@@ -194,10 +197,14 @@ class MicroTensor:
         buf = self._buf = _new_bytes(rows * pitch + scale_bytes, like)
         at = buf.data_ptr()
         self._codes = self._scales = None
-        self.shape, self.format, self.scale = (rows, cols), format, scale
+        self._shape, self._format, self._scale = (rows, cols), format, scale
         self._raw = _pack_tensor(fmt, 0, rows, cols, at, pitch, at + rows * pitch,
                                  scale.data_ptr() if scale is not None else 0)
         return self
+
+    shape = property(attrgetter("_shape"))
+    format = property(attrgetter("_format"))
+    scale = property(attrgetter("_scale"))
 
     @property
     def codes(self) -> torch.Tensor:
@@ -278,7 +285,7 @@ def dequantize(q: MicroTensor, dtype: torch.dtype = torch.bfloat16, out: torch.T
     if out is None:
         if dtype not in _VALUES:
             raise TypeError(f"dtype must be float16, bfloat16 or float32, not {dtype}")
-        out = q._buf.new_empty(q.shape, dtype=dtype)
+        out = q._buf.new_empty(q._shape, dtype=dtype)
     else:
         _check(out, "out", _VALUES, q._buf)
         if tuple(out.shape) != q.shape:
@@ -306,12 +313,12 @@ def _output(a: MicroTensor, b: MicroTensor, out: torch.Tensor | None, dtype: tor
         raise TypeError("a and b must be MicroTensors (quantize makes them)")
     if a._buf.get_device() != b._buf.get_device():
         raise ValueError(f"a is on {a.device}, b on {b.device}")
-    if a.format != b.format:
+    if a._format != b._format:
         raise ValueError(f"a is {a.format}, b {b.format}: a product needs one format")
-    if a.shape[1] != b.shape[1]:
+    if a._shape[1] != b._shape[1]:
         raise ValueError(f"a is {a.shape[0]}x{a.shape[1]}, b {b.shape[0]}x{b.shape[1]}: their columns are summed over and "
                          "must agree")
-    M, N = a.shape[0], b.shape[0]
+    M, N = a._shape[0], b._shape[0]
     if out is None:
         if dtype not in _HALF:
             raise TypeError(f"dtype must be float16 or bfloat16, not {dtype}")

@@ -146,6 +146,15 @@ def test_python_refuses_cpu_tensors_and_bad_formats():
         micro.MicroMatmul(torch.float32)
 
 
+def test_a_tensors_fields_cannot_be_assigned():
+    """The kernels read the addresses, sizes and format packed when the tensor was made: an assignment that they would not
+    see (and that could drop the only owner of a scale they go on reading) is refused."""
+    q = object.__new__(micro.MicroTensor)
+    for field in ("scale", "shape", "format", "codes", "scales", "device"):
+        with pytest.raises(AttributeError):
+            setattr(q, field, None)
+
+
 # ---------------------------------------------------------------- the oracle
 def test_oracle_codes_by_hand():
     x = np.zeros((1, 64))
