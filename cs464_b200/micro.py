@@ -20,7 +20,8 @@ scaled kinds. Formats:
 All of it enqueues on the current stream of the tensors' device and allocates its outputs (and the norm gradient's
 workspace) from torch's allocator on that stream; nothing is kept between calls, nothing synchronises, and every call
 can be captured into a CUDA graph (a training step with torch's own condition: no eager autograd graph of the same
-leaves may be alive during the capture). As elsewhere with torch, tensors made on another stream have to be ready on the
+leaves may be alive during the capture). The differentiable calls have a backward pass of first order; forward-mode
+derivatives through them are refused, and nothing is differentiable through the other calls. As elsewhere with torch, tensors made on another stream have to be ready on the
 current one. The product's kernels bound their waits: `check_status()` (from cs464_b200.matmul) raises if one ran out.
 
 The arithmetic of a quantisation is exact: which code and which scale a value gets follows from its bits alone
@@ -36,6 +37,7 @@ import weakref
 from operator import attrgetter
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from cs464_b200 import _abi
@@ -129,6 +131,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _like(t: torch.Tensor) -> torch.Tensor:
     """Uninitialised contiguous storage of t's shape and type."""
     return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _has_tangent(*tensors: torch.Tensor | None) -> bool:
+    """Whether a forward-mode derivative is being taken through one of them."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _check_scale(scale, like: torch.Tensor) -> None:
@@ -509,7 +516,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     x2 = x if x.dim() == 2 else _rows(x)
     r2 = residual if residual is None or residual.dim() == 2 else _rows(residual)
     grad = (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)) \
-        and torch.is_grad_enabled()
+        and torch.is_grad_enabled() or forward_ad._current_level >= 0 and _has_tangent(x, weight, residual)
     if not weight.is_contiguous():
         weight = weight.contiguous()
     if format is not None:
@@ -585,7 +592,7 @@ def silu_mul(gate_up: torch.Tensor, format: str | None = None, scale: torch.Tens
     same type, differentiable, or with `format` a MicroTensor [rows, cols] for the next product (nvfp4 needs `scale`)."""
     _gate_input(gate_up)
     x = _rows(gate_up)
-    grad = gate_up.requires_grad and torch.is_grad_enabled()
+    grad = gate_up.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 and _has_tangent(gate_up)
     if format is not None:
         return _gate_forward(x, _coded(x, x.shape[1] // 2, format, scale, grad))
     if scale is not None:

@@ -798,3 +798,26 @@ def test_offsets_past_32_bits():
     check_product(torch.cat([c[:, :2], c[:, -3:]], 1), a, f64(want))
     c = micro.micro_matmul(q, qa)  # the long side as rows
     check_product(torch.cat([c[:2], c[-3:]]), f64(want), a)
+
+
+# ---------------------------------------------------------------- derivatives and views that torch keeps lazily
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor has no requires_grad: the layers must not take it for a constant, whose tangent is zero."""
+    from torch.autograd import forward_ad
+    x, w, v, t = normal(4, 64), normal(64, seed=1), normal(8, 64, seed=2), normal(4, 64, seed=3)
+    plain = micro.rms_norm(x, w, residual=t)[0], micro.silu_mul(x)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, t)
+        dw = forward_ad.make_dual(w, t[0])
+        calls = (lambda **kw: micro.rms_norm(d, w, **kw), lambda **kw: micro.rms_norm(x, dw, **kw),
+                 lambda **kw: micro.rms_norm(x, w, residual=d, **kw), lambda **kw: micro.silu_mul(d, **kw))
+        for call in (*calls, lambda: micro.micro_linear(d, v)):
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call()
+        for call in calls:
+            with pytest.raises(ValueError, match="no gradient"):
+                call(format="mxfp8")
+        assert torch.equal(micro.rms_norm(x, w, residual=t)[0], plain[0]) and torch.equal(micro.silu_mul(x), plain[1])
+    for f in (lambda a: micro.rms_norm(a, w)[0], micro.silu_mul, lambda a: micro.micro_linear(a, v)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(f, (x,), (t,))
