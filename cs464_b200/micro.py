@@ -124,8 +124,21 @@ def _check(t: torch.Tensor, what: str, dtypes, like: torch.Tensor | None = None)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t as a matrix of rows (its last dimension)."""
+    """t as a matrix of rows (its last dimension) whose storage holds its values: torch keeps some views negated lazily
+    (the imaginary part of a conjugate; gradients of such come from autograd), which become copies."""
+    if t.is_neg():
+        t = t.resolve_neg()
     return t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+
+
+def _weight(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous, its storage holding its values."""
+    return t if t.is_contiguous() and not t.is_neg() else t.resolve_neg().contiguous()
+
+
+def _check_out(t: torch.Tensor) -> None:
+    if t.is_neg():
+        raise ValueError("out is a lazily negated view: its storage would hold the negated values")
 
 
 def _like(t: torch.Tensor) -> torch.Tensor:
@@ -140,8 +153,8 @@ def _has_tangent(*tensors: torch.Tensor | None) -> bool:
 
 def _check_scale(scale, like: torch.Tensor) -> None:
     if (not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or scale.numel() != 1
-            or scale.get_device() != like.get_device()):
-        raise ValueError(f"scale must be a float32 tensor of one element on {like.device}")
+            or scale.get_device() != like.get_device() or scale.is_neg()):
+        raise ValueError(f"scale must be a float32 tensor of one element on {like.device}, not negated lazily")
 
 
 def _layout(fmt: int, rows: int, cols: int) -> tuple[int, int]:
@@ -271,6 +284,8 @@ def quantize(x: torch.Tensor, format: str = "mxfp8", scale: torch.Tensor | None 
         _format(format)
         _check(x, "x", _VALUES)
         raise ValueError(f"x must be a matrix, not {tuple(x.shape)}")
+    if x.is_neg():
+        x = x.resolve_neg()
     rows, cols = x.shape
     mat, kind, index = _pack_matrix(x.data_ptr(), *x.stride()), _VALUES[x.dtype], x.get_device()
     if fmt == _abi.FMT_NVFP4:
@@ -297,6 +312,7 @@ def dequantize(q: MicroTensor, dtype: torch.dtype = torch.bfloat16, out: torch.T
         _check(out, "out", _VALUES, q._buf)
         if tuple(out.shape) != q.shape:
             raise ValueError(f"out must be {q.shape[0]}x{q.shape[1]}, not {tuple(out.shape)}")
+        _check_out(out)
     _call(q._buf.get_device(), _entry.dequantize, q._raw, _matrix(out), _VALUES[out.dtype])
     return out
 
@@ -334,6 +350,7 @@ def _output(a: MicroTensor, b: MicroTensor, out: torch.Tensor | None, dtype: tor
     if tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
         raise ValueError(f"out must be a {M}x{N} tensor with unit column stride and rows that do not overlap, not "
                          f"{tuple(out.shape)} with strides {out.stride()}")
+    _check_out(out)
     return out
 
 
@@ -420,7 +437,7 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, w = ctx.saved_tensors
-        fmt, dx, dw = ctx.fmt, None, None
+        fmt, dx, dw, dy = ctx.fmt, None, None, _rows(dy)
         if ctx.needs_input_grad[0]:
             dx = _values_product(dy, w.t(), fmt)
         if ctx.needs_input_grad[1]:
@@ -437,7 +454,7 @@ def micro_linear(x: torch.Tensor, w: torch.Tensor, format: str = "mxfp8") -> tor
     _check(w, "w", (x.dtype,), x)
     if w.ndim != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"x must be [..., K] and w [N, K], not {tuple(x.shape)} and {tuple(w.shape)}")
-    y = _Linear.apply(_rows(x), w, fmt)
+    y = _Linear.apply(_rows(x), _rows(w), fmt)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.shape[0])
 
 
@@ -490,8 +507,8 @@ def _norm_args(x, weight, residual) -> bool:
     """Whether rms_norm takes them: the checks that rms_norm repeats one by one where they fail."""
     try:
         dtype, index, shape = x.dtype, x.get_device(), x.shape
-        return (dtype in _HALF and index >= 0 and weight.dtype is dtype and weight.get_device() == index
-                and shape[-1:] == weight.shape and weight.dim() == 1
+        return bool(dtype in _HALF and index >= 0 and weight.dtype is dtype and weight.get_device() == index
+                and shape and shape[-1:] == weight.shape
                 and (residual is None or (residual.dtype is dtype and residual.shape == shape
                                           and residual.get_device() == index)))
     except (AttributeError, TypeError):
@@ -513,12 +530,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
             raise ValueError(f"weight must be [{x.shape[-1] if x.dim() else '?'}], not {tuple(weight.shape)}")
         _check(residual, "residual", (x.dtype,), x)
         raise ValueError(f"residual is {tuple(residual.shape)}, x {tuple(x.shape)}")
-    x2 = x if x.dim() == 2 else _rows(x)
-    r2 = residual if residual is None or residual.dim() == 2 else _rows(residual)
+    x2 = _rows(x)
+    r2 = None if residual is None else _rows(residual)
     grad = (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)) \
         and torch.is_grad_enabled() or forward_ad._current_level >= 0 and _has_tangent(x, weight, residual)
-    if not weight.is_contiguous():
-        weight = weight.contiguous()
+    weight = _weight(weight)
     if format is not None:
         y, h = _norm_forward(x2, r2, weight, eps, _coded(x2, x2.shape[1], format, scale, grad))
     elif scale is not None:
@@ -548,8 +564,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, e
         raise ValueError(f"dy {tuple(dy.shape)}, dh and h {tuple(h.shape)} must have one shape, weight "
                          f"{tuple(weight.shape)} its last dimension")
     dy2, h2, dh2 = _rows(dy), _rows(h), None if dh is None else _rows(dh)  # held until the launch: some may be copies
-    if not weight.is_contiguous():
-        weight = weight.contiguous()
+    weight = _weight(weight)
     rows, cols = h2.shape
     n = ctypes.c_size_t(0)
     _abi.check(_abi.load().b2g_micro_rms_norm_workspace(rows, cols, n), "b2g_micro_rms_norm_workspace")

@@ -821,3 +821,49 @@ def test_forward_mode_derivatives_are_refused():
     for f in (lambda a: micro.rms_norm(a, w)[0], micro.silu_mul, lambda a: micro.micro_linear(a, v)):
         with pytest.raises((RuntimeError, NotImplementedError)):
             torch.func.jvp(f, (x,), (t,))
+
+
+def negated(rows, cols, dtype, seed):
+    """A tensor whose values torch stores negated, with its flag set: the imaginary part of a conjugate."""
+    z = torch.complex(*(normal(rows, cols, dtype=torch.float32, seed=s) for s in (seed, seed + 1)))
+    if dtype == torch.float16:
+        z = z.to(torch.complex32)
+    v = z.conj().imag
+    assert v.is_neg() and v.dtype == dtype
+    return v
+
+
+def test_lazily_negated_tensors_keep_their_sign():
+    """The kernels read storage: values that torch would negate on the way have to be negated before."""
+    v = negated(40, 64, torch.float32, 1)
+    for fmt in FORMATS:
+        check_quantized(micro.quantize(v, fmt), f64(v))
+        check_quantized(micro.quantize(v.t(), fmt), f64(v.t()))
+    half = torch.float16
+    x, r, w, dy, dh = negated(40, 64, half, 2), negated(40, 64, half, 4), negated(1, 64, half, 6)[0], \
+        negated(40, 64, half, 8), negated(40, 64, half, 10)
+    plain = [t.resolve_neg() for t in (x, r, w, dy, dh)]
+    for got, want in ((micro.rms_norm(x, w, residual=r), micro.rms_norm(plain[0], plain[2], residual=plain[1])),
+                      (micro.rms_norm(x, w), micro.rms_norm(plain[0], plain[2])),
+                      (micro.rms_norm_backward(dy, x, w, dh=dh), micro.rms_norm_backward(plain[3], plain[0], plain[2], dh=plain[4])),
+                      ((micro.silu_mul(x),), (micro.silu_mul(plain[0]),)),
+                      ((micro.silu_mul_backward(dy[:, :32], x),), (micro.silu_mul_backward(plain[3][:, :32], plain[0]),)),
+                      ((micro.micro_linear(x, r),), (micro.micro_linear(plain[0], plain[1]),)),
+                      ((micro.rms_norm(x, w, format="mxfp8")[0].dequantize(half),), (micro.rms_norm(plain[0], plain[2], format="mxfp8")[0].dequantize(half),)),
+                      ((micro.silu_mul(x.view(4, 10, 64)),), (micro.silu_mul(plain[0]).view(4, 10, 32),)),
+                      (micro.rms_norm(x[:, :1], w[:1]), micro.rms_norm(plain[0][:, :1], plain[2][:1]))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+    # autograd hands such gradients down, the imaginary part of a complex gradient for one
+    leaves = [t.clone().requires_grad_() for t in (plain[0], plain[1])]
+    y = micro.micro_linear(*leaves)
+    n = micro.rms_norm(leaves[0], plain[2])[0]
+    for out, d in ((y, negated(40, 40, half, 12)), (n, dy), (micro.silu_mul(leaves[0]), dy[:, :32])):
+        for a, b in zip(*(torch.autograd.grad(out, leaves, g, retain_graph=True, allow_unused=True) for g in (d, d.resolve_neg()))):
+            assert (a is None and b is None) or torch.equal(a, b)
+    q = micro.quantize(v, "mxfp8")
+    with pytest.raises(ValueError, match="negated"):
+        micro.dequantize(q, out=negated(40, 64, torch.float32, 14))
+    with pytest.raises(ValueError, match="negated"):
+        micro.micro_matmul(q, micro.quantize(v[:1], "mxfp8"), out=negated(40, 1, half, 16))
+    with pytest.raises(ValueError, match="scale must be"):
+        micro.quantize(v, "nvfp4", scale=negated(1, 1, torch.float32, 18)[0])
