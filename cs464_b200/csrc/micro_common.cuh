@@ -392,8 +392,9 @@ __device__ __forceinline__ uint32_t amax8(const Raw8<float>& r) {
 //   processor", 1990). The residual is taken negated, so that zeros keep the value's sign. A block whose scale rounds to
 //   zero is zero.
 // The codes of a NaN block are cleared by `keep`. NVFP4's tensor scale g as a thread uses it: 6 g and its reciprocal,
-// once, so that a block's scale amax / (6 g) is three operations of the same kind. (Below 2^-60 the residual would
-// leave fp32's range: the division is done as such.)
+// once, so that a block's scale amax / (6 g) is three operations of the same kind. Residuals that would leave fp32's range
+// at the bottom are avoided: below g = 2^-60 a block's scale is divided as such, and codes8 lifts values and u where u may
+// be below 2^-100 (the last bit of a quotient above 2^-3, times that of u, is then below 2^-149).
 struct TensorScale {
   float g, six, inv;
   __device__ __forceinline__ explicit TensorScale(float scale) : g(scale), six(6.f * scale), inv(1.f / (6.f * scale)) {}
@@ -411,12 +412,14 @@ struct BlockQuant {
   uint32_t keep;  // all ones; 0 in a NaN block
   float mul;      // MX: 2^-e; NVFP4: 1 / u, or 0
   float unit;     // NVFP4: u
+  bool tiny;      // NVFP4: u may be below 2^-100, where a quotient's residual is among fp32's subnormals
   __device__ __forceinline__ void init(uint32_t amax_bits, const TensorScale& ts) {
     const bool bad = amax_bits >= 0x7f800000u;
     keep = bad ? 0u : 0xffffffffu;
     if constexpr (FMT == FMT_NVFP4) {
       byte = bad ? 0x7fu : __nv_cvt_float_to_fp8(ts.block(__uint_as_float(amax_bits)), __NV_SATFINITE, __NV_E4M3);
       unit = e4m3_to_f32(byte) * ts.g;
+      tiny = ts.g < 4.03896783e-28f;  // 2^-91: block scales go down to 2^-9
       mul = byte == 0u ? 0.f : reciprocal(unit);
     } else {
       byte = mx_scale_byte<FMT>(amax_bits);
@@ -465,17 +468,24 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
   return r;
 }
 
-// Eight values' codes: .x (and .y for MXFP8), lowest column in the lowest bits.
-template <int FMT>
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], const BlockQuant<FMT>& b) {
+// Eight values' codes: .x (and .y for MXFP8), lowest column in the lowest bits. EXACT: also with a tiny u, which only values
+// that are quantised as they lie are worth (a layer's outputs carry errors of their own, and the norm takes 4 % longer).
+template <int FMT, bool EXACT>
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], BlockQuant<FMT> b) {
   float s[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) s[i] = v[i];
   if constexpr (FMT == FMT_NVFP4) {
-    if (b.byte == 0x7eu) {  // the largest scale: values past 6 u saturate, and their quotients may leave fp32's range
-      const float top = 8.f * b.unit;
+    // The largest scale: values past 6 u saturate, and their quotients may leave fp32's range. (No other scale's values
+    // saturate.) A tiny u: the quotients are those of 2^40 times value and u, whose residuals fp32 holds.
+    const bool tiny = EXACT && b.tiny;
+    if (b.byte == 0x7eu || tiny) {
+      const float top = b.byte == 0x7eu ? 8.f * b.unit : __uint_as_float(0x7f800000u);
+      const float lift = tiny ? 1099511627776.f : 1.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = fminf(fmaxf(s[i], -top), top);
+      for (int i = 0; i < 8; ++i) s[i] = fminf(fmaxf(s[i], -top), top) * lift;
+      b.unit *= lift;
+      b.mul *= 1.f / lift;
     }
   }
 #pragma unroll
@@ -506,7 +516,7 @@ struct CodePlace {
 // Quantise them. `m`: the eight values' amax8. A block's lanes (4 for blocks of 32, 2 for 16) share their largest
 // magnitude by shuffles; the four scale bytes of one tile row are gathered into one 4-byte store. Called by a
 // converged warp.
-template <int FMT>
+template <int FMT, bool EXACT>
 __device__ __forceinline__ void quantize_store(const float (&v)[8], uint32_t m, int lane, const CodePlace<FMT>& to,
                                                const TensorScale& ts) {
   constexpr int kLanes = block_of(FMT) / 8;
@@ -514,7 +524,7 @@ __device__ __forceinline__ void quantize_store(const float (&v)[8], uint32_t m, 
   for (int d = 1; d < kLanes; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
   BlockQuant<FMT> b;
   b.init(m, ts);
-  const uint2 q = codes8<FMT>(v, b);
+  const uint2 q = codes8<FMT, EXACT>(v, b);
   if (to.has_codes) {
     if constexpr (FMT == FMT_MXFP8) *reinterpret_cast<uint2*>(to.codes) = q;
     else *reinterpret_cast<uint32_t*>(to.codes) = q.x;

@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(ROUNDS))
     } else {
       CodePlace<FMT> to(q, row, c, threadIdx.x & 31);
       to.has_codes = to.has_codes && live;
-      quantize_store<FMT>(f, amax8(f), threadIdx.x & 31, to, ts);
+      quantize_store<FMT, false>(f, amax8(f), threadIdx.x & 31, to, ts);
     }
   };
 #pragma unroll

@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(1024)
 template <typename T>
 struct ValueSource {
   static constexpr int kLoads = 1;
+  static constexpr bool kExact = true;
   __device__ __forceinline__ static uint32_t value(const Raw8<T> (&r)[1], float (&v)[8]) {  // and their amax8
     unpack8(r[0], v);
     return amax8(r[0]);
@@ -112,6 +113,7 @@ __device__ __forceinline__ float2 sigmoids(float x) {
 template <typename T>
 struct GateSource {
   static constexpr int kLoads = 2;
+  static constexpr bool kExact = false;
   __device__ __forceinline__ static uint32_t value(const Raw8<T> (&r)[2], float (&v)[8]) {
     float g[8], u[8];
     unpack8(r[0], g);
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       for (int k = 0; k < S::kLoads; ++k) r[k] = settle8<T, MODE>(f[i][k], scratch);
       float v[8];
       const uint32_t m = S::value(r, v);
-      quantize_store<FMT>(v, m, lane, to, ts);
+      quantize_store<FMT, S::kExact>(v, m, lane, to, ts);
     } else if (to.leads) {  // a row past the last: zero scales and no codes
       *reinterpret_cast<uint32_t*>(to.word) = 0u;
     }
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(128) quantize_cols_kernel(Mat x, int64_t rows,
         float e[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = v[8 * g + i];
-        const uint2 w = codes8<FMT>(e, b);
+        const uint2 w = codes8<FMT, true>(e, b);
         if constexpr (FMT == FMT_MXFP8) {
           word[2 * g] = w.x;
           word[2 * g + 1] = w.y;

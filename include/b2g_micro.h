@@ -13,7 +13,9 @@
  *   NVFP4  e2m1 codes, one e4m3 scale per 16 columns, one fp32 scale for the tensor
  * value = code * block scale [* tensor scale]. A block's power-of-two scale is the smallest one, from 2^-127 up, at
  * which no element passes the code's largest magnitude; an NVFP4 block's is its largest magnitude / (6 * tensor scale)
- * rounded to e4m3. Codes round to nearest, ties to even. A block that holds an infinity or a NaN gets a NaN scale.
+ * rounded to e4m3. Codes round to nearest, ties to even. A block that holds an infinity or a NaN gets a NaN scale. With a
+ * tensor scale that is no power of two, 6 * tensor scale and block scale * tensor scale are fp32 values, and the quotients
+ * by them are rounded to fp32 before they are rounded to e4m3 and to codes.
  *
  * Codes: row r starts at codes + r * pitch; MXFP8 has one byte a code, the 4-bit formats two codes a byte, the lower
  * column in the low four bits. What is left of the last byte of an odd row is zero.

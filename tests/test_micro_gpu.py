@@ -867,3 +867,45 @@ def test_lazily_negated_tensors_keep_their_sign():
         micro.micro_matmul(q, micro.quantize(v[:1], "mxfp8"), out=negated(40, 1, half, 16))
     with pytest.raises(ValueError, match="scale must be"):
         micro.quantize(v, "nvfp4", scale=negated(1, 1, torch.float32, 18)[0])
+
+
+@pytest.mark.parametrize("g", [2.0 ** -100, (1 + 3 * 2.0 ** -23) * 2.0 ** -100, (1 + 14 * 2.0 ** -23) * 2.0 ** -100, 1.9 * 2.0 ** -100, 1.37 * 2.0 ** -96, 1.6 * 2.0 ** -61, 1.2e-18, 1.1e-7, 3.3e-4, 0.05,
+                               1.0 / 448, 1.0, 7.7, 1e20, 1.99 * 2.0 ** 116, 2.0 ** 117])
+def test_nvfp4_codes_next_to_every_border(g):
+    """What include/b2g_micro.h defines for any scale: 6 g and u = block scale * g as fp32 values, quotients as fp32
+    divisions give them, then rounding to the codes. numpy's division is the reference; block maxima lie at and next to the
+    borders between block scales, values at and one fp32 step to either side of the borders between codes times u."""
+    rng = np.random.default_rng(int(np.float32(g).view(np.uint32)))
+    one = np.float32(1)
+    g = np.float32(g)
+    six = np.float32(6) * g
+
+    def step(v, k):  # k fp32 steps up, for positive v
+        return (v.view(np.uint32).astype(np.int64) + k).astype(np.uint32).view(np.float32)
+    rows, blocks = 2048, 20
+    mids = (om.E4M3[1:] + om.E4M3[:-1]) / 2
+    # block maxima: random, and around the middle between two block scales
+    with np.errstate(over="ignore"):
+        top = np.where(rng.random((rows, blocks)) < 0.5, np.exp(rng.uniform(np.log(0.002), np.log(450.0), (rows, blocks))),
+                       rng.choice(mids[:-1], (rows, blocks))).astype(np.float32) * six
+        top = np.minimum(top, np.float32(3e38))
+        top = step(top, rng.integers(-1, 2, top.shape))
+        quotient = np.minimum(top, np.float32(448) * six) / six
+    s = om._nearest(quotient.astype(np.float64), om.E4M3)
+    u = om.E4M3[s].astype(np.float32) * g
+    border = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], np.float32)
+    x = step(np.minimum(rng.choice(border, (rows, blocks, 16)) * np.maximum(u, 0.5 * g * om.E4M3[1].astype(np.float32))[..., None], top[..., None]),
+             rng.integers(-1, 2, (rows, blocks, 16)))
+    x = np.minimum(x, top[..., None])
+    x[..., 5] = top
+    x *= rng.choice([-one, one], x.shape)
+    with np.errstate(divide="ignore", over="ignore", invalid="ignore"):
+        q = np.where(s[..., None] > 0, x / u[..., None], np.float32(0))
+    code = om._nearest(np.abs(q).astype(np.float64), om.E2M1) | (np.signbit(x).astype(int) << 3)
+    x, code = x.reshape(rows, -1), code.reshape(rows, -1)
+    t = torch.from_numpy(x).cuda()
+    scale = torch.full((1,), float(g), device="cuda")
+    for v in (t, t.t().contiguous().t()):
+        c, sb = stored(micro.quantize(v, "nvfp4", scale=scale))
+        assert np.array_equal(sb, s), (sb != s).sum()
+        assert np.array_equal(c, code), ((c != code).sum(), x[c != code][:3], u.min())
