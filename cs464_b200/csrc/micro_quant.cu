@@ -366,9 +366,21 @@ __global__ void __launch_bounds__(256) gate_kernel(Mat x, T* y, int64_t syr, int
 }
 
 // With s = sigmoid(g): d gate = dy * up * s * (1 + g * (1 - s)), d up = dy * g * s. 1 - s is taken as sigmoid(-g),
-// which keeps its digits where s is near one.
+// which keeps its digits where s is near one. dy * up may leave fp32's range where the gradient does not (bf16's lowest
+// values among them, under a small s), and so may the small factor times the smaller of them: half the small factor meets
+// the larger one first.
+__device__ __forceinline__ void gate_gradient(float g, float u, float d, float& dg, float& du) {
+  const float2 s = sigmoids(g);
+  float larger;  // of dy's and up's magnitudes, with the product's sign
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(larger) : "f"(d), "f"(u));
+  const float half = s.x * fmaf(0.5f * g, s.y, 0.5f);
+  dg = half * larger * fminf(fabsf(d), fabsf(u)) * 2.f;
+  du = d * (g * s.x);
+}
+
+// Aligned rows take 32 registers a thread, so that SMs are full (36 without the bound: 45.5 us for 2048x14336).
 template <typename T, int MODE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, MODE == kVec ? 8 : 0)
     gate_backward_kernel(Mat dy, Mat x, T* dx, int64_t sxr, int64_t sxc, int64_t rows, int64_t cols,
                          uint32_t row_blocks) {
   // blockDim.y rows of blockDim.x chunks of eight columns (kUnit: whole warps of them); row_blocks blocks along a row
@@ -385,11 +397,7 @@ __global__ void __launch_bounds__(256)
   unpack8(ru, u);
   unpack8(rd, d);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 s = sigmoids(g[i]);
-    dg[i] = d[i] * u[i] * s.x * (1.f + g[i] * s.y);
-    du[i] = d[i] * g[i] * s.x;
-  }
+  for (int i = 0; i < 8; ++i) gate_gradient(g[i], u[i], d[i], dg[i], du[i]);
   T* o = dx + row * sxr;
   store8<T, MODE>(o, sxc, c, cols, pack8<T>(dg), scratch);
   store8<T, MODE>(o + cols * sxc, sxc, c, cols, pack8<T>(du), scratch);

@@ -909,3 +909,29 @@ def test_nvfp4_codes_next_to_every_border(g):
         c, sb = stored(micro.quantize(v, "nvfp4", scale=scale))
         assert np.array_equal(sb, s), (sb != s).sum()
         assert np.array_equal(c, code), ((c != code).sum(), x[c != code][:3], u.min())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_gate_gradient_of_large_and_small_factors(dtype):
+    """Factors whose partial products leave fp32's range where the gradient does not: upstream gradients and ups from tiny
+    to a mask's lowest value, gates from -100 up. Bound as in test_gate (the exponential errs by up to 2 + 1.173 * 100 ulps,
+    below 2^-15 in all) and as much of a step of fp32's subnormals as the sigmoid is above them; half a step of the type's
+    own subnormals. Past the type's largest value the gradient is infinite."""
+    top = torch.finfo(dtype).max
+    sizes = [1e-30, 1e-10, 1.0, 1e10, 1e20, 1e30, top] if dtype == torch.bfloat16 else [1e-4, 1.0, 300.0, top]
+    g = torch.tensor([-100.0, -95.0, -88.0, -70.0, -60.0, -20.0, -3.0, -1.25, 0.0, 0.5, 2.375, 20.0, 100.0])
+    g, u, d = (t.reshape(1, -1) for t in torch.meshgrid(g, torch.tensor([s * f for s in sizes for f in (1, -1)]), torch.tensor(sizes), indexing="ij"))
+    x, dy = torch.cat([g, u], 1).to(dtype).cuda(), d.to(dtype).cuda()
+    a, b = f64(dy), f64(x)
+    n = a.shape[1]
+    g, u = b[:, :n], b[:, n:]
+    s = 1 / (1 + np.exp(-g))
+    terms = [a * u * s * (1 + np.abs(g) * (1 - s)), a * g * s]
+    ref = [a * u * s * (1 + g * (1 - s)), a * g * s]
+    got = f64(micro.silu_mul_backward(dy, x))
+    for y, r, t in zip((got[:, :n], got[:, n:]), ref, terms):
+        bound = half_step(dtype) * np.abs(r) + (2.0 ** -15 + 2.0 ** -147 / s) * np.abs(t) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+        out = np.abs(r) > 1.01 * top
+        near = np.abs(r) + bound > 0.99 * top  # may round to the largest value or to an infinity
+        assert (np.isinf(y[out]) & (np.sign(y[out]) == np.sign(r[out]))).all()
+        assert (np.abs(y - r)[~near] <= bound[~near]).all() and not np.isnan(y).any()
