@@ -404,7 +404,8 @@ __global__ void __launch_bounds__(256, MODE == kVec ? 8 : 0)
 }
 
 // ---------------------------------------------------------------- host side
-// Blocks of 256 threads over rows of eight-column chunks: several rows a block where they are short.
+// Blocks of 256 threads over rows of eight-column chunks: several rows a block where they are short. Chunks are counted in
+// 32 bits, the last block's included: rows of more are given a grid past every limit.
 struct RowBlocks {
   dim3 block;
   uint32_t along;
@@ -416,7 +417,7 @@ RowBlocks row_blocks(int64_t rows, int64_t cols, int mode) {
   unsigned x = mode == kUnit ? 32 : 1;
   while (x < chunks && x < 256) x *= 2;
   RowBlocks b{dim3(x, 256 / x), static_cast<uint32_t>(ceil_div(chunks, x)), 0};
-  b.grid = ceil_div(rows, b.block.y) * b.along;
+  b.grid = chunks > (int64_t(1) << 32) - 256 ? kMaxGrid + 1 : ceil_div(rows, b.block.y) * b.along;
   return b;
 }
 

@@ -110,7 +110,8 @@ int32_t b2g_micro_rms_norm_backward(const b2g_micro_matrix* dy, const b2g_micro_
                                     void* workspace, size_t workspace_bytes, int64_t rows, int64_t cols, float eps,
                                     int32_t dtype, void* stream);
 
-/* y = gate / (1 + exp(-gate)) * up of gate_up [rows, 2 cols] = [gate | up], as values (y) or microscaled (q). */
+/* y = gate / (1 + exp(-gate)) * up of gate_up [rows, 2 cols] = [gate | up], as values (y) or microscaled (q). cols is at
+   most 2^35 - 2048. */
 int32_t b2g_micro_silu_mul(const b2g_micro_matrix* gate_up, const b2g_micro_matrix* y, const b2g_micro_tensor* q,
                            int64_t rows, int64_t cols, int32_t dtype, void* stream);
 /* dgate_up [rows, 2 cols] from dy [rows, cols] and gate_up. */

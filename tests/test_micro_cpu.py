@@ -115,6 +115,16 @@ def test_norm_refuses_columns_past_its_counters():
                                                None) == _abi.B2G_ERR_UNSUPPORTED
 
 
+def test_gate_refuses_columns_past_its_counters():
+    """A row's eight-column chunks are counted in 32 bits, those of a whole block of 256 threads past its end included."""
+    lib = _abi.load()
+    for cols in (2 ** 35 - 2047, 2 ** 35, 2 ** 36 + 64):
+        mat = _abi.MicroMatrix(4096, 0, 0)
+        for rc in (lib.b2g_micro_silu_mul(mat, mat, None, 1, cols, 1, None),
+                   lib.b2g_micro_silu_mul_backward(mat, mat, mat, 1, cols, 1, None)):
+            assert rc == _abi.B2G_ERR_UNSUPPORTED and _abi.last_error().startswith("dimension_too_large")
+
+
 def test_empty_calls_do_nothing():
     lib = _abi.load()
     e = _tensor(rows=0, codes=None, scales=None)
