@@ -102,7 +102,10 @@ def _new_bytes(n: int, like: torch.Tensor) -> torch.Tensor:
     index = like.get_device()
     proto = _BYTES.get(index)
     if proto is None:
-        proto = _BYTES[index] = torch.empty(0, dtype=torch.uint8, device=like.device)
+        proto = torch.empty(0, dtype=torch.uint8, device=like.device)
+        if type(proto) is not torch.Tensor:  # made under a mode that replaces tensors: it must not outlive that
+            raise RuntimeError(f"no kernel runs on a {type(proto).__name__}")
+        _BYTES[index] = proto
     return proto.new_empty(n)
 
 
@@ -327,7 +330,11 @@ def _status(index: int) -> int:
         if index not in _STATUS and torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"the first product on cuda:{index} makes the device's status word, which a stream capture "
                                "cannot hold: run a product there once before the capture")
-        at = _STATUS_AT[index] = status_word(torch.device("cuda", index)).data_ptr()
+        word = status_word(torch.device("cuda", index))
+        if type(word) is not torch.Tensor:  # as in _new_bytes
+            del _STATUS[index]
+            raise RuntimeError(f"no kernel runs on a {type(word).__name__}")
+        at = _STATUS_AT[index] = word.data_ptr()
     return at
 
 

@@ -165,6 +165,31 @@ def test_a_tensors_fields_cannot_be_assigned():
             setattr(q, field, None)
 
 
+def test_fake_tensors_leave_nothing_behind(monkeypatch):
+    """Under a mode that replaces tensors (torch's tracing) calls raise, and what the module keeps per device is not made of
+    replaced tensors: real calls would go on using them, a status word at address 0 among them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from cs464_b200.matmul import status_word
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(micro, "_get_device", lambda: 0)
+    monkeypatch.setattr(micro, "_raw_stream", lambda index: 0)
+    kept = micro._BYTES, micro._STATUS_AT, status_word.__globals__["_STATUS"]
+    before = [dict(d) for d in kept]
+    try:
+        for d in kept:
+            d.clear()
+        with FakeTensorMode():
+            x = torch.empty(4, 64, dtype=torch.bfloat16, device="cuda")
+            for call in (lambda: micro.rms_norm(x, x[0], format="mxfp8"), lambda: micro.quantize(x), lambda: micro._status(0)):
+                with pytest.raises(RuntimeError):
+                    call()
+        assert not any(kept)
+    finally:
+        for d, b in zip(kept, before):
+            d.clear()
+            d.update(b)
+
+
 # ---------------------------------------------------------------- the oracle
 def test_oracle_codes_by_hand():
     x = np.zeros((1, 64))
