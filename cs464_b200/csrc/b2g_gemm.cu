@@ -367,9 +367,6 @@ __global__ void __launch_bounds__((2 + EPI_WARPS) * 32, 1)
                 const __grid_constant__ CUtensorMap tma_b) {
   static_assert(!(LEAN && PAIR), "the lean form is single-CTA only");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  // Let a programmatically dependent launch (the split-K reduce, or the next GEMM) be scheduled once every CTA of this
-  // grid is running; the dependent waits for this grid's completion before it touches global memory.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // This grid may itself be such a dependent: its set-up (barriers, tensor memory, descriptor prefetch) overlaps the
   // previous kernel's tail, and every thread waits for that kernel to complete (its writes visible) before its first
   // global access — A and B may be its outputs, and C or the workspace its inputs. Without the launch attribute the
@@ -498,6 +495,9 @@ __global__ void __launch_bounds__((2 + EPI_WARPS) * 32, 1)
       tmem_alloc(ctl + OFF_TMEM, p.tmem_cols);
       tmem_relinquish();
     }
+    // Let a programmatically dependent launch (the split-K reduce, or the next GEMM) be scheduled once every CTA of this
+    // grid is running; the dependent waits for this grid's completion before it touches global memory.
+    launch_dependents();
   }
   // Lane 0 of warp 0 may still be issuing its first copies: the warp converges first, because a block or cluster
   // barrier reached by part of a warp counts the whole warp as arrived.

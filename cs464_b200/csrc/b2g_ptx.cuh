@@ -114,6 +114,13 @@ __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
+// ---------------------------------------------------------------- programmatic dependent launch
+// Let the grid that depends on this one be scheduled once every CTA of this grid has called this or ended. A kernel that
+// allocates tensor memory calls it after its allocation, never before: a dependent's CTA waits for this whole grid while it
+// holds columns of its own, so if it could get them while a CTA of this grid still waits for columns, both would wait for
+// good (the order among waiting allocations is not defined).
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------- tensor memory
 __device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols)

@@ -174,7 +174,6 @@ __global__ void __launch_bounds__(192, 1)
                    const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_sp,
                    const __grid_constant__ CUtensorMap map_sq) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr uint32_t kPBytes = 128 * 128, kTileBytes = 512u * tiles_of(KIND);
   const uint32_t ctl = smem_addr(smem_raw);
   const uint32_t ring = (ctl + kCtl + 1023u) & ~1023u;
@@ -217,6 +216,7 @@ __global__ void __launch_bounds__(192, 1)
   if (warp == 1) {
     tmem_alloc(ctl + O_TMEM, p.tmem_cols);
     tmem_relinquish();
+    launch_dependents();
   }
   __syncwarp();
   tc_fence_before();
@@ -377,7 +377,6 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
                         const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_sp,
                         const __grid_constant__ CUtensorMap map_sq, const __grid_constant__ CUtensorMap map_c) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr uint32_t kPBytes = 128 * 128, kTileBytes = 512u * tiles_of(KIND);
   const uint32_t ctl = smem_addr(smem_raw);
   const uint32_t ring = (ctl + kCtl + 1023u) & ~1023u;
@@ -409,6 +408,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
   if (warp == 1) {
     tmem_alloc_pair(ctl + O_TMEM, p.tmem_cols);
     tmem_relinquish_pair();
+    launch_dependents();
   }
   __syncwarp();
   tc_fence_before();

@@ -190,6 +190,22 @@ def test_fake_tensors_leave_nothing_behind(monkeypatch):
             d.update(b)
 
 
+def test_dependents_are_launched_after_the_tensor_memory_is_allocated():
+    """A dependent's CTA holds tensor memory while it waits for the whole grid before it. Were it let in while a CTA of that
+    grid still waits for columns, the two could wait for each other for good, so the signal has to stand after the
+    allocation in every kernel that has one, and nowhere else."""
+    for f in sorted(build.CSRC.glob("*.cu")):
+        text = re.sub(r"//[^\n]*", "", f.read_text())
+        kernels = re.split(r"\b__global__\b", text)[1:]
+        for k in kernels:
+            allocations = [m.start() for m in re.finditer(r"\btmem_alloc(?:_pair)?\(", k)]
+            signals = [m.start() for m in re.finditer(r"launch_dependents", k)]
+            assert bool(signals) == bool(allocations), f.name
+            assert not signals or min(signals) > max(allocations), f.name
+    asm = [f.name for f in sorted(build.CSRC.iterdir()) if "griddepcontrol.launch_dependents" in f.read_text()]
+    assert asm == ["b2g_ptx.cuh"]
+
+
 # ---------------------------------------------------------------- the oracle
 def test_oracle_codes_by_hand():
     x = np.zeros((1, 64))

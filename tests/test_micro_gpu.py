@@ -935,3 +935,39 @@ def test_gate_gradient_of_large_and_small_factors(dtype):
         near = np.abs(r) + bound > 0.99 * top  # may round to the largest value or to an infinity
         assert (np.isinf(y[out]) & (np.sign(y[out]) == np.sign(r[out]))).all()
         assert (np.abs(y - r)[~near] <= bound[~near]).all() and not np.isnan(y).any()
+
+
+# ---------------------------------------------------------------- both families on one stream
+def test_products_and_gemms_in_turn():
+    """Products and fp16 GEMMs follow one another as programmatic dependents, each with tensor memory of its own (half of it
+    or all, one or two CTAs to an SM), back to back and from a graph: everything is what each gives alone."""
+    from cs464_b200.gate import make_inputs
+    from cs464_b200.matmul import B200Matmul, MatmulConfig
+    runs = []
+    for cfg in (MatmulConfig(128, 256, 64, num_stages=2, PERSISTENT=0), MatmulConfig(128, 64, 64, num_stages=4, PERSISTENT=0),
+                MatmulConfig(256, 256, 64, num_stages=4, CLUSTER=2), MatmulConfig(16, 128, 128, num_stages=4, SPLIT_K=4)):
+        m = 16 if cfg.BLOCK_M == 16 else 512
+        runs.append(B200Matmul(cfg).make_runner(*make_inputs(m, 9600, 512)))
+    for fmt, m, n, k in (("mxfp8", 128, 9600, 512), ("nvfp4", 16, 19200, 256), ("mxfp4", 1, 4096, 4096), ("nvfp4", 512, 9600, 512)):
+        runs.append(micro.MicroMatmul().make_runner(random_operand(m, k, fmt, 1)[0], random_operand(n, k, fmt, 2)[0]))
+    want = []
+    for r in runs:
+        want.append(r().clone())
+        torch.cuda.synchronize()
+    order = torch.randint(len(runs), (400,), generator=torch.Generator().manual_seed(0)).tolist()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i in order:
+            runs[i]()
+
+    def eager():
+        for i in order:
+            runs[i]()
+    for go in (eager, graph.replay):
+        for r in runs:
+            r.c.zero_()
+        go()
+        torch.cuda.synchronize()
+        for r, w in zip(runs, want):
+            r.raise_on_status()
+            assert torch.equal(r.c, w)
