@@ -37,7 +37,7 @@ EXPORTS = (
 # every symbol include/b2g_micro.h declares
 MICRO_EXPORTS = (
     "b2g_micro_layout", "b2g_micro_tensor_scale", "b2g_micro_quantize", "b2g_micro_dequantize", "b2g_micro_plan_create",
-    "b2g_micro_plan_launch", "b2g_micro_plan_destroy", "b2g_micro_matmul", "b2g_micro_matmul_values_workspace",
+    "b2g_micro_plan_launch", "b2g_micro_plan_wait_limit", "b2g_micro_plan_destroy", "b2g_micro_matmul", "b2g_micro_matmul_values_workspace",
     "b2g_micro_matmul_values", "b2g_micro_rms_norm",
     "b2g_micro_rms_norm_workspace", "b2g_micro_rms_norm_backward", "b2g_micro_silu_mul", "b2g_micro_silu_mul_backward",
 )
@@ -133,6 +133,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b2g_micro_dequantize": (c_int32, [mt, mm, c_int32, c_void_p]),
         "b2g_micro_plan_create": (c_int32, [mt, mt, c_void_p, i64, c_int32, c_void_p, P(c_void_p)]),
         "b2g_micro_plan_launch": (c_int32, [c_void_p, c_void_p]),
+        "b2g_micro_plan_wait_limit": (c_int32, [c_void_p, c_int32]),
         "b2g_micro_plan_destroy": (c_int32, [c_void_p]),
         "b2g_micro_matmul": (c_int32, [mt, mt, c_void_p, i64, c_int32, c_void_p, c_void_p]),
         "b2g_micro_matmul_values_workspace": (c_int32, [c_int32, i64, i64, i64, P(c_size_t)]),

@@ -15,7 +15,11 @@
 // mxfp8 690 (2.8).
 // With its loads, scales or stores left out the last shape's nvfp4 time falls by some 100, 55 and 45 us: the MMAs alone take
 // 244 us, and shared memory's bandwidth, which they share with the copies in and out, is what is between.
-// Every wait is bounded as in b2g_gemm.cu: on expiry the status word gets a code and the CTA drains and returns.
+// Every wait on an mbarrier is bounded as in b2g_gemm.cu (1 s; less where a plan of single CTAs sets it): on expiry the
+// status word gets a code, the CTA's other roles stop, its copies and MMAs in flight land (waits of 50 ms each at most)
+// and it returns without storing. The allocation of tensor memory and the cluster barriers have no limit of their own: the
+// first ends because whoever holds columns runs to its end (launch_dependents), the second because every thread of every
+// CTA reaches them after bounded waits.
 
 #include <cuda.h>
 
@@ -31,7 +35,7 @@ namespace micro {
 
 constexpr uint32_t kCtl = 1024;                       // barriers and flags in front of the ring
 constexpr int kMaxStages = 16;
-constexpr uint64_t kWaitNs = 1000000000ull;           // 1 s per wait: far above any legal stall
+constexpr uint64_t kWaitNs = 1000000000ull;           // 1 s per wait unless the plan sets less: far above any legal stall
 constexpr uint64_t kDrainNs = 50000000ull;            // 50 ms to drain in-flight work after an abort
 constexpr uint32_t kMaxSmem = 232448;                 // sm_100 opt-in maximum dynamic shared memory per block
 constexpr int kStepsPerStage = 4;                     // MMAs of 32 bytes of K in a 128-byte stage
@@ -64,15 +68,23 @@ struct Params {
   int32_t out_bf16, vec;             // vec: C's rows can be stored in 16-byte pieces
   const float *scale_a, *scale_b;    // NVFP4 tensor scales
   int* status;
+  uint64_t wait_ns;
 };
 
-__device__ __noinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int* status, int code) {
+// The slow path suspends in slices of at most a quarter of the limit and at most 1 ms, so the limit holds to within one.
+__device__ __forceinline__ uint32_t wait_slice(uint64_t limit_ns) {
+  return static_cast<uint32_t>(limit_ns / 4 < 1000000ull ? limit_ns / 4 : 1000000ull);
+}
+
+__device__ __noinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int* status,
+                                        uint64_t limit_ns, int code) {
   if (mbar_try_wait(bar, parity)) return true;
+  const uint32_t slice = wait_slice(limit_ns);
   const uint64_t t0 = global_timer_ns();
   for (;;) {
-    if (mbar_try_wait_hint(bar, parity, 1000000u)) return true;
+    if (mbar_try_wait_hint(bar, parity, slice)) return true;
     if (*abort_flag) return false;
-    if (global_timer_ns() - t0 > kWaitNs) {
+    if (global_timer_ns() - t0 > limit_ns) {
       *abort_flag = 1u;
       if (status) atomicCAS(status, 0, code);
       return false;
@@ -84,13 +96,15 @@ __device__ __noinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile 
 // descriptor of the warp's loop, uniform in the compiler's eyes. Operands of tcgen05 instructions come from uniform
 // registers; from per-thread ones each costs a move of tens of cycles, and the issue, not the tensor core, sets the
 // pace.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int* status, int code) {
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int* status,
+                                          uint64_t limit_ns, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint32_t slice = wait_slice(limit_ns);
   const uint64_t t0 = global_timer_ns();
   for (;;) {
-    if (__all_sync(0xffffffffu, mbar_try_wait_hint(bar, parity, 1000000u))) return true;
+    if (__all_sync(0xffffffffu, mbar_try_wait_hint(bar, parity, slice))) return true;
     if (__any_sync(0xffffffffu, *abort_flag != 0u)) return false;
-    if (__any_sync(0xffffffffu, global_timer_ns() - t0 > kWaitNs)) {
+    if (__any_sync(0xffffffffu, global_timer_ns() - t0 > limit_ns)) {
       *abort_flag = 1u;
       if (status) atomicCAS(status, 0, code);
       return false;
@@ -225,31 +239,20 @@ __global__ void __launch_bounds__(192, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + O_TMEM);
 
+  int issued = 1;  // by thread 0: stages whose copies went out
   if (warp == 0) {
     if (lane == 0) {  // TMA producer; the first stage is under way
-      int s = 1, issued = 1;
+      int s = 1;
       uint32_t ph = 0;
-      bool ok = true;
       for (int kb = kb0 + 1; kb < kb1; ++kb) {
         const uint32_t empty = ctl + O_EMPTY + 8 * s;
-        if (!mbar_try_wait(empty, ph ^ 1u) && !wait_phase(empty, ph ^ 1u, abort_flag, p.status, kProducerTimeout)) {
-          ok = false;
+        if (!mbar_try_wait(empty, ph ^ 1u) && !wait_phase(empty, ph ^ 1u, abort_flag, p.status, p.wait_ns, kProducerTimeout))
           break;
-        }
         load_stage(s, kb);
         ++issued;
         if (++s == p.stages) {
           s = 0;
           ph ^= 1u;
-        }
-      }
-      if (!ok) {  // let the copies already issued land before shared memory is released
-        for (int i = min(issued, p.stages); i > 0; --i) {
-          if (--s < 0) {
-            s = p.stages - 1;
-            ph ^= 1u;
-          }
-          drain_phase(ctl + O_FULL + 8 * s, ph, kDrainNs);
         }
       }
     }
@@ -264,7 +267,7 @@ __global__ void __launch_bounds__(192, 1)
     bool ok = true;
     for (int kb = kb0; kb < kb1; ++kb) {
       const uint32_t full = ctl + O_FULL + 8 * s;
-      if (!warp_wait(full, ph, abort_flag, p.status, kMmaTimeout)) {
+      if (!warp_wait(full, ph, abort_flag, p.status, p.wait_ns, kMmaTimeout)) {
         ok = false;
         break;
       }
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(192, 1)
     // Epilogue, part one: this split's fp32 tile into shared memory as [column j][row i] (128 + 4 floats a column: 32
     // lanes store 32 consecutive words). The ring is free: every MMA has completed.
     const int q = warp & 3;
-    if (wait_phase(ctl + O_TFULL, 0u, abort_flag, p.status, kEpilogueTimeout)) {
+    if (wait_phase(ctl + O_TFULL, 0u, abort_flag, p.status, p.wait_ns, kEpilogueTimeout)) {
       tc_fence_after();
       const int i = q * 32 + lane;
       for (int c = 0; c < p.tile_q; c += 32) {
@@ -304,11 +307,12 @@ __global__ void __launch_bounds__(192, 1)
   }
   // Part two: CTA r of the cluster adds its share of the tile over the cluster's CTAs in split order, scales, converts
   // and stores, a lane four consecutive values (a warp's loads of other CTAs' memory are whole lines that way). Every
-  // thread of every CTA reaches both barriers.
+  // thread of every CTA reaches both barriers. A CTA that gave up stores nothing.
   __syncwarp();
   if (p.split > 1) cluster_sync();
   else __syncthreads();
-  {
+  const bool gave_up = *abort_flag != 0u;
+  if (!gave_up) {
     const float2 alpha = output_scale(p);
     const int cols = min(p.tile_q, p.rows_q - tq * p.tile_q);  // columns of the tile inside C^T
     const int groups = cols * 32;  // of four values
@@ -348,6 +352,12 @@ __global__ void __launch_bounds__(192, 1)
   if (p.split > 1) cluster_sync();  // a CTA's shared memory stays until its peers have read it
   else __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, p.tmem_cols);
+  if (gave_up && threadIdx.x == 0) {
+    // Shared memory is released when this thread ends: whichever role gave up, every copy that went out lands first. The
+    // last one filled stage (issued - 1) mod stages, in lap (issued - 1) / stages.
+    for (int i = issued - 1; i >= 0 && i >= issued - p.stages; --i)
+      drain_phase(ctl + O_FULL + 8 * (i % p.stages), static_cast<uint32_t>(i / p.stages) & 1u, kDrainNs);
+  }
 }
 
 // ---------------------------------------------------------------- CTA pairs
@@ -428,7 +438,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
         pair_tile(p, t, tp, tq);
         for (int kb = kb0; kb < kb1; ++kb) {
           const uint32_t empty = ctl + O_EMPTY + 8 * s, full = full0 + 8 * s;
-          if (!mbar_try_wait(empty, ph ^ 1u) && !wait_phase(empty, ph ^ 1u, abort_flag, p.status, kProducerTimeout)) {
+          if (!mbar_try_wait(empty, ph ^ 1u) && !wait_phase(empty, ph ^ 1u, abort_flag, p.status, p.wait_ns, kProducerTimeout)) {
             ok = false;
             break;
           }
@@ -471,7 +481,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
       for (int t = first; ok && t < p.units; t += step) {
-        if (!warp_wait(ctl + O_TEMPTY, acc_ph ^ 1u, abort_flag, p.status, kMmaTimeout)) {
+        if (!warp_wait(ctl + O_TEMPTY, acc_ph ^ 1u, abort_flag, p.status, p.wait_ns, kMmaTimeout)) {
           ok = false;
           break;
         }
@@ -479,7 +489,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
         tc_fence_after();
         for (int kb = kb0; kb < kb1; ++kb) {
           const uint32_t full = ctl + O_FULL + 8 * s;
-          if (!warp_wait(full, ph, abort_flag, p.status, kMmaTimeout)) {
+          if (!warp_wait(full, ph, abort_flag, p.status, p.wait_ns, kMmaTimeout)) {
             ok = false;
             break;
           }
@@ -511,7 +521,7 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
     for (int t = first; t < p.units; t += step) {
       int tp, tq;
       pair_tile(p, t, tp, tq);
-      if (!wait_phase(ctl + O_TFULL, ph, abort_flag, p.status, kEpilogueTimeout)) break;
+      if (!wait_phase(ctl + O_TFULL, ph, abort_flag, p.status, p.wait_ns, kEpilogueTimeout)) break;
       ph ^= 1u;
       tc_fence_after();
       if (p.split > 1) {  // the pair's only tile: this split's part of it stays in shared memory, fp32 (below)
@@ -812,6 +822,7 @@ int32_t plan_init(Plan& pl, const b2g_micro_tensor* a, const b2g_micro_tensor* b
   p.out_bf16 = dtype == B2G_VALUE_BF16;
   p.vec = aligned16(C) && ldc % 8 == 0;
   p.status = status;
+  p.wait_ns = kWaitNs;
   if (pl.kind == FMT_NVFP4) {
     p.scale_a = a->scale;
     p.scale_b = b->scale;
@@ -997,6 +1008,20 @@ int32_t b2g_micro_plan_launch(const b2g_micro_plan* plan, void* stream) {
   return guarded([&]() -> int32_t {
     if (!plan) return record_error(B2G_ERR_INVALID_ARG, "null plan");
     return plan_launch(plan->plan, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int32_t b2g_micro_plan_wait_limit(b2g_micro_plan* plan, int32_t wait_limit_us) {
+  return guarded([&]() -> int32_t {
+    if (!plan) return record_error(B2G_ERR_INVALID_ARG, "null plan");
+    if (wait_limit_us < 0) return record_error(B2G_ERR_INVALID_ARG, "wait_limit_us must be >= 0");
+    Plan& pl = plan->plan;
+    if (pl.empty || pl.zero) return B2G_OK;  // nothing waits
+    if (wait_limit_us > 0 && (pl.pair || pl.p.split > 1))
+      return record_error(B2G_ERR_UNSUPPORTED, "wait_limit_single_cta_only: CTA pairs and the splits of a cluster keep the "
+                                               "default wait limit (an early stop cannot wait out other CTAs' copies)");
+    pl.p.wait_ns = wait_limit_us > 0 ? static_cast<uint64_t>(wait_limit_us) * 1000ull : kWaitNs;
+    return B2G_OK;
   });
 }
 

@@ -404,10 +404,12 @@ class MicroMatmul:
 
     family = "b200_sm100a_micro"
 
-    def __init__(self, dtype: torch.dtype = torch.bfloat16):
+    def __init__(self, dtype: torch.dtype = torch.bfloat16, wait_limit_us: int = 0):
+        """`wait_limit_us`: limit of the kernels' bounded device waits (0: the library's default of one second); refused for
+        products that run as CTA pairs or split K over a cluster."""
         if dtype not in _HALF:
             raise TypeError(f"dtype must be float16 or bfloat16, not {dtype}")
-        self.dtype = dtype
+        self.dtype, self.wait_limit_us = dtype, int(wait_limit_us)
 
     def make_runner(self, a: MicroTensor, b: MicroTensor, out: torch.Tensor | None = None) -> _MicroRunner:
         c = _output(a, b, out, self.dtype)
@@ -417,7 +419,10 @@ class MicroMatmul:
             _abi.check(_abi.load().b2g_micro_plan_create(
                 _abi.MicroTensor.from_buffer_copy(a._raw), _abi.MicroTensor.from_buffer_copy(b._raw), c.data_ptr(), _ldc(c),
                 _HALF[c.dtype], status.data_ptr(), ctypes.byref(plan)), "b2g_micro_plan_create")
-        return _MicroRunner(plan, c, status, (a, b))
+        run = _MicroRunner(plan, c, status, (a, b))
+        if self.wait_limit_us:
+            _abi.check(_abi.load().b2g_micro_plan_wait_limit(plan, self.wait_limit_us), "b2g_micro_plan_wait_limit")
+        return run
 
 
 def _values_product(a: torch.Tensor, b: torch.Tensor, fmt: int) -> torch.Tensor:

@@ -80,6 +80,10 @@ int32_t b2g_micro_plan_create(const b2g_micro_tensor* a, const b2g_micro_tensor*
                               int32_t* status, b2g_micro_plan** out);
 int32_t b2g_micro_plan_launch(const b2g_micro_plan* plan, void* stream);
 int32_t b2g_micro_plan_destroy(b2g_micro_plan* plan);
+/* Limit of the kernel's bounded waits, in microseconds (0: the default, one second). Plans that run as CTA pairs or split K
+   over a cluster keep the default: B2G_ERR_UNSUPPORTED. A launch in which a wait runs out sets the status word; what it
+   leaves in C is undefined. */
+int32_t b2g_micro_plan_wait_limit(b2g_micro_plan* plan, int32_t wait_limit_us);
 /* One-shot: plan, launch. */
 int32_t b2g_micro_matmul(const b2g_micro_tensor* a, const b2g_micro_tensor* b, void* C, int64_t ldc, int32_t dtype,
                          int32_t* status, void* stream);

@@ -206,6 +206,16 @@ def test_dependents_are_launched_after_the_tensor_memory_is_allocated():
     assert asm == ["b2g_ptx.cuh"]
 
 
+def test_wait_limit_refusals():
+    lib = _abi.load()
+    assert lib.b2g_micro_plan_wait_limit(None, 5) == _abi.B2G_ERR_INVALID_ARG and "null plan" in _abi.last_error()
+    e, plan = _tensor(rows=0, codes=None, scales=None), ctypes.c_void_p()
+    assert lib.b2g_micro_plan_create(e, _tensor(), None, 64, 1, None, ctypes.byref(plan)) == 0
+    assert lib.b2g_micro_plan_wait_limit(plan, -1) == _abi.B2G_ERR_INVALID_ARG and "wait_limit_us" in _abi.last_error()
+    assert lib.b2g_micro_plan_wait_limit(plan, 5) == 0  # an empty product: nothing waits
+    assert lib.b2g_micro_plan_destroy(plan) == 0
+
+
 # ---------------------------------------------------------------- the oracle
 def test_oracle_codes_by_hand():
     x = np.zeros((1, 64))

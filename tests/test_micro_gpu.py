@@ -971,3 +971,55 @@ def test_products_and_gemms_in_turn():
         for r, w in zip(runs, want):
             r.raise_on_status()
             assert torch.equal(r.c, w)
+
+
+# ---------------------------------------------------------------- bounded waits that run out
+TIMEOUTS = {0x101, 0x102, 0x103}
+
+
+def test_expired_wait_reports_status_and_stores_nothing():
+    """A product whose epilogue waits tens of microseconds for its tile, its waits limited to one: some wait runs out, the
+    kernel ends, C stays as it was, the status word says so, and the next products are right."""
+    (qa, a), (qb, b) = random_operand(128, 16384, "mxfp8", 1), random_operand(12800, 16384, "mxfp8", 2)
+    run = micro.MicroMatmul(wait_limit_us=1).make_runner(qa, qb)
+    for _ in range(2):  # cleared, the same runner gives up again rather than hanging
+        run.c.fill_(7.0)
+        run()
+        torch.cuda.synchronize()
+        assert run.device_status() in TIMEOUTS
+        assert bool((run.c == 7).all())
+        with pytest.raises(RuntimeError, match="status 0x10"):
+            run.raise_on_status()
+        run.status.zero_()
+    ok = micro.MicroMatmul().make_runner(qa, qb)
+    c = ok()
+    ok.raise_on_status()
+    check_product(c, a, b)
+
+
+@pytest.mark.parametrize("k", [1, 128, 384, 1500])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_expired_waits_of_short_products(fmt, k):
+    """Few K blocks: all copies are under way before any role gives up, and land before the CTA ends. Launches that gave up
+    are followed at once by products whose ring lies in the same shared memory; a launch that made it stored its result."""
+    (qa, a), (qb, b) = random_operand(128, k, fmt, 1), random_operand(12800, k, fmt, 2)
+    run, ok = micro.MicroMatmul(wait_limit_us=1).make_runner(qa, qb), micro.MicroMatmul().make_runner(qa, qb)
+    want = ok().clone()
+    check_product(want, a, b)
+    for _ in range(20):
+        run()
+        assert torch.equal(ok(), want)
+    assert run.device_status() in TIMEOUTS | {0}
+    ok.raise_on_status()
+
+
+def test_wait_limit_is_refused_for_pairs_and_splits():
+    from cs464_b200 import _abi
+    (qa, _), (qb, _), (qc, _) = (random_operand(m, 512, "mxfp8", m) for m in (300, 400, 16))
+    for a in (qa, qc):  # pairs; splits of a cluster
+        with pytest.raises(_abi.Unsupported, match="wait_limit_single_cta_only"):
+            micro.MicroMatmul(wait_limit_us=10).make_runner(a, qb)
+        micro.MicroMatmul().make_runner(a, qb)()
+    with pytest.raises(_abi.B2GError, match="wait_limit_us"):
+        micro.MicroMatmul(wait_limit_us=-1).make_runner(qa, qb)
+    micro.check_status()
