@@ -463,6 +463,20 @@ __global__ void __launch_bounds__((2 + EPI_WARPS) * 32, 1)
     }
   };
 
+  // Let the copies already issued land before shared memory is released (the leader's barriers count the pair's bytes).
+  auto drain_copies = [&]() {
+    const int pending = min(pissued, p.stages);
+    int ds = ps;
+    uint32_t dph = pph;
+    for (int i = 0; i < pending; ++i) {
+      if (--ds < 0) {
+        ds = p.stages - 1;
+        dph ^= 1u;
+      }
+      drain_phase(ctl + OFF_FULL + 8 * ds, dph, kDrainTimeoutNs);
+    }
+  };
+
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tma_a);
     tma_prefetch_desc(&tma_b);
@@ -516,20 +530,7 @@ __global__ void __launch_bounds__((2 + EPI_WARPS) * 32, 1)
     // ------------------------------------------------------------ TMA producer (every CTA loads its own tiles)
     if (lane == 0) {
       produce(0x7fffffff, PAIR ? map_to_rank(ctl + OFF_FULL, 0) : ctl + OFF_FULL);
-      if (!pok && leader) {
-        // Let the copies already issued land before shared memory is released (the leader's barriers count the
-        // pair's bytes).
-        const int pending = min(pissued, p.stages);
-        int ds = ps;
-        uint32_t dph = pph;
-        for (int i = 0; i < pending; ++i) {
-          if (--ds < 0) {
-            ds = p.stages - 1;
-            dph ^= 1u;
-          }
-          drain_phase(ctl + OFF_FULL + 8 * ds, dph, kDrainTimeoutNs);
-        }
-      }
+      if (!pok && leader) drain_copies();
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (the pair's leader issues for both)
@@ -964,6 +965,9 @@ __global__ void __launch_bounds__((2 + EPI_WARPS) * 32, 1)
     if (PAIR) tmem_dealloc_pair(tmem_base, p.tmem_cols);
     else tmem_dealloc(tmem_base, p.tmem_cols);
   }
+  // Another role gave up when every copy had gone out already: shared memory is released when this thread ends. (A pair's
+  // limit is the default one, past which no copy is still under way.)
+  if (!PAIR && threadIdx.x == 0 && *abort_flag) drain_copies();
 }
 
 // dst[o * ld + i] = src[o * s_outer + i * s_inner] for o < outer, i < inner (2-byte elements). Stages an operand TMA

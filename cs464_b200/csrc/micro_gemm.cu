@@ -16,8 +16,9 @@
 // With its loads, scales or stores left out the last shape's nvfp4 time falls by some 100, 55 and 45 us: the MMAs alone take
 // 244 us, and shared memory's bandwidth, which they share with the copies in and out, is what is between.
 // Every wait on an mbarrier is bounded as in b2g_gemm.cu (1 s; less where a plan of single CTAs sets it): on expiry the
-// status word gets a code, the CTA's other roles stop, its copies and MMAs in flight land (waits of 50 ms each at most)
-// and it returns without storing. The allocation of tensor memory and the cluster barriers have no limit of their own: the
+// status word gets a code, the CTA's other roles stop, its copies and MMAs in flight land (waits of 50 ms each at most; a
+// pair whose issuer gave up relies on its second of waiting for copies that the producers had sent before) and it returns
+// without storing. The allocation of tensor memory and the cluster barriers have no limit of their own: the
 // first ends because whoever holds columns runs to its end (launch_dependents), the second because every thread of every
 // CTA reaches them after bounded waits.
 

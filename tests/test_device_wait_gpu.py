@@ -61,3 +61,20 @@ def test_wait_limit_is_refused_for_cta_pairs():
     a, b = gate.make_inputs(512, 512, 512)
     with pytest.raises(_abi.Unsupported, match="wait_limit_single_cta_only"):
         B200Matmul(MatmulConfig(256, 256, 64, num_stages=6, CLUSTER=2), wait_limit_us=10).make_runner(a, b)
+
+
+@pytest.mark.parametrize("K", [64, 192, 512])
+@pytest.mark.parametrize("cfg", [MatmulConfig(128, 128, 64, num_stages=4), MatmulConfig(128, 64, 64, num_stages=8, PERSISTENT=0),
+                                 MatmulConfig(16, 128, 64, num_stages=8, PERSISTENT=0)])
+def test_expired_waits_of_short_problems(cfg, K):
+    """Few K blocks: all copies are under way before any role gives up, and land before the CTA ends. Launches that gave
+    up are followed at once by GEMMs whose ring lies in the same shared memory."""
+    a, b = gate.make_inputs(640, 2048, K)
+    run, ok = B200Matmul(cfg, wait_limit_us=1).make_runner(a, b), B200Matmul(cfg).make_runner(a, b)
+    want = ok().clone()
+    assert gate.check_norm_relative(want, gate.reference(a, b), a, b).valid
+    for _ in range(20):
+        run()
+        assert torch.equal(ok(), want)
+    assert run.device_status() in TIMEOUT_CODES | {0}
+    ok.raise_on_status()
