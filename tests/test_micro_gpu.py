@@ -1023,3 +1023,90 @@ def test_wait_limit_is_refused_for_pairs_and_splits():
     with pytest.raises(_abi.B2GError, match="wait_limit_us"):
         micro.MicroMatmul(wait_limit_us=-1).make_runner(qa, qb)
     micro.check_status()
+
+
+FAR = 540_000_000  # five rows this many values apart reach past 2^31 values
+
+
+def test_far_rows_of_every_input():
+    """Views whose last rows lie past 2^31 values (a buffer of 4.3 GB): every operator's inputs, by rows and through
+    transposes, aligned and not, against contiguous copies."""
+    for shift in (0, 1):
+        step = FAR + shift
+        base = torch.empty(4 * step + 2048, dtype=torch.bfloat16, device="cuda")
+        def far(cols, seed, at):
+            v = base.as_strided((5, cols), (step, 1), at)
+            v.copy_(normal(5, cols, seed=seed))
+            return v, v.clone()
+        (x, cx), (r, cr) = far(520, 1, 0), far(520, 2, 520)
+        (d, cd), w = far(260, 3, 1040 + 8 * shift), normal(520, seed=4)
+        for fmt in FORMATS:
+            for a, b in ((x, cx), (x.t(), cx.t())):
+                p, q = micro.quantize(a, fmt), micro.quantize(b, fmt)
+                assert torch.equal(p.codes, q.codes) and torch.equal(p.scales, q.scales)
+                assert torch.equal(p.scale, q.scale) if fmt == "nvfp4" else True
+        for a, b in ((micro.rms_norm(x, w, residual=r), micro.rms_norm(cx, w, residual=cr)),
+                     (micro.rms_norm_backward(r, x, w, dh=x), micro.rms_norm_backward(cr, cx, w, dh=cx)),
+                     ((micro.silu_mul(x), micro.silu_mul_backward(d, x)), (micro.silu_mul(cx), micro.silu_mul_backward(cd, cx)))):
+            assert all(torch.equal(s, t) for s, t in zip(a, b))
+        q = micro.quantize(cx, "nvfp4")
+        micro.dequantize(q, out=x)
+        assert torch.equal(x, q.dequantize())
+
+
+@pytest.mark.parametrize("ldc", [8, 1])
+def test_far_rows_of_products(ldc):
+    """C with its last rows past 2^31 values, of few rows (single CTAs), of many (pairs), and of few pairs' tiles with a
+    long K (splits); nothing else of the buffer is written."""
+    base = torch.zeros(2 ** 31 + 2 ** 25, dtype=torch.bfloat16, device="cuda")
+    for m, n, k in ((100, 264, 300), (300, 264, 300), (510, 200, 9000), (130, 5000, 96), (513, 2050, 9300)):
+        step = (2 ** 31 // (m - 1) // 8 + 1) * 8 + (1 if ldc == 1 else 0)
+        out = base.as_strided((m, n), (step, 1))
+        (qa, a), (qb, b) = random_operand(m, k, "nvfp4", 1), random_operand(n, k, "nvfp4", 2, std=0.05)
+        micro.micro_matmul(qa, qb, out=out)
+        check_product(out, a, b)
+        out.zero_()
+        assert not base.any()
+    micro.check_status()
+
+
+def test_outputs_past_32_bits():
+    """Codes past 2^31 bytes and outputs past 2^31 values that the operators allocate themselves (up to 40 GB here): first
+    and last rows against the same rows alone."""
+    rows, cols = 70000, 32768
+    x = torch.ones(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[:2], x[-3:] = normal(2, cols, seed=1), normal(3, cols, seed=2)
+    w = normal(cols, seed=3)
+
+    def ends(t):
+        return torch.cat([t[:2], t[-3:]])
+    few = ends(x)
+    q = micro.quantize(x, "mxfp8")
+    assert torch.equal(ends(q.codes), micro.quantize(few, "mxfp8").codes)
+    want = f64(micro.quantize(few, "mxfp8").dequantize())
+    d = q.dequantize()
+    assert torch.equal(ends(d), micro.quantize(few, "mxfp8").dequantize()) and bool((d[2:-3] == 1).all())
+    del d
+    for m in (1, 200):  # single CTAs, pairs
+        qa, a = random_operand(m, cols, "mxfp8", 4)
+        check_product(ends(micro.micro_matmul(qa, q).t()), want, a)
+        check_product(ends(micro.micro_matmul(q, qa)), want, a)
+    del q
+    y, h = micro.rms_norm(x, w, residual=x)
+    fy, fh = micro.rms_norm(few, w, residual=few)
+    assert torch.equal(ends(h), fh) and torch.equal(ends(y), fy) and torch.equal(y[2], y[-4])
+    del y, h
+    n, fn = micro.rms_norm(x, w, format="mxfp8")[0], micro.rms_norm(few, w, format="mxfp8")[0]
+    assert torch.equal(ends(n.codes), fn.codes)
+    del n
+    dx, _ = micro.rms_norm_backward(x, x, w)
+    assert torch.equal(ends(dx), micro.rms_norm_backward(few, few, w)[0])
+    del dx
+    dx = micro.silu_mul_backward(x[:, :cols // 2], x)
+    assert torch.equal(ends(dx), micro.silu_mul_backward(few[:, :cols // 2], few))
+    del dx
+    wide = x[:, None, :].expand(rows, 2, cols).reshape(rows, 2 * cols)
+    y = micro.silu_mul(wide)
+    assert torch.equal(ends(y), micro.silu_mul(ends(wide)))
+    assert torch.equal(ends(micro.silu_mul(wide, format="mxfp8").codes), micro.silu_mul(ends(wide), format="mxfp8").codes)
+    micro.check_status()
