@@ -365,20 +365,24 @@ __global__ void __launch_bounds__(256) gate_kernel(Mat x, T* y, int64_t syr, int
   store8<T, MODE>(y + row * syr, syc, c, cols, pack8<T>(v), scratch);
 }
 
-// With s = sigmoid(g): d gate = dy * up * s * (1 + g * (1 - s)), d up = dy * g * s. 1 - s is taken as sigmoid(-g),
-// which keeps its digits where s is near one. dy * up may leave fp32's range where the gradient does not (bf16's lowest
-// values among them, under a small s), and so may the small factor times the smaller of them: half the small factor meets
-// the larger one first.
+// With s = sigmoid(g): d up = dy * (g s), d gate = dy * up * (s + g s (1 - s)). 1 - s is taken as sigmoid(-g), which keeps
+// its digits where s is near one. bf16's dy * up may leave fp32's range where the gradient does not (a mask's lowest values,
+// a small s), and so may the factor times the smaller of them: half the factor meets the larger one first.
+template <typename T>
 __device__ __forceinline__ void gate_gradient(float g, float u, float d, float& dg, float& du) {
   const float2 s = sigmoids(g);
-  float larger;  // of dy's and up's magnitudes, with the product's sign
-  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(larger) : "f"(d), "f"(u));
-  const float half = s.x * fmaf(0.5f * g, s.y, 0.5f);
-  dg = half * larger * fminf(fabsf(d), fabsf(u)) * 2.f;
-  du = d * (g * s.x);
+  const float gs = g * s.x, factor = fmaf(gs, s.y, s.x);
+  du = d * gs;
+  if constexpr (std::is_same<T, __half>::value) {
+    dg = d * u * factor;
+  } else {
+    float larger;  // of dy's and up's magnitudes, with the product's sign
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(larger) : "f"(d), "f"(u));
+    dg = 0.5f * factor * larger * fminf(fabsf(d), fabsf(u)) * 2.f;
+  }
 }
 
-// Aligned rows take 32 registers a thread, so that SMs are full (36 without the bound: 45.5 us for 2048x14336).
+// Aligned rows take 32 registers a thread, so that SMs are full.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(256, MODE == kVec ? 8 : 0)
     gate_backward_kernel(Mat dy, Mat x, T* dx, int64_t sxr, int64_t sxc, int64_t rows, int64_t cols,
@@ -397,7 +401,7 @@ __global__ void __launch_bounds__(256, MODE == kVec ? 8 : 0)
   unpack8(ru, u);
   unpack8(rd, d);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) gate_gradient(g[i], u[i], d[i], dg[i], du[i]);
+  for (int i = 0; i < 8; ++i) gate_gradient<T>(g[i], u[i], d[i], dg[i], du[i]);
   T* o = dx + row * sxr;
   store8<T, MODE>(o, sxc, c, cols, pack8<T>(dg), scratch);
   store8<T, MODE>(o + cols * sxc, sxc, c, cols, pack8<T>(du), scratch);
