@@ -471,8 +471,8 @@ def micro_linear(x: torch.Tensor, w: torch.Tensor, format: str = "mxfp8") -> tor
 
 
 # ---------------------------------------------------------------- the layers between two products
-def _coded(x: torch.Tensor, cols: int, format: str, scale, grad: bool) -> MicroTensor:
-    """The MicroTensor [rows of x, cols] a layer writes to."""
+def _coded(x: torch.Tensor, rows: int, cols: int, format: str, scale, grad: bool) -> MicroTensor:
+    """The MicroTensor [rows, cols] a layer of x writes to."""
     fmt = _format(format)
     if grad:
         raise ValueError("an output in a microscaled format has no gradient: detach the inputs, or leave format out and "
@@ -483,13 +483,12 @@ def _coded(x: torch.Tensor, cols: int, format: str, scale, grad: bool) -> MicroT
         _check_scale(scale, x)
     elif scale is not None:
         raise ValueError(f"{format} has no tensor scale")
-    return MicroTensor._new(x, fmt, format, x.shape[0], cols, scale)
+    return MicroTensor._new(x, fmt, format, rows, cols, scale)
 
 
-def _norm_forward(x, residual, weight, eps, q):
+def _norm_forward(x, residual, weight, eps, q, rows, cols):
     h = x if residual is None else _like(x)
     y = _like(x) if q is None else None
-    rows, cols = x.shape
     _call(x.get_device(), _entry.rms_norm, _matrix(x), None if residual is None else _matrix(residual), weight.data_ptr(),
           None if residual is None else _matrix(h), None if y is None else _matrix(y), None if q is None else q._raw, rows,
           cols, eps, _HALF[x.dtype])
@@ -500,7 +499,7 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
         ctx.set_materialize_grads(False)
-        y, h = _norm_forward(x, residual, weight, eps, None)
+        y, h = _norm_forward(x, residual, weight, eps, None, *x.shape)
         ctx.save_for_backward(h, weight)
         ctx.eps = eps
         return y if residual is None else (y, h)
@@ -547,16 +546,17 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     grad = (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)) \
         and torch.is_grad_enabled() or forward_ad._current_level >= 0 and _has_tangent(x, weight, residual)
     weight = _weight(weight)
+    rows, cols = x2.shape
     if format is not None:
-        y, h = _norm_forward(x2, r2, weight, eps, _coded(x2, x2.shape[1], format, scale, grad))
+        y, h = _norm_forward(x2, r2, weight, eps, _coded(x2, rows, cols, format, scale, grad), rows, cols)
     elif scale is not None:
         raise ValueError("scale belongs to format='nvfp4'")
     elif grad:
         out = _Norm.apply(x2, r2, weight, eps)
         y, h = (out, x2) if residual is None else out
     else:
-        y, h = _norm_forward(x2, r2, weight, eps, None)
-    if x.dim() != 2:
+        y, h = _norm_forward(x2, r2, weight, eps, None, rows, cols)
+    if x2 is not x and x.dim() != 2:
         y = y if format is not None else y.reshape(x.shape)
         h = h.reshape(x.shape)
     return y, (x if residual is None else h)
@@ -588,8 +588,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, e
     return (dx if h.dim() == 2 else dx.reshape(h.shape)), dw
 
 
-def _gate_forward(x, q):
-    rows, cols = x.shape[0], x.shape[1] // 2
+def _gate_forward(x, q, rows, cols):
     y = x.new_empty((rows, cols)) if q is None else None
     _call(x.get_device(), _entry.silu_mul, _matrix(x), None if y is None else _matrix(y), None if q is None else q._raw,
           rows, cols, _HALF[x.dtype])
@@ -600,7 +599,7 @@ class _Gate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x):
         ctx.save_for_backward(x)
-        return _gate_forward(x, None)
+        return _gate_forward(x, None, x.shape[0], x.shape[1] // 2)
 
     @staticmethod
     @once_differentiable
@@ -620,12 +619,14 @@ def silu_mul(gate_up: torch.Tensor, format: str | None = None, scale: torch.Tens
     _gate_input(gate_up)
     x = _rows(gate_up)
     grad = gate_up.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 and _has_tangent(gate_up)
+    rows, cols = x.shape
+    cols //= 2
     if format is not None:
-        return _gate_forward(x, _coded(x, x.shape[1] // 2, format, scale, grad))
+        return _gate_forward(x, _coded(x, rows, cols, format, scale, grad), rows, cols)
     if scale is not None:
         raise ValueError("scale belongs to format='nvfp4'")
-    y = _Gate.apply(x) if grad else _gate_forward(x, None)
-    return y if gate_up.dim() == 2 else y.reshape(*gate_up.shape[:-1], x.shape[1] // 2)
+    y = _Gate.apply(x) if grad else _gate_forward(x, None, rows, cols)
+    return y if x is gate_up or gate_up.dim() == 2 else y.reshape(*gate_up.shape[:-1], cols)
 
 
 def silu_mul_backward(dy: torch.Tensor, gate_up: torch.Tensor) -> torch.Tensor:
