@@ -1110,3 +1110,72 @@ def test_outputs_past_32_bits():
     assert torch.equal(ends(y), micro.silu_mul(ends(wide)))
     assert torch.equal(ends(micro.silu_mul(wide, format="mxfp8").codes), micro.silu_mul(ends(wide), format="mxfp8").codes)
     micro.check_status()
+
+
+# ---------------------------------------------------------------- calls that the documentation allows
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_wrapped_codes_in_wider_rows(fmt):
+    """MicroTensors made of another program's bytes: rows further apart than they have to be, anything between them,
+    scales inside a larger buffer."""
+    for m, n, k in ((5, 130, 100), (300, 264, 1100), (16, 4096, 1500)):
+        wrapped, values = [], []
+        for rows, seed in ((m, 1), (n, 2)):
+            q, v = random_operand(rows, k, fmt, seed)
+            pitch = q.codes.shape[1]
+            wide = torch.full((rows, pitch + 96), 0x7F, dtype=torch.uint8, device="cuda")
+            used = k if fmt == "mxfp8" else (k + 1) // 2
+            wide[:, :used] = q.codes[:, :used]
+            buf = torch.full((q.scales.numel() + 48,), 0xFF, dtype=torch.uint8, device="cuda")
+            buf[16:-32] = q.scales
+            w = micro.MicroTensor(wide[:, :pitch], buf[16:-32], (rows, k), fmt, q.scale)
+            assert torch.equal(w.dequantize(torch.float32), q.dequantize(torch.float32))
+            assert torch.equal(w.scale_tiles().view(torch.uint8), q.scale_tiles().view(torch.uint8))
+            if fmt == "mxfp8":
+                assert torch.equal(w.code_values().view(torch.uint8), q.code_values().view(torch.uint8))
+            wrapped.append(w)
+            values.append(v)
+        check_product(micro.micro_matmul(*wrapped), *values)
+        check_product(micro.MicroMatmul().make_runner(*wrapped)(), *values)
+    micro.check_status()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_broadcast_inputs(fmt):
+    """Inputs whose rows or columns are one and the same in memory."""
+    row, col = normal(1, 200, seed=1), normal(200, 1, seed=2)
+    for x in (row.expand(70, 200), col.expand(200, 70), col.expand(200, 70).t(), row.t().expand(200, 70).t(), row[:, :1].expand(70, 200)):
+        check_quantized(micro.quantize(x, fmt), f64(x))
+    x = row.expand(70, 200)
+    assert torch.equal(micro.silu_mul(x), micro.silu_mul(x.contiguous()))
+    assert torch.equal(micro.silu_mul_backward(col[:100].t().expand(70, 100), x), micro.silu_mul_backward(col[:100].t().repeat(70, 1), x.contiguous()))
+    for got, want in ((micro.rms_norm_backward(x, x, row[0], dh=x), micro.rms_norm_backward(*[x.contiguous()] * 2, row[0], dh=x.contiguous())),
+                      (micro.rms_norm(x, row[0, :1].expand(200), residual=x), micro.rms_norm(x.contiguous(), row[0, :1].repeat(200), residual=x.contiguous()))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_mlp_of_odd_sizes_and_no_tokens(fmt, dtype):
+    hidden, ff = 200, 136
+    r = normal(2, 3, hidden, dtype=dtype, seed=1)
+    nw = normal(hidden, dtype=dtype, seed=3)
+    gu, down = micro.quantize(normal(2 * ff, hidden, seed=4, std=0.05), fmt), micro.quantize(normal(hidden, ff, seed=5, std=0.05), fmt)
+    scales = (torch.full((1,), 0.01, device="cuda"),) * 2 if fmt == "nvfp4" else None
+    y, h = micro.micro_mlp(r, None, nw, gu, down, scales=scales)
+    assert y.shape == h.shape == (2, 3, hidden) and h is r and y.dtype == dtype
+    flat, _ = micro.micro_mlp(r.view(6, hidden), None, nw, gu, down, scales=scales)
+    assert torch.equal(y.view(6, hidden), flat)
+    for i in range(6):  # a token's result does not depend on its company beyond the order of K splits, which tiles share
+        one, _ = micro.micro_mlp(r.view(6, hidden)[i:i + 1], None, nw, gu, down, scales=scales)
+        assert torch.equal(one[0], flat[i])
+    y, h = micro.micro_mlp(r[:0], r[:0], nw, gu, down, scales=scales)
+    assert y.shape == h.shape == (0, 3, hidden)
+    x = normal(0, hidden, dtype=dtype).requires_grad_()
+    w = nw.clone().requires_grad_()
+    n, _ = micro.rms_norm(x, w)
+    n.sum().backward()
+    assert x.grad.shape == x.shape and (w.grad == 0).all()
+    a, b = normal(0, 64, dtype=dtype).requires_grad_(), normal(40, 64, dtype=dtype).requires_grad_()
+    micro.micro_linear(a, b, fmt).sum().backward()
+    assert a.grad.shape == a.shape and (b.grad == 0).all()
+    micro.check_status()
