@@ -11,8 +11,8 @@
 //                        splits of a tile are one thread-block cluster and are summed through distributed shared memory.
 //   product_pair_kernel  CTA pairs (cta_group::2) of 256 x 256 tiles for products with many of them.
 // Measured: nvfp4 1x28672x4096 13.6 us (4.85 TB/s: the weights' bytes and 3 us of launch, first loads and epilogue bound
-// it), mxfp4 128x4096x14336 12.7 us; 8192x28672x4096 nvfp4 383-401 us from GPU to GPU (4.8-5.0 PFLOP/s), mxfp4 366-376,
-// mxfp8 690 (2.8).
+// it), mxfp4 128x4096x14336 12.7 us; 8192x28672x4096 nvfp4 383-408 us from GPU to GPU (4.7-5.0 PFLOP/s), mxfp4 366-376,
+// mxfp8 690 (2.8), in launches with pauses between them: back to back for seconds, under the power cap, nvfp4 takes 461.
 // With its loads, scales or stores left out the last shape's nvfp4 time falls by some 100, 55 and 45 us: the MMAs alone take
 // 244 us, and shared memory's bandwidth, which they share with the copies in and out, is what is between.
 // Every wait on an mbarrier is bounded as in b2g_gemm.cu (1 s; less where a plan of single CTAs sets it): on expiry the
@@ -739,8 +739,8 @@ int32_t init_device(int dev) {
   return B2G_OK;
 }
 
-// Clusters of 1..8 CTAs with the whole shared memory of an SM each that a B200 holds at once (a cluster lives inside a
-// GPC): a launch of more would run in waves.
+// Clusters of 1..8 CTAs with the whole shared memory of an SM each that the measured B200 holds at once (a cluster lives
+// inside a GPC): a launch of more runs in waves, with the same results.
 constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
 
 constexpr int kPairs = 74;  // CTA pairs resident at once

@@ -98,7 +98,8 @@ int32_t b2g_micro_matmul_values(const b2g_micro_matrix* A, const b2g_micro_matri
                                 void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /* h = x + residual (x alone where residual is NULL); y = h * weight / sqrt(mean(h^2) + eps) by rows of `cols`. The norm
-   is taken of the fp32 sum, before h is rounded. Outputs: h (NULL: not wanted; without a residual it is x itself and has
+   is taken of the fp32 sum, before h is rounded; squares are summed in fp32, past whose range a row's norm is infinite.
+   Outputs: h (NULL: not wanted; without a residual it is x itself and has
    to be NULL), and either y (values) or q (a
    microscaled tensor). x, residual, weight, h and y share `dtype` (F16 or BF16); weight is contiguous; cols is at most
    2^31 - 8192. */
