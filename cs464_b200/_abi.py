@@ -37,8 +37,8 @@ EXPORTS = (
 # every symbol include/b2g_micro.h declares
 MICRO_EXPORTS = (
     "b2g_micro_layout", "b2g_micro_tensor_scale", "b2g_micro_quantize", "b2g_micro_dequantize", "b2g_micro_plan_create",
-    "b2g_micro_plan_launch", "b2g_micro_plan_wait_limit", "b2g_micro_plan_destroy", "b2g_micro_matmul", "b2g_micro_matmul_values_workspace",
-    "b2g_micro_matmul_values", "b2g_micro_rms_norm",
+    "b2g_micro_plan_launch", "b2g_micro_plan_wait_limit", "b2g_micro_plan_destroy", "b2g_micro_matmul",
+    "b2g_micro_matmul_values_workspace", "b2g_micro_matmul_values", "b2g_micro_rms_norm",
     "b2g_micro_rms_norm_workspace", "b2g_micro_rms_norm_backward", "b2g_micro_silu_mul", "b2g_micro_silu_mul_backward",
 )
 

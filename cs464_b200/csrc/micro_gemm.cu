@@ -439,7 +439,8 @@ __global__ void __launch_bounds__((2 + kPairEpilogueWarps) * 32, 1)
         pair_tile(p, t, tp, tq);
         for (int kb = kb0; kb < kb1; ++kb) {
           const uint32_t empty = ctl + O_EMPTY + 8 * s, full = full0 + 8 * s;
-          if (!mbar_try_wait(empty, ph ^ 1u) && !wait_phase(empty, ph ^ 1u, abort_flag, p.status, p.wait_ns, kProducerTimeout)) {
+          if (!mbar_try_wait(empty, ph ^ 1u) &&
+              !wait_phase(empty, ph ^ 1u, abort_flag, p.status, p.wait_ns, kProducerTimeout)) {
             ok = false;
             break;
           }

@@ -21,8 +21,9 @@ All of it enqueues on the current stream of the tensors' device and allocates it
 workspace) from torch's allocator on that stream; nothing is kept between calls, nothing synchronises, and every call
 can be captured into a CUDA graph (a training step with torch's own condition: no eager autograd graph of the same
 leaves may be alive during the capture). The differentiable calls have a backward pass of first order; forward-mode
-derivatives through them are refused, and nothing is differentiable through the other calls. As elsewhere with torch, tensors made on another stream have to be ready on the
-current one. The product's kernels bound their waits: `check_status()` (from cs464_b200.matmul) raises if one ran out.
+derivatives through them are refused, and nothing is differentiable through the other calls. As elsewhere with torch,
+tensors made on another stream have to be ready on the current one. The product's kernels bound their waits:
+`check_status()` (from cs464_b200.matmul) raises if one ran out.
 
 The arithmetic of a quantisation is exact: which code and which scale a value gets follows from its bits alone
 (include/b2g_micro.h), so results do not depend on the launch. Infinities and NaN make their block's scale NaN, and with
